@@ -2,7 +2,10 @@
  * ssd_b200.h -- C ABI of libssd_b200.so: the Mamba2 SSD forward hot path on NVIDIA B200
  * (sm_100a): chunk cumsum of dt*A, per-chunk state, inter-chunk state passing, their
  * fused form, and the two chunk GEMM steps (C.B^T and the chunk scan) that the
- * end-to-end forward check needs.
+ * end-to-end forward check needs; and the operators that stand around the scan in a layer
+ * (sections 8 to 10): residual addition with the root-mean-square norm, the short causal
+ * convolution, and the token-by-token selective scan, each with its gradients or its
+ * single-token form.
  *
  * Conventions
  *   - Every pointer is a DEVICE pointer on the device that is current when the call is
@@ -43,7 +46,9 @@ typedef struct CUstream_st* ssd_stream_t; /* a cudaStream_t / CUstream handle */
 typedef enum {
   SSD_F32 = 0,
   SSD_BF16 = 1,
-  SSD_F16 = 2
+  SSD_F16 = 2,
+  SSD_I8 = 3,   /* the 8-bit outputs of ssd_add_rms_norm_fwd only */
+  SSD_E4M3 = 4
 } ssd_dtype_t;
 
 typedef enum {
@@ -410,6 +415,225 @@ typedef struct {
 } ssd_seqpar_fixup_params_t;
 
 SSD_API int ssd_seqpar_fixup(const ssd_seqpar_fixup_params_t* prm, ssd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * 8. residual addition + root-mean-square norm over the last dimension.  No counterpart in the
+ *    reference (its path begins behind a layer's input projection).
+ *      t = x + residual (fp32);  rstd = (mean(t^2) + eps)^(-1/2);  y = t * rstd * weight
+ *      residual_out = t rounded to the residual's type;  out = y rounded to x's type, or in 8 bits:
+ *      scale = max|y| / 127 (SSD_I8) or / 448 (SSD_E4M3) for each row, out = y / scale rounded.
+ *    A row of zeros has scale 0; a row that holds an infinity or a NaN has a NaN scale.
+ *    x (b, l, dim) and residual with contiguous last dimension; every output is contiguous.
+ *    out_dtype: x_dtype, SSD_I8 or SSD_E4M3.  residual_dtype: x_dtype or SSD_F32.
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  const void* x;             /* (b, l, dim) of x_dtype */
+  const void* residual;      /* (b, l, dim) of residual_dtype, or NULL */
+  const void* weight;        /* (dim,) of weight_dtype, contiguous */
+  void* out;                 /* (b, l, dim) of out_dtype */
+  void* residual_out;        /* (b, l, dim) of residual_dtype, or NULL */
+  float* rstd;               /* (b, l): (mean of the squares of t as kept, or of x + eps)^(-1/2), for the gradients */
+  float* scales;             /* (b, l); required for an 8-bit out */
+  int32_t x_dtype, residual_dtype, weight_dtype, out_dtype;
+  int32_t batch, seqlen, dim;
+  int64_t x_stride[2], residual_stride[2]; /* b, l */
+  float eps;
+} ssd_add_rms_norm_params_t;
+
+SSD_API int ssd_add_rms_norm_fwd(const ssd_add_rms_norm_params_t* prm, ssd_stream_t stream);
+
+/*    Gradients at `total`, the sum as it was kept (residual_out, or x where there is no residual):
+ *      ds = rstd * (weight * dout - total * rstd * mean(weight * dout * total * rstd)) + dresidual
+ *      dx = ds rounded to x_dtype;  dresidual_in = ds rounded to total_dtype;
+ *      dweight = sum over rows of dout * total * rstd (fp32, the same bits on every run)
+ *    total_dtype: x_dtype or SSD_F32; dout is of x_dtype.  workspace: 16-byte aligned, at least
+ *    ssd_add_rms_norm_bwd_workspace_bytes() bytes, any contents, for one call at a time. */
+typedef struct {
+  const void* dout;          /* (b, l, dim) of x_dtype */
+  const void* total;         /* (b, l, dim) of total_dtype */
+  const void* weight;        /* (dim,) of weight_dtype, contiguous */
+  const float* rstd;         /* (b, l) contiguous */
+  const void* dresidual;     /* (b, l, dim) of total_dtype, or NULL */
+  void* dx;                  /* (b, l, dim) of x_dtype, contiguous */
+  void* dresidual_in;        /* (b, l, dim) of total_dtype, contiguous, or NULL */
+  float* dweight;            /* (dim,) */
+  int32_t x_dtype, total_dtype, weight_dtype;
+  int32_t batch, seqlen, dim;
+  int64_t dout_stride[2], total_stride[2], dresidual_stride[2]; /* b, l */
+  void* workspace;
+  size_t workspace_bytes;
+} ssd_add_rms_norm_bwd_params_t;
+
+SSD_API size_t ssd_add_rms_norm_bwd_workspace_bytes(const ssd_add_rms_norm_bwd_params_t* prm);
+SSD_API int ssd_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t* prm, ssd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * 9. short causal convolution over the sequence, one filter for each channel.  No counterpart in
+ *    the reference.
+ *      pre[t, c] = bias[c] + sum_{k < width} weight[c, k] * x[t - (width - 1) + k, c]
+ *      out = pre, or pre * sigmoid(pre) with `silu`
+ *    Positions before the first are initial_states (b, width - 1, c), oldest first, or zero.  With
+ *    seq_idx a tap that would see a position of another sequence sees zero; the initial states
+ *    belong to sequence 0, as in the chunk kernels.  final_states: the last width - 1 inputs in the
+ *    same layout (zero where they belong to another sequence than the last position).
+ *    width 2 to 4; x with contiguous channels; out and the states contiguous.
+ * ---------------------------------------------------------------------------------- */
+typedef struct {
+  const void* x;             /* (b, l, c) of x_dtype */
+  const void* weight;        /* (c, width) of weight_dtype, contiguous */
+  const void* bias;          /* (c,) of bias_dtype, contiguous, or NULL */
+  const void* initial_states; /* (b, width - 1, c) of x_dtype, contiguous, or NULL */
+  const int32_t* seq_idx;    /* (b, l) or NULL */
+  void* out;                 /* (b, l, c) of x_dtype, contiguous */
+  void* final_states;        /* (b, width - 1, c) of x_dtype, contiguous, or NULL */
+  int32_t x_dtype, weight_dtype, bias_dtype;
+  int32_t batch, seqlen, channels, width;
+  int32_t silu;
+  int64_t x_stride[2];       /* b, l */
+  int64_t seq_idx_stride[2]; /* b, l */
+} ssd_short_conv_params_t;
+
+SSD_API int ssd_short_conv_fwd(const ssd_short_conv_params_t* prm, ssd_stream_t stream);
+
+/*    Gradients.  conv.out and conv.final_states are ignored.  dweight and dbias are fp32 and carry the
+ *    same bits on every run.  dinitial_states is written when not NULL (conv.initial_states given).
+ *    workspace: as for ssd_add_rms_norm_bwd. */
+typedef struct {
+  ssd_short_conv_params_t conv;
+  const void* dout;          /* (b, l, c) of x_dtype */
+  const void* dfinal_states; /* (b, width - 1, c) of x_dtype, contiguous, or NULL */
+  void* dx;                  /* (b, l, c) of x_dtype, contiguous */
+  float* dweight;            /* (c, width) */
+  float* dbias;              /* (c,) or NULL */
+  void* dinitial_states;     /* (b, width - 1, c) of x_dtype, contiguous, or NULL */
+  int64_t dout_stride[2];    /* b, l */
+  void* workspace;
+  size_t workspace_bytes;
+} ssd_short_conv_bwd_params_t;
+
+SSD_API size_t ssd_short_conv_bwd_workspace_bytes(const ssd_short_conv_bwd_params_t* prm);
+SSD_API int ssd_short_conv_bwd(const ssd_short_conv_bwd_params_t* prm, ssd_stream_t stream);
+
+/*    One position of each running sequence.  conv_state (slots, width - 1, c), oldest first, is
+ *    shifted by one position in place.  state_indices[i] is the slot of row i (NULL: row i uses slot
+ *    i).  A row whose index is negative or not below `slots`, or whose slot an earlier row names
+ *    too, is padding: its output is zero and no state is touched. */
+typedef struct {
+  const void* x;             /* (b, c) of x_dtype */
+  void* conv_state;          /* (slots, width - 1, c) of x_dtype */
+  const void* weight;        /* (c, width) of weight_dtype, contiguous */
+  const void* bias;          /* (c,) of bias_dtype, contiguous, or NULL */
+  const int32_t* state_indices; /* (b,) contiguous, or NULL */
+  void* out;                 /* (b, c) of x_dtype, contiguous */
+  int32_t x_dtype, weight_dtype, bias_dtype;
+  int32_t batch, slots, channels, width;
+  int32_t silu;
+  int64_t x_stride;          /* b */
+  int64_t state_stride[2];   /* slot, position */
+} ssd_short_conv_step_params_t;
+
+SSD_API int ssd_short_conv_step(const ssd_short_conv_step_params_t* prm, ssd_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * 10. selective scan, position by position, with a decay for each channel and state component (the
+ *    chunk kernels above have one for each head).  No counterpart in the reference.  Per channel d of
+ *    group g = d / (channels / ngroups):
+ *      dt' = clamp(softplus?(dt + dt_bias), dt_min, dt_max)
+ *      h[n] = exp(dt' * A[d, n]) * h[n] + dt' * x * B[g, n];   y = sum_n C[g, n] * h[n] + D[d] * x
+ *      out = y, or y * z * sigmoid(z)
+ *    h starts from initial_states or zero and stays fp32.  With seq_idx the state is dropped where
+ *    the sequence changes; initial_states belong to sequence 0.
+ *    For a later ssd_token_scan_bwd give `checkpoints` (the states before positions 0, 16, 32, ...)
+ *    and, with z, `out_x` (y before the gate).
+ *    x, dt, z with contiguous channels, B and C with contiguous state components; dt_dtype is x_dtype
+ *    or SSD_F32; dstate at most 256; every output contiguous.
+ *    workspace: 16-byte aligned, at least ssd_token_scan_workspace_bytes() bytes (may be 0), any
+ *    contents, for one call at a time.
+ * ---------------------------------------------------------------------------------- */
+#define SSD_TOKEN_SCAN_CHECKPOINT 16
+typedef struct {
+  const void* x;             /* (b, l, d) of x_dtype */
+  const void* dt;            /* (b, l, d) of dt_dtype */
+  const void* A;             /* (d, n) of A_dtype, contiguous */
+  const void* B;             /* (b, l, g, n) of x_dtype */
+  const void* C;             /* (b, l, g, n) of x_dtype */
+  const void* D;             /* (d,) of D_dtype, contiguous, or NULL */
+  const void* z;             /* (b, l, d) of x_dtype, or NULL */
+  const void* dt_bias;       /* (d,) of bias_dtype, contiguous, or NULL */
+  const void* initial_states; /* (b, d, n) of init_dtype, contiguous, or NULL */
+  const int32_t* seq_idx;    /* (b, l) or NULL */
+  void* out;                 /* (b, l, d) of x_dtype */
+  void* out_x;               /* (b, l, d) of x_dtype, or NULL */
+  float* final_states;       /* (b, d, n) */
+  float* checkpoints;        /* (b, ceil(l / SSD_TOKEN_SCAN_CHECKPOINT), d, n), or NULL */
+  int32_t x_dtype, dt_dtype, A_dtype, D_dtype, bias_dtype, init_dtype;
+  int32_t batch, seqlen, channels, ngroups, dstate;
+  int32_t dt_softplus;
+  float dt_min, dt_max;
+  int64_t x_stride[2], dt_stride[2], z_stride[2]; /* b, l */
+  int64_t B_stride[3], C_stride[3];               /* b, l, g */
+  int64_t seq_idx_stride[2]; /* b, l */
+  void* workspace;
+  size_t workspace_bytes;
+} ssd_token_scan_params_t;
+
+SSD_API size_t ssd_token_scan_workspace_bytes(const ssd_token_scan_params_t* prm);
+SSD_API int ssd_token_scan_fwd(const ssd_token_scan_params_t* prm, ssd_stream_t stream);
+
+/*    Gradients of the scan.  `scan` holds the forward call's inputs with its checkpoints and out_x
+ *    (now inputs); scan.out, scan.final_states and scan.workspace are ignored.  The parameters'
+ *    gradients are fp32; every gradient carries the same bits on every run. */
+typedef struct {
+  ssd_token_scan_params_t scan;
+  const void* dout;          /* (b, l, d) of x_dtype */
+  const float* dfinal_states; /* (b, d, n) contiguous, or NULL */
+  void* dx;                  /* (b, l, d) of x_dtype, contiguous */
+  void* ddt;                 /* (b, l, d) of dt_dtype, contiguous */
+  float* dA;                 /* (d, n) */
+  void* dB;                  /* (b, l, g, n) of x_dtype, contiguous */
+  void* dC;                  /* (b, l, g, n) of x_dtype, contiguous */
+  float* dD;                 /* (d,), required with D */
+  void* dz;                  /* (b, l, d) of x_dtype, contiguous, required with z */
+  float* ddt_bias;           /* (d,), required with dt_bias */
+  float* dinitial_states;    /* (b, d, n), or NULL */
+  int64_t dout_stride[2];    /* b, l */
+  void* workspace;
+  size_t workspace_bytes;
+} ssd_token_scan_bwd_params_t;
+
+SSD_API size_t ssd_token_scan_bwd_workspace_bytes(const ssd_token_scan_bwd_params_t* prm);
+SSD_API int ssd_token_scan_bwd(const ssd_token_scan_bwd_params_t* prm, ssd_stream_t stream);
+
+/*    One position of each running sequence.  state (slots, h, p, n) is updated in place.  Both forms of
+ *    the scan: a decay for each head (A_stride[1] = 0, x (b, h, p); continues the
+ *    final_states of the chunk kernels) and a decay for each channel and component (headdim 1).
+ *    state_indices: as for ssd_short_conv_step. */
+typedef struct {
+  void* state;               /* (slots, h, p, n) of state_dtype, n contiguous */
+  const void* x;             /* (b, h, p) of x_dtype */
+  const void* dt;            /* (b, h) of dt_dtype */
+  const void* A;             /* (h, n) of A_dtype */
+  const void* B;             /* (b, g, n) of x_dtype, n contiguous */
+  const void* C;             /* (b, g, n) of x_dtype, n contiguous */
+  const void* D;             /* (h, p) of D_dtype, or NULL */
+  const void* z;             /* (b, h, p) of x_dtype, or NULL */
+  const void* dt_bias;       /* (h,) of bias_dtype, or NULL */
+  const int32_t* state_indices; /* (b,) contiguous, or NULL */
+  void* out;                 /* (b, h, p) of x_dtype, contiguous */
+  int32_t state_dtype, x_dtype, dt_dtype, A_dtype, D_dtype, bias_dtype;
+  int32_t batch, slots, nheads, headdim, ngroups, dstate;
+  int32_t dt_softplus;
+  float dt_min, dt_max;
+  int64_t state_stride[3];   /* slot, h, p */
+  int64_t x_stride[3], z_stride[3]; /* b, h, p */
+  int64_t dt_stride[2];      /* b, h */
+  int64_t A_stride[2];       /* h, n */
+  int64_t B_stride[2], C_stride[2]; /* b, g */
+  int64_t D_stride[2];       /* h, p */
+  int64_t bias_stride;
+} ssd_token_scan_step_params_t;
+
+SSD_API int ssd_token_scan_step(const ssd_token_scan_step_params_t* prm, ssd_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -23,8 +23,11 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 
-CUDA_SOURCES = ["ssd_abi.cu", "ssd_general.cu", "ssd_fused_sm100.cu", "ssd_gemm_sm100.cu", "ssd_static_scratch.cu"]
-CUDA_HEADERS = ["ssd_common.cuh", "ssd_carry.cuh", "ssd_launch.h", "sm100_ptx.cuh", os.path.join(INCLUDE, "ssd_b200.h")]
+CUDA_SOURCES = ["ssd_abi.cu", "ssd_general.cu", "ssd_fused_sm100.cu", "ssd_gemm_sm100.cu", "ssd_static_scratch.cu",
+                "add_rms_norm.cu", "short_conv.cu", "token_scan.cu", "token_scan_bwd.cu", "token_step.cu"]
+CUDA_HEADERS = ["ssd_common.cuh", "ssd_carry.cuh", "ssd_launch.h", "sm100_ptx.cuh", "layer_common.cuh", "token_scan.cuh",
+                os.path.join(INCLUDE, "ssd_b200.h")]
+EXT_SOURCES = ["torch_ext.cpp", "torch_layer.cpp"]
 LIB = os.path.join(PKG, "libssd_b200.so")
 EXT = os.path.join(PKG, "_C.so")
 
@@ -102,17 +105,31 @@ def build_lib(force=False, verbose=False):
 def build_ext(force=False, verbose=False):
     import torch
     from torch.utils import cpp_extension as ce
-    src = os.path.join(CSRC, "torch_ext.cpp")
-    stamp = _digest([src, os.path.join(INCLUDE, "ssd_b200.h")], torch.__version__)
+    srcs = [os.path.join(CSRC, f) for f in EXT_SOURCES]
+    stamp = _digest(srcs + [os.path.join(CSRC, "torch_common.h"), os.path.join(INCLUDE, "ssd_b200.h")], torch.__version__)
     if not force and not _stale(EXT, stamp):
         return EXT
     cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
     inc = ce.include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda_home, "include"), INCLUDE]
     libdirs = ce.library_paths()
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DTORCH_EXTENSION_NAME=_C",
-           "-DTORCH_API_INCLUDE_EXTENSION_H",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), src, "-o", EXT]
-    cmd += ["-I" + p for p in inc]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)] + ["-I" + p for p in inc]
+    objs = []
+    procs = []
+    for s in srcs:
+        o = os.path.join(PKG, "build", os.path.basename(s) + ".o")
+        os.makedirs(os.path.dirname(o), exist_ok=True)
+        cmd = ["g++"] + flags + ["-c", s, "-o", o]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+        objs.append(o)
+    for cmd, pr in procs:
+        out, _ = pr.communicate()
+        if pr.returncode != 0:
+            sys.stderr.write(out)
+            raise RuntimeError("build step failed: " + " ".join(cmd))
+    cmd = ["g++", "-shared", "-o", EXT] + objs
     cmd += ["-L" + p for p in libdirs] + ["-L" + PKG]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-l:libssd_b200.so"]
     cmd += ["-Wl,-rpath,$ORIGIN"] + ["-Wl,-rpath," + p for p in libdirs]

@@ -1,0 +1,466 @@
+// Residual addition + root-mean-square norm (forward with an output in x's type or in 8 bits, gradients).
+//
+//   t = x + residual;  r = (mean t^2 + eps)^(-1/2);  y = t r w
+//   8 bits: scale = max|y| / M, q = round(y / scale), M = 127 or 448
+//
+// Both directions move every element once and compute little: the bound is memory bandwidth.  A block
+// holds a row in registers between the sum over it and the writing, so nothing is read twice.
+#include "layer_common.cuh"
+
+namespace ssd {
+namespace {
+
+constexpr int kMaxThreads = 1024;
+
+struct NormArgs {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* out;
+  void* residual_out;
+  float* rstd;
+  float* scales;
+  int weight_dtype, seqlen, dim;
+  int64_t x_sb, x_sl, r_sb, r_sl;
+  float eps;
+};
+
+// What an output element is made of: y for the input's types, y / scale for the 8-bit types.
+struct I8 {};
+struct E4M3 {};
+template <typename O> struct OutKind { static constexpr float kMost = 0.0f; };
+template <> struct OutKind<I8> { static constexpr float kMost = 127.0f; };
+template <> struct OutKind<E4M3> { static constexpr float kMost = 448.0f; };
+
+template <typename O, int V>
+__device__ __forceinline__ void store_out(void* base, int64_t idx, const float (&y)[V], float inv) {
+  if constexpr (std::is_same<O, I8>::value) {
+    Pack<int8_t, V> t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.e[i] = (int8_t)max(-127, min(127, __float2int_rn(y[i] * inv)));
+    *reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(base) + idx) = t;
+  } else if constexpr (std::is_same<O, E4M3>::value) {
+    Pack<uint8_t, V> t;
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.e[i] = __nv_cvt_float_to_fp8(y[i] * inv, __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<Pack<uint8_t, V>*>(static_cast<uint8_t*>(base) + idx) = t;
+  } else {
+    store_vec<V>(static_cast<O*>(base) + idx, y);
+  }
+}
+
+// One row per block.  VPT > 0: the row is held in registers, VPT vectors of V elements per thread;
+// VPT == 0: rows longer than the registers hold are read again (from L2) for each pass.
+template <typename T, typename R, typename O, int V, int VPT>
+__global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
+  __shared__ float slots[3][32];
+  constexpr bool kHold = VPT > 0;
+  constexpr bool kScaled = OutKind<O>::kMost > 0.0f;
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / a.seqlen), l = (int)(row - (int64_t)b * a.seqlen);
+  const T* x = static_cast<const T*>(a.x) + b * a.x_sb + l * a.x_sl;
+  const R* res = a.residual ? static_cast<const R*>(a.residual) + b * a.r_sb + l * a.r_sl : nullptr;
+  const int64_t obase = row * a.dim;
+  float t[kHold ? VPT : 1][V];
+
+  const auto fetch = [&](int col, float (&v)[V]) {
+    load_vec<V>(x + col, v);
+    if (res) {
+      float u[V];
+      load_vec<V>(res + col, u);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += u[i];
+    }
+  };
+  // two sums of squares: of t, which y is made of, and of t as it is kept, whose rstd the gradients use
+  // (they see nothing but what was kept)
+  float sum = 0.0f, kept = 0.0f;
+  constexpr bool kRounds = sizeof(R) < 4;
+  const auto square = [&](const float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      sum += v[i] * v[i];
+      if (kRounds) {
+        const float w = widen(narrow<R>(v[i]));
+        kept += w * w;
+      }
+    }
+  };
+  if (kHold) {
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int col = (k * blockDim.x + threadIdx.x) * V;
+      if (col < a.dim) {
+        fetch(col, t[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[k][i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) square(t[k]);
+  } else {
+    for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
+      fetch(col, t[0]);
+      square(t[0]);
+    }
+  }
+  if (kRounds) {
+    block_reduce2(sum, kept, slots);
+  } else {
+    kept = sum = block_reduce<false>(sum, slots[0]);
+  }
+  const float r = rsqrtf(sum / (float)a.dim + a.eps);
+  if (threadIdx.x == 0) a.rstd[row] = rsqrtf(kept / (float)a.dim + a.eps);
+
+  // y of one vector; `keep` writes the sum beside it
+  const auto finish = [&](int col, float (&v)[V], bool keep) {
+    if (keep && a.residual_out) store_vec<V>(static_cast<R*>(a.residual_out) + obase + col, v);
+    float w[V];
+    load_param<V>(a.weight, a.weight_dtype, col, w);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = v[i] * r * w[i];
+  };
+  if constexpr (!kScaled) {
+    if (kHold) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        const int col = (k * blockDim.x + threadIdx.x) * V;
+        if (col < a.dim) {
+          finish(col, t[k], true);
+          store_out<O, V>(a.out, obase + col, t[k], 0.0f);
+        }
+      }
+    } else {
+      for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
+        fetch(col, t[0]);
+        finish(col, t[0], true);
+        store_out<O, V>(a.out, obase + col, t[0], 0.0f);
+      }
+    }
+  } else {
+    float most = 0.0f;
+    if (kHold) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        const int col = (k * blockDim.x + threadIdx.x) * V;
+        if (col < a.dim) {
+          finish(col, t[k], true);
+#pragma unroll
+          for (int i = 0; i < V; ++i) most = combine<true>(most, fabsf(t[k][i]));
+        }
+      }
+    } else {
+      for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
+        fetch(col, t[0]);
+        finish(col, t[0], true);
+#pragma unroll
+        for (int i = 0; i < V; ++i) most = combine<true>(most, fabsf(t[0][i]));
+      }
+    }
+    most = block_reduce<true>(most, slots[2]);
+    // an infinite y has no scale either: infinity becomes the NaN that marks such a row
+    const float scale = most <= 3.4028235e38f ? most / OutKind<O>::kMost : __int_as_float(0x7fc00000);
+    if (threadIdx.x == 0) a.scales[row] = scale;
+    // zero for a row of zeros; finite for the smallest rows
+    const float inv = most > 0.0f ? fminf(OutKind<O>::kMost / most, 3.4028235e38f) : 0.0f;
+    if (kHold) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) {
+        const int col = (k * blockDim.x + threadIdx.x) * V;
+        if (col < a.dim) store_out<O, V>(a.out, obase + col, t[k], inv);
+      }
+    } else {
+      for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
+        fetch(col, t[0]);
+        finish(col, t[0], false);
+        store_out<O, V>(a.out, obase + col, t[0], inv);
+      }
+    }
+  }
+}
+
+int round_up(int v, int m) { return (v + m - 1) / m * m; }
+
+// Threads and vectors per thread of a row of `nvec` vectors: `most` vectors per thread at most (the
+// registers they take); 0 vectors per thread where the row does not fit a block's registers.
+void row_shape(int nvec, int64_t rows, int most, int* threads, int* vpt) {
+  int v = 1;
+  // few rows: one vector per thread, the shortest way through a row.  Many rows: blocks of about 256
+  // threads, so that several rows are in flight on an SM and one row's sums hide behind another's loads.
+  const int want = rows >= 2 * 148 ? 256 : kMaxThreads;
+  while (v < most && (nvec + v - 1) / v > want) v *= 2;
+  *vpt = v;
+  *threads = round_up((nvec + v - 1) / v, 32);
+  if (*threads > kMaxThreads) {
+    *vpt = 0;
+    *threads = 512;
+  }
+}
+
+template <typename T, typename R, typename O, int V>
+int launch_norm_v(const NormArgs& a, int64_t rows, cudaStream_t stream) {
+  int threads, vpt;
+  row_shape((a.dim + V - 1) / V, rows, V == 8 ? 4 : 8, &threads, &vpt);
+  const unsigned grid = (unsigned)rows;
+  switch (vpt) {
+    case 1: add_rms_norm_kernel<T, R, O, V, 1><<<grid, threads, 0, stream>>>(a); break;
+    case 2: add_rms_norm_kernel<T, R, O, V, 2><<<grid, threads, 0, stream>>>(a); break;
+    case 4: add_rms_norm_kernel<T, R, O, V, 4><<<grid, threads, 0, stream>>>(a); break;
+    case 8:
+      if constexpr (V < 8) add_rms_norm_kernel<T, R, O, V, 8><<<grid, threads, 0, stream>>>(a);
+      break;
+    default: add_rms_norm_kernel<T, R, O, V, 0><<<grid, threads, 0, stream>>>(a); break;
+  }
+  SSD_CUDA_OK(cudaGetLastError());
+  return SSD_OK;
+}
+
+template <typename T, typename R, typename O>
+int launch_norm(const NormArgs& a, const ssd_add_rms_norm_params_t& p, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t rows = (int64_t)p.batch * p.seqlen;
+  const bool vec = p.dim % V == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), 16) && aligned_to(p.out, V) &&
+                   (sizeof(O) == 1 || aligned_to(p.out, 16)) &&
+                   (p.residual == nullptr || rows_aligned(p.residual, p.residual_stride, 2, sizeof(R), 16)) &&
+                   (p.residual_out == nullptr || aligned_to(p.residual_out, 16));
+  return vec ? launch_norm_v<T, R, O, V>(a, rows, stream) : launch_norm_v<T, R, O, 1>(a, rows, stream);
+}
+
+// =====================================================================================================
+// gradients
+// =====================================================================================================
+struct NormBwdArgs {
+  const void* dout;
+  const void* total;
+  const void* weight;
+  const float* rstd;
+  const void* dresidual;
+  void* dx;
+  void* dresidual_in;
+  float* partial;      // (grid, dim)
+  int weight_dtype, seqlen, dim;
+  int64_t rows;
+  int64_t d_sb, d_sl, t_sb, t_sl, r_sb, r_sl;
+};
+
+// A block walks rows blockIdx.x, + gridDim.x, ...; each thread keeps its columns' share of the weight
+// gradient in registers and writes it once, as the block's row of `partial`.  The second kernel adds the
+// rows of `partial` in a fixed order, so the result does not depend on which block ran first.
+template <typename T, typename S, int V, int VPT>
+__global__ void __launch_bounds__(kMaxThreads) add_rms_norm_bwd_kernel(NormBwdArgs a) {
+  __shared__ float slots[2][32];
+  float w[VPT][V], dw[VPT][V];
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    const int col = (k * blockDim.x + threadIdx.x) * V;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[k][i] = dw[k][i] = 0.0f;
+    if (col < a.dim) load_param<V>(a.weight, a.weight_dtype, col, w[k]);
+  }
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const int b = (int)(row / a.seqlen), l = (int)(row - (int64_t)b * a.seqlen);
+    const T* dout = static_cast<const T*>(a.dout) + b * a.d_sb + l * a.d_sl;
+    const S* total = static_cast<const S*>(a.total) + b * a.t_sb + l * a.t_sl;
+    const S* dres = a.dresidual ? static_cast<const S*>(a.dresidual) + b * a.r_sb + l * a.r_sl : nullptr;
+    const float r = a.rstd[row];
+    float g[VPT][V], hat[VPT][V];
+    float sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int col = (k * blockDim.x + threadIdx.x) * V;
+      if (col < a.dim) {
+        load_vec<V>(dout + col, g[k]);
+        load_vec<V>(total + col, hat[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) g[k][i] = hat[k][i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        hat[k][i] *= r;
+        dw[k][i] += g[k][i] * hat[k][i];
+        g[k][i] *= w[k][i];
+        sum += g[k][i] * hat[k][i];
+      }
+    }
+    const float mean = block_reduce<false>(sum, slots[turn]) / (float)a.dim;
+    const int64_t obase = row * a.dim;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) {
+      const int col = (k * blockDim.x + threadIdx.x) * V;
+      if (col >= a.dim) continue;
+      float u[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[i] = 0.0f;
+      if (dres) load_vec<V>(dres + col, u);
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[i] += r * (g[k][i] - hat[k][i] * mean);
+      store_vec<V>(static_cast<T*>(a.dx) + obase + col, u);
+      if (a.dresidual_in) store_vec<V>(static_cast<S*>(a.dresidual_in) + obase + col, u);
+    }
+  }
+  float* part = a.partial + (int64_t)blockIdx.x * a.dim;
+#pragma unroll
+  for (int k = 0; k < VPT; ++k) {
+    const int col = (k * blockDim.x + threadIdx.x) * V;
+    if (col < a.dim) store_vec<V>(part + col, dw[k]);
+  }
+}
+
+// The same for rows longer than a block's registers hold: every row is read twice and the weight
+// gradient comes from a kernel of its own that walks columns.
+template <typename T, typename S>
+__global__ void __launch_bounds__(kMaxThreads) add_rms_norm_bwd_long_kernel(NormBwdArgs a) {
+  __shared__ float slots[2][32];
+  const int64_t row = blockIdx.x;
+  const int b = (int)(row / a.seqlen), l = (int)(row - (int64_t)b * a.seqlen);
+  const T* dout = static_cast<const T*>(a.dout) + b * a.d_sb + l * a.d_sl;
+  const S* total = static_cast<const S*>(a.total) + b * a.t_sb + l * a.t_sl;
+  const S* dres = a.dresidual ? static_cast<const S*>(a.dresidual) + b * a.r_sb + l * a.r_sl : nullptr;
+  const float r = a.rstd[row];
+  float sum = 0.0f;
+  for (int col = threadIdx.x; col < a.dim; col += blockDim.x)
+    sum += widen(dout[col]) * load_f(a.weight, a.weight_dtype, col) * (widen(total[col]) * r);
+  const float mean = block_reduce<false>(sum, slots[0]) / (float)a.dim;
+  for (int col = threadIdx.x; col < a.dim; col += blockDim.x) {
+    const float g = widen(dout[col]) * load_f(a.weight, a.weight_dtype, col);
+    float u = r * (g - widen(total[col]) * r * mean);
+    if (dres) u += widen(dres[col]);
+    static_cast<T*>(a.dx)[row * a.dim + col] = narrow<T>(u);
+    if (a.dresidual_in) static_cast<S*>(a.dresidual_in)[row * a.dim + col] = narrow<S>(u);
+  }
+}
+template <typename T, typename S>
+__global__ void __launch_bounds__(256) add_rms_norm_bwd_long_weight_kernel(NormBwdArgs a) {
+  const int col = blockIdx.x * blockDim.x + threadIdx.x;
+  if (col >= a.dim) return;
+  float acc = 0.0f;
+  for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    const int b = (int)(row / a.seqlen), l = (int)(row - (int64_t)b * a.seqlen);
+    acc += widen(static_cast<const T*>(a.dout)[b * a.d_sb + l * a.d_sl + col]) *
+           (widen(static_cast<const S*>(a.total)[b * a.t_sb + l * a.t_sl + col]) * a.rstd[row]);
+  }
+  a.partial[(int64_t)blockIdx.y * a.dim + col] = acc;
+}
+
+// out[c] = sum over p of partial[p][c]: 32 columns and 32 strides of rows per block, joined in a fixed order.
+__global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial, float* out, int parts, int dim) {
+  __shared__ float s[32][33];
+  const int col = blockIdx.x * 32 + threadIdx.x;
+  float acc = 0.0f;
+  if (col < dim) {
+#pragma unroll 4
+    for (int p = threadIdx.y; p < parts; p += 32) acc += partial[(int64_t)p * dim + col];
+  }
+  s[threadIdx.y][threadIdx.x] = acc;
+  __syncthreads();
+  float v = s[threadIdx.x][threadIdx.y];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  const int c = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && c < dim) out[c] = v;
+}
+
+// Rows of `partial`: as many blocks as are resident at once, two an SM, and no more than there are rows.
+int bwd_parts(int64_t rows) {
+  const int64_t most = 2 * 148;
+  return (int)(rows < most ? rows : most);
+}
+
+template <typename T, typename S, int V>
+int launch_norm_bwd_v(const NormBwdArgs& a, cudaStream_t stream) {
+  int threads, vpt;
+  row_shape((a.dim + V - 1) / V, 0, V == 8 ? 2 : 4, &threads, &vpt);
+  const int parts = bwd_parts(a.rows);
+  switch (vpt) {
+    case 1: add_rms_norm_bwd_kernel<T, S, V, 1><<<parts, threads, 0, stream>>>(a); break;
+    case 2: add_rms_norm_bwd_kernel<T, S, V, 2><<<parts, threads, 0, stream>>>(a); break;
+    case 4:
+      if constexpr (V < 8) add_rms_norm_bwd_kernel<T, S, V, 4><<<parts, threads, 0, stream>>>(a);
+      break;
+    default:
+      add_rms_norm_bwd_long_kernel<T, S><<<(unsigned)a.rows, 1024, 0, stream>>>(a);
+      SSD_CUDA_OK(cudaGetLastError());
+      add_rms_norm_bwd_long_weight_kernel<T, S><<<dim3((a.dim + 255) / 256, parts), 256, 0, stream>>>(a);
+      break;
+  }
+  SSD_CUDA_OK(cudaGetLastError());
+  return SSD_OK;
+}
+
+template <typename T, typename S>
+int launch_norm_bwd(const NormBwdArgs& a, const ssd_add_rms_norm_bwd_params_t& p, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = p.dim % V == 0 && rows_aligned(p.dout, p.dout_stride, 2, sizeof(T), 16) &&
+                   rows_aligned(p.total, p.total_stride, 2, sizeof(S), 16) && aligned_to(p.dx, 16) &&
+                   (p.dresidual == nullptr || rows_aligned(p.dresidual, p.dresidual_stride, 2, sizeof(S), 16)) &&
+                   (p.dresidual_in == nullptr || aligned_to(p.dresidual_in, 16));
+  return vec ? launch_norm_bwd_v<T, S, V>(a, stream) : launch_norm_bwd_v<T, S, 1>(a, stream);
+}
+
+}  // namespace
+
+int launch_add_rms_norm(const ssd_add_rms_norm_params_t& p, cudaStream_t stream) {
+  NormArgs a;
+  a.x = p.x;
+  a.residual = p.residual;
+  a.weight = p.weight;
+  a.out = p.out;
+  a.residual_out = p.residual_out;
+  a.rstd = p.rstd;
+  a.scales = p.scales;
+  a.weight_dtype = p.weight_dtype;
+  a.seqlen = p.seqlen;
+  a.dim = p.dim;
+  a.x_sb = p.x_stride[0], a.x_sl = p.x_stride[1];
+  a.r_sb = p.residual_stride[0], a.r_sl = p.residual_stride[1];
+  a.eps = p.eps;
+  return with_type(p.x_dtype, [&](auto t) {
+    using T = decltype(t);
+    const auto go = [&](auto r) {
+      using R = decltype(r);
+      if (p.out_dtype == SSD_I8) return launch_norm<T, R, I8>(a, p, stream);
+      if (p.out_dtype == SSD_E4M3) return launch_norm<T, R, E4M3>(a, p, stream);
+      return launch_norm<T, R, T>(a, p, stream);
+    };
+    return p.residual_dtype == SSD_F32 ? go(float()) : go(T());
+  });
+}
+
+size_t add_rms_norm_bwd_workspace(const ssd_add_rms_norm_bwd_params_t& p) {
+  return (size_t)bwd_parts((int64_t)p.batch * p.seqlen) * p.dim * sizeof(float);
+}
+
+int launch_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t& p, cudaStream_t stream) {
+  NormBwdArgs a;
+  a.dout = p.dout;
+  a.total = p.total;
+  a.weight = p.weight;
+  a.rstd = p.rstd;
+  a.dresidual = p.dresidual;
+  a.dx = p.dx;
+  a.dresidual_in = p.dresidual_in;
+  a.partial = static_cast<float*>(p.workspace);
+  a.weight_dtype = p.weight_dtype;
+  a.seqlen = p.seqlen;
+  a.dim = p.dim;
+  a.rows = (int64_t)p.batch * p.seqlen;
+  a.d_sb = p.dout_stride[0], a.d_sl = p.dout_stride[1];
+  a.t_sb = p.total_stride[0], a.t_sl = p.total_stride[1];
+  a.r_sb = p.dresidual_stride[0], a.r_sl = p.dresidual_stride[1];
+  const int rc = with_type(p.x_dtype, [&](auto t) {
+    using T = decltype(t);
+    return p.total_dtype == SSD_F32 ? launch_norm_bwd<T, float>(a, p, stream) : launch_norm_bwd<T, T>(a, p, stream);
+  });
+  if (rc != SSD_OK) return rc;
+  sum_partials_kernel<<<(p.dim + 31) / 32, dim3(32, 32), 0, stream>>>(a.partial, p.dweight, bwd_parts(a.rows), p.dim);
+  SSD_CUDA_OK(cudaGetLastError());
+  return SSD_OK;
+}
+
+}  // namespace ssd

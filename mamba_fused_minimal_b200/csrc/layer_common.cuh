@@ -1,0 +1,166 @@
+// Helpers shared by the layer operators around the scan (add_rms_norm.cu, short_conv.cu, token_scan.cu,
+// token_scan_bwd.cu, token_step.cu): vectors of elements widened to fp32, block sums, the activation
+// functions, and the deterministic second pass over partial sums.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include <type_traits>
+
+#include "ssd_common.cuh"
+#include "ssd_launch.h"
+
+namespace ssd {
+
+// ---- V consecutive elements of type T, widened to fp32 ---------------------------------------------
+template <typename T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+  T e[V];
+};
+
+__device__ __forceinline__ float widen(float v) { return v; }
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+
+template <typename T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
+template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
+
+template <int V, typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
+  const Pack<T, V> t = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = widen(t.e[i]);
+}
+template <int V, typename T>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
+  Pack<T, V> t;
+#pragma unroll
+  for (int i = 0; i < V; ++i) t.e[i] = narrow<T>(v[i]);
+  *reinterpret_cast<Pack<T, V>*>(p) = t;
+}
+
+// V parameters (weights, biases) of any of the three types, always read as V separate elements or, in
+// fp32 and aligned, as 16-byte vectors; read once per thread, so the branch costs nothing.
+template <int V>
+__device__ __forceinline__ void load_param(const void* base, int dtype, int64_t idx, float (&v)[V]) {
+  if (V % 4 == 0 && dtype == SSD_F32 && (reinterpret_cast<uintptr_t>(static_cast<const float*>(base) + idx) & 15) == 0) {
+#pragma unroll
+    for (int i = 0; i + 3 < V; i += 4) {
+      const float4 t = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + idx + i);
+      v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = load_f(base, dtype, idx + i);
+}
+
+// ---- activations -----------------------------------------------------------------------------------
+__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float silu_f(float v) { return v * sigmoid_f(v); }
+// d/dv of v * sigmoid(v)
+__device__ __forceinline__ float dsilu_f(float v) {
+  const float g = sigmoid_f(v);
+  return g * (1.0f + v * (1.0f - g));
+}
+// log(1 + exp(v)), exact to a few units in the last place also where it is small: the layer's steps
+// lie between 1e-4 and 1e-1, where log(exp(v) + 1) would keep three digits.
+__device__ __forceinline__ float softplus_f(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
+// dt' of one position and channel, and the factor of its gradient
+__device__ __forceinline__ float scan_dt(float raw, bool softplus, float lo, float hi) {
+  const float v = softplus ? softplus_f(raw) : raw;
+  return fminf(fmaxf(v, lo), hi);
+}
+
+// ---- block-wide sum and maximum --------------------------------------------------------------------
+// `slots` is shared memory for 32 floats that no other reduction in flight uses.  Every thread gets the
+// result; the order of the additions depends on the block's size alone.
+template <bool MAX>
+__device__ __forceinline__ float combine(float a, float b) {
+  if (!MAX) return a + b;
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));   // a NaN stays
+  return r;
+}
+template <bool MAX>
+__device__ __forceinline__ float block_reduce(float v, float* slots) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = combine<MAX>(v, __shfl_xor_sync(0xffffffffu, v, off));
+  const int warps = blockDim.x >> 5;
+  if (warps == 1) return v;
+  if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = slots[(threadIdx.x & 31) < warps ? (threadIdx.x & 31) : 0];
+  if (!MAX && (threadIdx.x & 31) >= warps) v = 0.0f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = combine<MAX>(v, __shfl_xor_sync(0xffffffffu, v, off));
+  return v;
+}
+
+// two sums with one barrier; slots[0] and slots[1] as above
+__device__ __forceinline__ void block_reduce2(float& u, float& v, float (*slots)[32]) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    u += __shfl_xor_sync(0xffffffffu, u, off);
+    v += __shfl_xor_sync(0xffffffffu, v, off);
+  }
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if (warps == 1) return;
+  if (lane == 0) slots[0][threadIdx.x >> 5] = u, slots[1][threadIdx.x >> 5] = v;
+  __syncthreads();
+  u = lane < warps ? slots[0][lane] : 0.0f;
+  v = lane < warps ? slots[1][lane] : 0.0f;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    u += __shfl_xor_sync(0xffffffffu, u, off);
+    v += __shfl_xor_sync(0xffffffffu, v, off);
+  }
+}
+
+// ---- the state slot of a row of a single-token call --------------------------------------------------
+// A row is padding (it gets zeros and touches no state) if its index lies outside the slots, or if an
+// earlier row names the same slot: two rows would race on it.  step_slot gives the slot or -1;
+// step_taken, called by every thread of the block behind its loads and before its stores, says whether an
+// earlier row has it: the search runs while the loads are in flight.
+__device__ __forceinline__ int step_slot(const int32_t* indices, int row, int slots) {
+  const int slot = indices == nullptr ? row : indices[row];
+  return slot < slots ? slot : -1;
+}
+__device__ __forceinline__ bool step_taken(const int32_t* indices, int row, int slot) {
+  if (indices == nullptr) return false;
+  bool taken = false;
+  for (int j = threadIdx.x; j < row; j += blockDim.x) taken |= indices[j] == slot;
+  return __syncthreads_or(taken) != 0;
+}
+
+// ---- alignment of what a vector access of `bytes` needs --------------------------------------------
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+inline bool rows_aligned(const void* p, const int64_t* stride, int n, int elem, size_t bytes) {
+  if (!aligned_to(p, bytes)) return false;
+  for (int i = 0; i < n; ++i)
+    if ((stride[i] * elem) % (int64_t)bytes != 0) return false;
+  return true;
+}
+
+// calls f with a value of the type that `dtype` names
+template <typename F>
+int with_type(int dtype, F f) {
+  switch (dtype) {
+    case SSD_BF16: return f(__nv_bfloat16());
+    case SSD_F16: return f(__half());
+    default: return f(float());
+  }
+}
+
+inline int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  return n;
+}
+
+}  // namespace ssd

@@ -1,0 +1,457 @@
+// Short causal convolution over the sequence, one filter of 2 to 4 taps for each channel: prompts,
+// gradients, single tokens.
+//
+//   pre[t] = bias + sum_j wr[j] x[t - j],  wr[j] = weight[width - 1 - j];   out = pre or silu(pre)
+//   dpre = dout * silu'(pre);  dx[s] = sum_j wr[j] dpre[s + j];  dwr[j] = sum_t dpre[t] x[t - j]
+//
+// Every element is read and written once: the bound is memory bandwidth.  Channels are contiguous, so a
+// thread owns a vector of channels and walks a strip of positions with the last width - 1 inputs in
+// registers; only a strip's first width - 1 positions are read twice.
+#include "layer_common.cuh"
+
+namespace ssd {
+namespace {
+
+constexpr int kConvThreads = 128;
+constexpr int kFwdStrip = 32;     // positions of a forward strip
+constexpr int kBwdStrip = 64;     // positions of a gradient strip: fewer partial sums of the weights
+constexpr int kAhead = 8;         // positions whose loads are in flight together
+
+struct ConvArgs {
+  const void* x;
+  const void* weight;
+  const void* bias;
+  const void* init;
+  const int32_t* seq;
+  void* out;
+  void* final_states;
+  int weight_dtype, bias_dtype;
+  int seqlen, channels;
+  int silu;
+  int64_t x_sb, x_sl, s_sb, s_sl;
+};
+
+// The sequence number of position t; positions before the first belong to sequence 0.
+__device__ __forceinline__ int seq_at(const ConvArgs& a, int64_t base, int t) { return t < 0 ? 0 : a.seq[base + (int64_t)t * a.s_sl]; }
+
+// Weights of V channels as wr[j][v], and the bias.
+template <int W, int V>
+__device__ __forceinline__ void load_filter(const void* weight, int wdt, const void* bias, int bdt, int c, float (&wr)[W][V], float (&bs)[V]) {
+  float flat[V * W];
+  load_param<V * W>(weight, wdt, (int64_t)c * W, flat);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) wr[j][v] = flat[v * W + (W - 1 - j)];
+    bs[v] = 0.0f;
+  }
+  if (bias) load_param<V>(bias, bdt, c, bs);
+}
+
+// Input of position t (t may lie before the first: initial states or zero).
+template <typename T, int W, int V>
+__device__ __forceinline__ void load_input(const ConvArgs& a, const T* x, int b, int c, int t, float (&v)[V]) {
+  if (t >= 0) {
+    load_vec<V>(x + (int64_t)t * a.x_sl, v);
+  } else if (a.init != nullptr && t >= -(W - 1)) {
+    load_vec<V>(static_cast<const T*>(a.init) + ((int64_t)b * (W - 1) + (t + W - 1)) * a.channels + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.0f;
+  }
+}
+
+template <typename T, int W, int V, bool SEQ>
+__global__ void __launch_bounds__(kConvThreads) short_conv_fwd_kernel(ConvArgs a) {
+  const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
+  if (c >= a.channels) return;
+  const int b = blockIdx.z;
+  const int t0 = blockIdx.y * kFwdStrip, t1 = min(t0 + kFwdStrip, a.seqlen);
+  const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
+  T* out = static_cast<T*>(a.out) + ((int64_t)b * a.seqlen) * a.channels + c;
+  const int64_t sbase = SEQ ? b * a.s_sb : 0;
+  float wr[W][V], bs[V];
+  load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, c, wr, bs);
+  float win[W - 1][V];                 // win[j] = x[t - 1 - j]
+  int id[W - 1];
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) {
+    load_input<T, W, V>(a, x, b, c, t0 - 1 - j, win[j]);
+    id[j] = SEQ ? seq_at(a, sbase, t0 - 1 - j) : 0;
+  }
+  for (int t = t0; t < t1; t += kAhead) {
+    float cur[kAhead][V];
+    int cid[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (t + u < t1) {
+        load_vec<V>(x + (int64_t)(t + u) * a.x_sl, cur[u]);
+        cid[u] = SEQ ? seq_at(a, sbase, t + u) : 0;
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (t + u >= t1) break;
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float acc = fmaf(wr[0][i], cur[u][i], bs[i]);
+#pragma unroll
+        for (int j = 1; j < W; ++j) {
+          // the value j positions back, masked where it belongs to another sequence (a select: what is
+          // masked may be an infinity or a NaN)
+          const float past = !SEQ || id[j - 1] == cid[u] ? win[j - 1][i] : 0.0f;
+          acc = fmaf(wr[j][i], past, acc);
+        }
+        y[i] = a.silu ? silu_f(acc) : acc;
+      }
+      store_vec<V>(out + (int64_t)(t + u) * a.channels, y);
+#pragma unroll
+      for (int j = W - 2; j > 0; --j) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j][i] = win[j - 1][i];
+        id[j] = id[j - 1];
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) win[0][i] = cur[u][i];
+      id[0] = cid[u];
+    }
+  }
+  if (a.final_states != nullptr && t1 == a.seqlen) {
+    T* fin = static_cast<T*>(a.final_states) + (int64_t)b * (W - 1) * a.channels + c;
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {          // win[j] = x[seqlen - 1 - j]
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = !SEQ || id[j] == id[0] ? win[j][i] : 0.0f;
+      store_vec<V>(fin + (int64_t)(W - 2 - j) * a.channels, v);
+    }
+  }
+}
+
+// ---- gradients --------------------------------------------------------------------------------------
+struct ConvBwdArgs {
+  ConvArgs f;
+  const void* dout;
+  const void* dfinal;
+  void* dx;
+  void* dinit;
+  float* partial;      // (strips, width + 1, channels): the strip's share of dwr[0..width-1] and dbias
+  int64_t d_sb, d_sl;
+};
+
+// A strip walks its positions and the width - 1 behind it (whose dpre its last dx need); dx of a
+// position is complete once dpre of the width - 1 positions after it is known.
+template <typename T, int W, int V, bool SEQ>
+__global__ void __launch_bounds__(kConvThreads) short_conv_bwd_kernel(ConvBwdArgs g) {
+  const ConvArgs& a = g.f;
+  const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
+  if (c >= a.channels) return;
+  const int b = blockIdx.z;
+  const int t0 = blockIdx.y * kBwdStrip, t1 = min(t0 + kBwdStrip, a.seqlen);
+  const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
+  const T* dout = static_cast<const T*>(g.dout) + b * g.d_sb + c;
+  T* dx = static_cast<T*>(g.dx) + ((int64_t)b * a.seqlen) * a.channels + c;
+  const int64_t sbase = SEQ ? b * a.s_sb : 0;
+  const int last_id = SEQ ? seq_at(a, sbase, a.seqlen - 1) : 0;
+  float wr[W][V], bs[V];
+  load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, c, wr, bs);
+  float win[W][V], dp[W][V], dw[W][V], db[V];       // win[j] = x[t - j], dp[j] = dpre[t - j]
+  int id[W];
+  const bool first = t0 == 0;
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) dp[j][i] = dw[j][i] = win[j][i] = 0.0f;
+    id[j] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) db[i] = 0.0f;
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) {
+    load_input<T, W, V>(a, x, b, c, t0 - 1 - j, win[j]);
+    id[j] = SEQ ? seq_at(a, sbase, t0 - 1 - j) : 0;
+  }
+  // t runs width - 1 positions past the strip, to its end or the sequence's: behind the sequence's end
+  // dpre is zero
+  for (int t = t0; t < t1 + W - 1; ++t) {
+    float in[V], d[V];
+    int now = 0;
+    const bool inside = t < a.seqlen;
+    if (inside) {
+      load_vec<V>(x + (int64_t)t * a.x_sl, in);
+      load_vec<V>(dout + (int64_t)t * g.d_sl, d);
+      now = SEQ ? seq_at(a, sbase, t) : 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) in[i] = d[i] = 0.0f;
+    }
+#pragma unroll
+    for (int j = W - 1; j > 0; --j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) win[j][i] = win[j - 1][i], dp[j][i] = dp[j - 1][i];
+      id[j] = id[j - 1];
+    }
+    id[0] = now;
+#pragma unroll
+    for (int i = 0; i < V; ++i) win[0][i] = in[i];
+    const bool own = t < t1;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float acc = fmaf(wr[0][i], in[i], bs[i]);
+#pragma unroll
+      for (int j = 1; j < W; ++j) acc = fmaf(wr[j][i], !SEQ || id[j] == now ? win[j][i] : 0.0f, acc);
+      const float v = inside ? (a.silu ? d[i] * dsilu_f(acc) : d[i]) : 0.0f;
+      dp[0][i] = v;
+      if (own) {
+        db[i] += v;
+        dw[0][i] += v * in[i];
+#pragma unroll
+        for (int j = 1; j < W; ++j) dw[j][i] += v * (!SEQ || id[j] == now ? win[j][i] : 0.0f);
+      }
+    }
+    // the position width - 1 back: dx[s] = sum_j wr[j] dpre[s + j]; s + j lies j behind s in the window
+    const int s = t - (W - 1);
+    if (s >= t0 || (first && g.dinit != nullptr)) {
+      float r[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        r[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+          // before the first position there is no dpre, and behind the last one it is zero
+          if (s + j >= 0 && s + j < a.seqlen && (!SEQ || id[W - 1] == id[W - 1 - j])) r[i] = fmaf(wr[j][i], dp[W - 1 - j][i], r[i]);
+        }
+      }
+      const int k = s - (a.seqlen - (W - 1));
+      if (g.dfinal != nullptr && k >= 0 && (!SEQ || id[W - 1] == last_id)) {
+        float u[V];
+        load_vec<V>(static_cast<const T*>(g.dfinal) + ((int64_t)b * (W - 1) + k) * a.channels + c, u);
+#pragma unroll
+        for (int i = 0; i < V; ++i) r[i] += u[i];
+      }
+      if (s >= 0)
+        store_vec<V>(dx + (int64_t)s * a.channels, r);
+      else
+        store_vec<V>(static_cast<T*>(g.dinit) + ((int64_t)b * (W - 1) + (s + W - 1)) * a.channels + c, r);
+    }
+  }
+  float* part = g.partial + ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * (W + 1)) * a.channels + c;
+#pragma unroll
+  for (int j = 0; j < W; ++j) store_vec<V>(part + (int64_t)j * a.channels, dw[j]);
+  store_vec<V>(part + (int64_t)W * a.channels, db);
+}
+
+// dweight[c][k] and dbias[c] from the strips' shares, added in a fixed order.
+template <int W>
+__global__ void __launch_bounds__(1024) short_conv_sum_kernel(const float* partial, float* dweight, float* dbias, int strips, int channels) {
+  __shared__ float s[32][33];
+  const int j = blockIdx.y;
+  const int col = blockIdx.x * 32 + threadIdx.x;
+  float acc = 0.0f;
+  if (col < channels) {
+#pragma unroll 4
+    for (int p = threadIdx.y; p < strips; p += 32) acc += partial[((int64_t)p * (W + 1) + j) * channels + col];
+  }
+  s[threadIdx.y][threadIdx.x] = acc;
+  __syncthreads();
+  float v = s[threadIdx.x][threadIdx.y];
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  const int c = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && c < channels) {
+    if (j < W)
+      dweight[(int64_t)c * W + (W - 1 - j)] = v;
+    else if (dbias != nullptr)
+      dbias[c] = v;
+  }
+}
+
+// ---- single tokens ----------------------------------------------------------------------------------
+struct ConvStepArgs {
+  const void* x;
+  void* state;
+  const void* weight;
+  const void* bias;
+  const int32_t* indices;
+  void* out;
+  int weight_dtype, bias_dtype;
+  int slots, channels;
+  int silu;
+  int64_t x_sb, st_ss, st_sp;
+};
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvStepArgs a) {
+  const int row = blockIdx.y;
+  const int slot = step_slot(a.indices, row, a.slots);
+  const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
+  const bool inside = c < a.channels;
+  T* out = static_cast<T*>(a.out) + (int64_t)row * a.channels + c;
+  T* st = static_cast<T*>(a.state) + (int64_t)max(slot, 0) * a.st_ss + c;
+  float y[V], in[V], past[W - 1][V], wr[W][V], bs[V];
+  if (inside && slot >= 0) {
+    load_vec<V>(static_cast<const T*>(a.x) + row * a.x_sb + c, in);
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) load_vec<V>(st + (int64_t)j * a.st_sp, past[j]);    // oldest first
+    load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, c, wr, bs);
+  }
+  const bool taken = step_taken(a.indices, row, slot);
+  if (!inside) return;
+  if (slot < 0 || taken) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) y[i] = 0.0f;
+    store_vec<V>(out, y);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float acc = fmaf(wr[0][i], in[i], bs[i]);
+#pragma unroll
+    for (int j = 1; j < W; ++j) acc = fmaf(wr[j][i], past[W - 1 - j][i], acc);
+    y[i] = a.silu ? silu_f(acc) : acc;
+  }
+  store_vec<V>(out, y);
+#pragma unroll
+  for (int j = 0; j < W - 2; ++j) store_vec<V>(st + (int64_t)j * a.st_sp, past[j + 1]);
+  store_vec<V>(st + (int64_t)(W - 2) * a.st_sp, in);
+}
+
+ConvArgs conv_args(const ssd_short_conv_params_t& p) {
+  ConvArgs a;
+  a.x = p.x;
+  a.weight = p.weight;
+  a.bias = p.bias;
+  a.init = p.initial_states;
+  a.seq = p.seq_idx;
+  a.out = p.out;
+  a.final_states = p.final_states;
+  a.weight_dtype = p.weight_dtype;
+  a.bias_dtype = p.bias_dtype;
+  a.seqlen = p.seqlen;
+  a.channels = p.channels;
+  a.silu = p.silu;
+  a.x_sb = p.x_stride[0], a.x_sl = p.x_stride[1];
+  a.s_sb = p.seq_idx_stride[0], a.s_sl = p.seq_idx_stride[1];
+  return a;
+}
+
+// calls f with the filter's width as a constant
+template <typename F>
+int with_width(int width, F f) {
+  switch (width) {
+    case 2: return f(std::integral_constant<int, 2>());
+    case 3: return f(std::integral_constant<int, 3>());
+    default: return f(std::integral_constant<int, 4>());
+  }
+}
+
+int strips_of(int seqlen, int strip) { return (seqlen + strip - 1) / strip; }
+
+}  // namespace
+
+int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream) {
+  const ConvArgs a = conv_args(p);
+  const int strips = strips_of(p.seqlen, kFwdStrip);
+  SSD_REQUIRE(strips <= 65535 && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv: seqlen %d or batch %d too large", p.seqlen, p.batch);
+  return with_type(p.x_dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = p.channels % V == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), 16) && aligned_to(p.out, 16) &&
+                     aligned_to(p.initial_states, 16) && aligned_to(p.final_states, 16);
+    return with_width(p.width, [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      const auto go = [&](auto v, auto s) -> int {
+        constexpr int N = decltype(v)::value;
+        const dim3 grid((p.channels + kConvThreads * N - 1) / (kConvThreads * N), strips, p.batch);
+        short_conv_fwd_kernel<T, W, N, decltype(s)::value><<<grid, kConvThreads, 0, stream>>>(a);
+        SSD_CUDA_OK(cudaGetLastError());
+        return SSD_OK;
+      };
+      const std::integral_constant<int, V> wide;
+      const std::integral_constant<int, 1> one;
+      if (p.seq_idx) return vec ? go(wide, std::true_type()) : go(one, std::true_type());
+      return vec ? go(wide, std::false_type()) : go(one, std::false_type());
+    });
+  });
+}
+
+size_t short_conv_bwd_workspace(const ssd_short_conv_bwd_params_t& p) {
+  return (size_t)p.conv.batch * strips_of(p.conv.seqlen, kBwdStrip) * (p.conv.width + 1) * p.conv.channels * sizeof(float);
+}
+
+int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& q, cudaStream_t stream) {
+  const ssd_short_conv_params_t& p = q.conv;
+  ConvBwdArgs g;
+  g.f = conv_args(p);
+  g.dout = q.dout;
+  g.dfinal = q.dfinal_states;
+  g.dx = q.dx;
+  g.dinit = q.dinitial_states;
+  g.partial = static_cast<float*>(q.workspace);
+  g.d_sb = q.dout_stride[0], g.d_sl = q.dout_stride[1];
+  const int strips = strips_of(p.seqlen, kBwdStrip);
+  SSD_REQUIRE(strips <= 65535 && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv: seqlen %d or batch %d too large", p.seqlen, p.batch);
+  return with_type(p.x_dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 4;
+    constexpr size_t kBytes = V * sizeof(T);
+    const bool vec = p.channels % V == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), kBytes) &&
+                     rows_aligned(q.dout, q.dout_stride, 2, sizeof(T), kBytes) && aligned_to(q.dx, kBytes) &&
+                     aligned_to(p.initial_states, kBytes) && aligned_to(q.dfinal_states, kBytes) && aligned_to(q.dinitial_states, kBytes);
+    return with_width(p.width, [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      const auto go = [&](auto v, auto s) -> int {
+        constexpr int N = decltype(v)::value;
+        const dim3 grid((p.channels + kConvThreads * N - 1) / (kConvThreads * N), strips, p.batch);
+        short_conv_bwd_kernel<T, W, N, decltype(s)::value><<<grid, kConvThreads, 0, stream>>>(g);
+        SSD_CUDA_OK(cudaGetLastError());
+        short_conv_sum_kernel<W><<<dim3((p.channels + 31) / 32, W + 1), dim3(32, 32), 0, stream>>>(g.partial, q.dweight, q.dbias,
+                                                                                                    strips * p.batch, p.channels);
+        SSD_CUDA_OK(cudaGetLastError());
+        return SSD_OK;
+      };
+      const std::integral_constant<int, V> wide;
+      const std::integral_constant<int, 1> one;
+      if (p.seq_idx) return vec ? go(wide, std::true_type()) : go(one, std::true_type());
+      return vec ? go(wide, std::false_type()) : go(one, std::false_type());
+    });
+  });
+}
+
+int launch_short_conv_step(const ssd_short_conv_step_params_t& p, cudaStream_t stream) {
+  ConvStepArgs a;
+  a.x = p.x;
+  a.state = p.conv_state;
+  a.weight = p.weight;
+  a.bias = p.bias;
+  a.indices = p.state_indices;
+  a.out = p.out;
+  a.weight_dtype = p.weight_dtype;
+  a.bias_dtype = p.bias_dtype;
+  a.slots = p.slots;
+  a.channels = p.channels;
+  a.silu = p.silu;
+  a.x_sb = p.x_stride;
+  a.st_ss = p.state_stride[0], a.st_sp = p.state_stride[1];
+  SSD_REQUIRE(p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv step: batch %d too large", p.batch);
+  return with_type(p.x_dtype, [&](auto t) {
+    using T = decltype(t);
+    constexpr int V = 16 / sizeof(T);
+    const bool vec = p.channels % V == 0 && rows_aligned(p.x, &p.x_stride, 1, sizeof(T), 16) &&
+                     rows_aligned(p.conv_state, p.state_stride, 2, sizeof(T), 16) && aligned_to(p.out, 16);
+    return with_width(p.width, [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      const auto go = [&](auto v) -> int {
+        constexpr int N = decltype(v)::value;
+        const dim3 grid((p.channels + kConvThreads * N - 1) / (kConvThreads * N), p.batch);
+        short_conv_step_kernel<T, W, N><<<grid, kConvThreads, 0, stream>>>(a);
+        SSD_CUDA_OK(cudaGetLastError());
+        return SSD_OK;
+      };
+      return vec ? go(std::integral_constant<int, V>()) : go(std::integral_constant<int, 1>());
+    });
+  });
+}
+
+}  // namespace ssd

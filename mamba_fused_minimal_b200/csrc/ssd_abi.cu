@@ -59,6 +59,37 @@ size_t general_states_bytes(const ssd_fused_state_params_t& p) {
   return (size_t)in.batch * nchunks * in.nheads * in.headdim * in.dstate * sizeof(float);
 }
 
+// A parameter tensor that may be absent
+bool absent_or_valid(const void* p, int dtype) { return p == nullptr || valid_dtype(dtype); }
+
+int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  if (need == 0) return SSD_OK;
+  SSD_REQUIRE(workspace != nullptr && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0, SSD_ERR_WORKSPACE,
+              "workspace is NULL or not 16-byte aligned");
+  SSD_REQUIRE(bytes >= need, SSD_ERR_WORKSPACE, "workspace holds %zu bytes, %zu needed", bytes, need);
+  return SSD_OK;
+}
+
+int check_conv(const ssd_short_conv_params_t& p) {
+  SSD_REQUIRE(p.x && p.weight, SSD_ERR_BAD_ARGUMENT, "x and weight must not be NULL");
+  SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype) && absent_or_valid(p.bias, p.bias_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.channels > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE(p.width >= 2 && p.width <= 4, SSD_ERR_UNSUPPORTED, "short conv: width %d is not 2, 3 or 4", p.width);
+  return SSD_OK;
+}
+
+int check_scan(const ssd_token_scan_params_t& p) {
+  SSD_REQUIRE(p.x && p.dt && p.A && p.B && p.C, SSD_ERR_BAD_ARGUMENT, "x, dt, A, B and C must not be NULL");
+  SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.A_dtype) && absent_or_valid(p.D, p.D_dtype) &&
+                  absent_or_valid(p.dt_bias, p.bias_dtype) && absent_or_valid(p.initial_states, p.init_dtype),
+              SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE(p.dt_dtype == p.x_dtype || p.dt_dtype == SSD_F32, SSD_ERR_UNSUPPORTED, "dt must have x's dtype or be fp32");
+  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.channels > 0 && p.ngroups > 0 && p.dstate > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE(p.channels % p.ngroups == 0, SSD_ERR_BAD_ARGUMENT, "channels %d not a multiple of ngroups %d", p.channels, p.ngroups);
+  SSD_REQUIRE(p.dstate <= 256, SSD_ERR_UNSUPPORTED, "token scan: dstate %d > 256", p.dstate);
+  return SSD_OK;
+}
+
 bool use_fast(const ssd_fused_state_params_t& p) {
   return !p.force_general && fused_fast_variant(p, nullptr) != 0;
 }
@@ -377,6 +408,126 @@ int ssd_combined_fwd(const ssd_combined_params_t* prm, ssd_stream_t stream) {
   const int rc = ssd_state_path_fwd(&prm->path, stream);
   if (rc != SSD_OK) return rc;
   return ssd_chunk_scan_fused_fwd(&prm->scan, stream);
+}
+
+int ssd_add_rms_norm_fwd(const ssd_add_rms_norm_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_add_rms_norm_fwd");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  const ssd_add_rms_norm_params_t& p = *prm;
+  SSD_REQUIRE(p.x && p.weight && p.out && p.rstd, SSD_ERR_BAD_ARGUMENT, "x, weight, out and rstd must not be NULL");
+  SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE((p.residual == nullptr && p.residual_out == nullptr) || p.residual_dtype == p.x_dtype || p.residual_dtype == SSD_F32,
+              SSD_ERR_UNSUPPORTED, "the residual must have x's dtype or be fp32");
+  SSD_REQUIRE(p.out_dtype == p.x_dtype || p.out_dtype == SSD_I8 || p.out_dtype == SSD_E4M3, SSD_ERR_UNSUPPORTED,
+              "out must have x's dtype, int8 or e4m3");
+  SSD_REQUIRE(p.out_dtype == p.x_dtype || p.scales != nullptr, SSD_ERR_BAD_ARGUMENT, "an 8-bit out needs scales");
+  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.dim > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE((int64_t)p.batch * p.seqlen <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
+  return launch_add_rms_norm(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ssd_add_rms_norm_bwd_workspace_bytes(const ssd_add_rms_norm_bwd_params_t* prm) {
+  return prm == nullptr ? 0 : add_rms_norm_bwd_workspace(*prm);
+}
+
+int ssd_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_add_rms_norm_bwd");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  const ssd_add_rms_norm_bwd_params_t& p = *prm;
+  SSD_REQUIRE(p.dout && p.total && p.weight && p.rstd && p.dx && p.dweight, SSD_ERR_BAD_ARGUMENT,
+              "dout, total, weight, rstd, dx and dweight must not be NULL");
+  SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE(p.total_dtype == p.x_dtype || p.total_dtype == SSD_F32, SSD_ERR_UNSUPPORTED, "total must have x's dtype or be fp32");
+  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.dim > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE((int64_t)p.batch * p.seqlen <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
+  const int rc = check_workspace(p.workspace, p.workspace_bytes, add_rms_norm_bwd_workspace(p));
+  if (rc != SSD_OK) return rc;
+  return launch_add_rms_norm_bwd(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ssd_short_conv_fwd(const ssd_short_conv_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_short_conv_fwd");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  const int rc = check_conv(*prm);
+  if (rc != SSD_OK) return rc;
+  SSD_REQUIRE(prm->out != nullptr, SSD_ERR_BAD_ARGUMENT, "out must not be NULL");
+  return launch_short_conv_fwd(*prm, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ssd_short_conv_bwd_workspace_bytes(const ssd_short_conv_bwd_params_t* prm) {
+  return prm == nullptr ? 0 : short_conv_bwd_workspace(*prm);
+}
+
+int ssd_short_conv_bwd(const ssd_short_conv_bwd_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_short_conv_bwd");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  int rc = check_conv(prm->conv);
+  if (rc != SSD_OK) return rc;
+  SSD_REQUIRE(prm->dout && prm->dx && prm->dweight, SSD_ERR_BAD_ARGUMENT, "dout, dx and dweight must not be NULL");
+  rc = check_workspace(prm->workspace, prm->workspace_bytes, short_conv_bwd_workspace(*prm));
+  if (rc != SSD_OK) return rc;
+  return launch_short_conv_bwd(*prm, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ssd_short_conv_step(const ssd_short_conv_step_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_short_conv_step");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  const ssd_short_conv_step_params_t& p = *prm;
+  SSD_REQUIRE(p.x && p.conv_state && p.weight && p.out, SSD_ERR_BAD_ARGUMENT, "x, conv_state, weight and out must not be NULL");
+  SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype) && absent_or_valid(p.bias, p.bias_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE(p.batch > 0 && p.slots > 0 && p.channels > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE(p.width >= 2 && p.width <= 4, SSD_ERR_UNSUPPORTED, "short conv: width %d is not 2, 3 or 4", p.width);
+  return launch_short_conv_step(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ssd_token_scan_workspace_bytes(const ssd_token_scan_params_t* prm) {
+  return prm == nullptr || check_scan(*prm) != SSD_OK ? 0 : token_scan_workspace(*prm);
+}
+
+int ssd_token_scan_fwd(const ssd_token_scan_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_token_scan_fwd");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  int rc = check_scan(*prm);
+  if (rc != SSD_OK) return rc;
+  SSD_REQUIRE(prm->out && prm->final_states, SSD_ERR_BAD_ARGUMENT, "out and final_states must not be NULL");
+  rc = check_workspace(prm->workspace, prm->workspace_bytes, token_scan_workspace(*prm));
+  if (rc != SSD_OK) return rc;
+  return launch_token_scan(*prm, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t ssd_token_scan_bwd_workspace_bytes(const ssd_token_scan_bwd_params_t* prm) {
+  return prm == nullptr || check_scan(prm->scan) != SSD_OK ? 0 : token_scan_bwd_workspace(*prm);
+}
+
+int ssd_token_scan_bwd(const ssd_token_scan_bwd_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_token_scan_bwd");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  const ssd_token_scan_bwd_params_t& p = *prm;
+  int rc = check_scan(p.scan);
+  if (rc != SSD_OK) return rc;
+  SSD_REQUIRE(p.scan.checkpoints && (p.scan.z == nullptr || p.scan.out_x), SSD_ERR_BAD_ARGUMENT,
+              "the forward call's checkpoints (and, with z, its out_x) must not be NULL");
+  SSD_REQUIRE(p.dout && p.dx && p.ddt && p.dA && p.dB && p.dC && (p.scan.D == nullptr || p.dD) && (p.scan.z == nullptr || p.dz) &&
+                  (p.scan.dt_bias == nullptr || p.ddt_bias),
+              SSD_ERR_BAD_ARGUMENT, "dout and the gradients of the given inputs must not be NULL");
+  rc = check_workspace(p.workspace, p.workspace_bytes, token_scan_bwd_workspace(p));
+  if (rc != SSD_OK) return rc;
+  return launch_token_scan_bwd(p, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int ssd_token_scan_step(const ssd_token_scan_step_params_t* prm, ssd_stream_t stream) {
+  NvtxRange nvtx_range("ssd_token_scan_step");
+  SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
+  const ssd_token_scan_step_params_t& p = *prm;
+  SSD_REQUIRE(p.state && p.x && p.dt && p.A && p.B && p.C && p.out, SSD_ERR_BAD_ARGUMENT,
+              "state, x, dt, A, B, C and out must not be NULL");
+  SSD_REQUIRE(valid_dtype(p.state_dtype) && valid_dtype(p.x_dtype) && valid_dtype(p.dt_dtype) && valid_dtype(p.A_dtype) &&
+                  absent_or_valid(p.D, p.D_dtype) && absent_or_valid(p.dt_bias, p.bias_dtype),
+              SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE(p.batch > 0 && p.slots > 0 && p.nheads > 0 && p.headdim > 0 && p.ngroups > 0 && p.dstate > 0, SSD_ERR_BAD_ARGUMENT,
+              "sizes must be positive");
+  SSD_REQUIRE(p.nheads % p.ngroups == 0, SSD_ERR_BAD_ARGUMENT, "nheads %d not a multiple of ngroups %d", p.nheads, p.ngroups);
+  return launch_token_step(p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

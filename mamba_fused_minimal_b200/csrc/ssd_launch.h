@@ -77,4 +77,18 @@ int launch_chunk_scan_fast(const ssd_chunk_scan_params_t& p, cudaStream_t stream
 int scan_fused_ok(const ssd_chunk_scan_fused_params_t& f);
 int launch_chunk_scan_fused(const ssd_chunk_scan_fused_params_t& f, cudaStream_t stream);
 
+// ---- the operators around the scan ------------------------------------------------------
+int launch_add_rms_norm(const ssd_add_rms_norm_params_t& p, cudaStream_t stream);            // add_rms_norm.cu
+size_t add_rms_norm_bwd_workspace(const ssd_add_rms_norm_bwd_params_t& p);
+int launch_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t& p, cudaStream_t stream);
+int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream);            // short_conv.cu
+size_t short_conv_bwd_workspace(const ssd_short_conv_bwd_params_t& p);
+int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& p, cudaStream_t stream);
+int launch_short_conv_step(const ssd_short_conv_step_params_t& p, cudaStream_t stream);
+size_t token_scan_workspace(const ssd_token_scan_params_t& p);                               // token_scan.cu
+int launch_token_scan(const ssd_token_scan_params_t& p, cudaStream_t stream);
+size_t token_scan_bwd_workspace(const ssd_token_scan_bwd_params_t& p);                       // token_scan_bwd.cu
+int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& p, cudaStream_t stream);
+int launch_token_step(const ssd_token_scan_step_params_t& p, cudaStream_t stream);           // token_step.cu
+
 }  // namespace ssd

@@ -3,64 +3,17 @@
 // device), looks up the current CUDA stream and calls the C ABI (include/ssd_b200.h).
 // Shape assertions live in the Python shims so that they raise AssertionError like the
 // reference; this layer raises RuntimeError for anything the C ABI rejects.
-#include <c10/cuda/CUDAFunctions.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/extension.h>
-
 #include <limits>
 #include <map>
 #include <mutex>
-#include <optional>
 #include <utility>
 #include <vector>
 
-#include "ssd_b200.h"
+#include "torch_common.h"
+
+using namespace ssd_torch;
 
 namespace {
-
-using torch::Tensor;
-using OptTensor = std::optional<Tensor>;
-
-int dtype_code(const Tensor& t, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return SSD_F32;
-    case at::kBFloat16: return SSD_BF16;
-    case at::kHalf: return SSD_F16;
-    default: TORCH_CHECK(false, name, ": dtype ", t.scalar_type(), " is not fp32 / bf16 / fp16");
-  }
-}
-int dtype_code(at::ScalarType st) {
-  switch (st) {
-    case at::kFloat: return SSD_F32;
-    case at::kBFloat16: return SSD_BF16;
-    case at::kHalf: return SSD_F16;
-    default: TORCH_CHECK(false, "dtype ", st, " is not fp32 / bf16 / fp16");
-  }
-}
-
-void check_cuda(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor (libssd_b200 has no CPU path)");
-  TORCH_CHECK(t.device() == like.device(), name, " is on ", t.device(), ", expected ", like.device());
-}
-
-ssd_stream_t current_stream(const Tensor& t) {
-  return reinterpret_cast<ssd_stream_t>(c10::cuda::getCurrentCUDAStream(t.device().index()).stream());
-}
-
-void check_rc(int rc, const char* what) {
-  TORCH_CHECK(rc == SSD_OK, what, " failed (status ", rc, "): ", ssd_last_error());
-}
-
-template <int N>
-void copy_strides(int64_t (&dst)[N], const Tensor& t, std::initializer_list<int> dims) {
-  int i = 0;
-  for (int d : dims) dst[i++] = t.stride(d);
-}
-
-Tensor as_int32(const Tensor& seq_idx) {
-  return seq_idx.scalar_type() == at::kInt ? seq_idx : seq_idx.to(at::kInt);
-}
 
 void fill_state_inputs(ssd_state_inputs_t& in, const Tensor& B, const Tensor& x, const Tensor& dt,
                        const Tensor& dA, const OptTensor& seq_idx, Tensor& seq_idx_hold) {
@@ -132,7 +85,9 @@ struct Guarded {
 };
 std::vector<Guarded> g_guarded;
 
-Tensor alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts) {
+}  // namespace
+
+Tensor ssd_torch::alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts) {
   int64_t guard;
   {
     std::lock_guard<std::mutex> lock(g_guard_mutex);
@@ -149,6 +104,8 @@ Tensor alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts) {
   g_guarded.push_back({buf, payload});
   return out;
 }
+
+namespace {
 
 void debug_set_guard_bytes(int64_t bytes) {
   TORCH_CHECK(bytes >= 0 && bytes % 256 == 0, "guard bytes must be a non-negative multiple of 256");
@@ -799,4 +756,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("chunk_scan_fwd", &chunk_scan_fwd, py::arg("cb"), py::arg("x"), py::arg("dt"), py::arg("dA_cumsum"),
         py::arg("C"), py::arg("states"), py::arg("D") = py::none(), py::arg("z") = py::none(),
         py::arg("seq_idx") = py::none());
+  bind_layer(m);
 }

@@ -1,0 +1,59 @@
+"""Short causal convolution over the sequence, one filter of 2 to 4 taps for each channel: what stands
+between a layer's input projection and the scan (its channels are x, B and C side by side).  Prompts,
+gradients and single tokens.  The reference has no counterpart.
+
+The state of a sequence is its last width - 1 inputs, (width - 1, channels), oldest first."""
+from .._ext import C as _C
+
+
+def _check(x, weight, bias, initial_states, seq_idx):
+    batch, seqlen, channels = x.shape
+    _, width = weight.shape
+    assert weight.shape == (channels, width)
+    if bias is not None:
+        assert bias.shape == (channels,)
+    if initial_states is not None:
+        assert initial_states.shape == (batch, width - 1, channels)
+    if seq_idx is not None:
+        assert seq_idx.shape == (batch, seqlen)
+    return batch, width, channels
+
+
+def _short_conv_fwd(x, weight, bias=None, apply_silu=True, initial_states=None, seq_idx=None, return_final_states=False):
+    """x (batch, seqlen, channels) with contiguous channels (a column range of a wider buffer will do),
+    weight (channels, width):
+
+        out[t] = act(bias + sum_k weight[:, k] * x[t - (width - 1) + k]),  act = silu or nothing
+
+    Before the first position stand initial_states (batch, width - 1, channels) or zeros.  With seq_idx
+    (batch, seqlen) a position sees only its own sequence; initial_states belong to sequence 0.
+    Returns (out, final_states); final_states is None unless asked for."""
+    _check(x, weight, bias, initial_states, seq_idx)
+    return _C.short_conv_fwd(x, weight, bias, bool(apply_silu), initial_states, seq_idx, bool(return_final_states))
+
+
+def _short_conv_bwd(dout, x, weight, bias=None, apply_silu=True, initial_states=None, seq_idx=None, dfinal_states=None):
+    """Gradients of `_short_conv_fwd` from its inputs (nothing has to be kept).  Returns (dx, dweight, dbias,
+    dinitial_states): x's dtype, except dweight and dbias in fp32; dbias and dinitial_states are None where
+    bias and initial_states are.  The same inputs give the same bits."""
+    batch, width, channels = _check(x, weight, bias, initial_states, seq_idx)
+    assert dout.shape == x.shape
+    if dfinal_states is not None:
+        assert dfinal_states.shape == (batch, width - 1, channels)
+    return _C.short_conv_bwd(dout, x, weight, bias, bool(apply_silu), initial_states, seq_idx, dfinal_states)
+
+
+def _short_conv_step(x, conv_state, weight, bias=None, apply_silu=True, state_indices=None):
+    """One position of each running sequence: x (batch, channels), conv_state (slots, width - 1, channels),
+    which is shifted by one position IN PLACE.  state_indices (batch,) int32 gives each row's slot (without
+    it row i uses slot i).  A row whose index lies outside the slots, or whose slot an earlier row names
+    too, is padding: its output is zero and no state is touched.  Returns out (batch, channels)."""
+    batch, channels = x.shape
+    slots, past, _ = conv_state.shape
+    assert weight.shape == (channels, past + 1)
+    assert conv_state.shape == (slots, past, channels)
+    if bias is not None:
+        assert bias.shape == (channels,)
+    if state_indices is not None:
+        assert state_indices.shape == (batch,)
+    return _C.short_conv_step(x, conv_state, weight, bias, bool(apply_silu), state_indices)

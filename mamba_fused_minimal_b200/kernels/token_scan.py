@@ -1,0 +1,98 @@
+"""Selective scan, position by position, with a decay for each channel and state component; the chunk kernels
+of this package have one decay for each head.  Prompts, gradients, and single tokens; the single-token
+step takes both forms, so it also continues what the chunk kernels began (their final_states are its
+state).  The reference has no counterpart."""
+from .._ext import C as _C
+
+
+def _check(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx):
+    batch, seqlen, channels = x.shape
+    _, _, ngroups, dstate = B.shape
+    assert channels % ngroups == 0
+    assert dt.shape == x.shape
+    assert A.shape == (channels, dstate)
+    assert B.shape == (batch, seqlen, ngroups, dstate)
+    assert C.shape == B.shape
+    if D is not None:
+        assert D.shape == (channels,)
+    if z is not None:
+        assert z.shape == x.shape
+    if dt_bias is not None:
+        assert dt_bias.shape == (channels,)
+    if initial_states is not None:
+        assert initial_states.shape == (batch, channels, dstate)
+    if seq_idx is not None:
+        assert seq_idx.shape == (batch, seqlen)
+    return batch, seqlen, channels, dstate
+
+
+def _token_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, dt_limit=(0.0, float("inf")),
+                    initial_states=None, seq_idx=None, for_backward=False):
+    """x, dt, z (batch, seqlen, channels), A (channels, dstate), B, C (batch, seqlen, ngroups, dstate), D and
+    dt_bias (channels,).  Per channel, with its group's B and C:
+
+        dt' = clamp(softplus?(dt + dt_bias), *dt_limit)
+        h = exp(dt' * A) * h + dt' * x * B;   y = sum(C * h) + D * x;   out = y, or y * silu(z)
+
+    h (fp32) starts from initial_states (batch, channels, dstate) or zero; with seq_idx (batch, seqlen) it is
+    dropped where the sequence changes, and initial_states belong to sequence 0.  dt has x's dtype or fp32.
+
+    Returns (out, final_states, saved): final_states (batch, channels, dstate) fp32, and with for_backward
+    what `_token_scan_bwd` needs, else None."""
+    _check(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx)
+    out, final, checkpoints, out_x = _C.token_scan_fwd(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus), float(dt_limit[0]),
+                                                       float(dt_limit[1]), initial_states, seq_idx, bool(for_backward))
+    return out, final, (checkpoints, out_x) if for_backward else None
+
+
+def _token_scan_bwd(dout, x, dt, A, B, C, saved, D=None, z=None, dt_bias=None, dt_softplus=False, dt_limit=(0.0, float("inf")),
+                    initial_states=None, seq_idx=None, dfinal_states=None):
+    """Gradients of `_token_scan_fwd`, called with the same inputs and with what it saved.  Returns (dx, ddt, dA,
+    dB, dC, dD, dz, ddt_bias, dinitial_states): dA, dD, ddt_bias and dinitial_states in fp32, the others in
+    their input's dtype; None for what was not given.  The same inputs give the same bits."""
+    batch, seqlen, channels, dstate = _check(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx)
+    checkpoints, out_x = saved
+    assert dout.shape == x.shape
+    assert checkpoints.shape == (batch, (seqlen + 15) // 16, channels, dstate)
+    assert (out_x is not None) == (z is not None)
+    if z is not None:
+        assert out_x.shape == x.shape
+    if dfinal_states is not None:
+        assert dfinal_states.shape == (batch, channels, dstate)
+    return _C.token_scan_bwd(dout, x, dt, A, B, C, checkpoints, out_x, D, z, dt_bias, bool(dt_softplus), float(dt_limit[0]),
+                             float(dt_limit[1]), initial_states, seq_idx, dfinal_states)
+
+
+def _token_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, dt_limit=(0.0, float("inf")),
+                     state_indices=None):
+    """One position of each running sequence; `state` is updated IN PLACE.  Two forms:
+
+      per head:    state (slots, nheads, headdim, dstate), x, z (batch, nheads, headdim), A (nheads,),
+                   D (nheads,) or (nheads, headdim) -- the chunk kernels' form and layouts
+      per channel: state (slots, channels, dstate), x, z (batch, channels), A (channels, dstate), D (channels,)
+
+    dt (batch, nheads or channels), dt_bias (nheads or channels,), B, C (batch, ngroups, dstate).  The state
+    may be fp32, bf16 or fp16; the update is computed in fp32 and y sees it before it is rounded.
+
+    state_indices (batch,) int32 gives each row's slot (without it row i uses slot i).  A row whose index
+    lies outside the slots, or whose slot an earlier row names too, is padding: its output is zero and no
+    state is touched.  Returns out, x's shape and dtype."""
+    batch, nheads = x.shape[:2]
+    _, ngroups, dstate = B.shape
+    assert nheads % ngroups == 0
+    assert state.dim() == x.dim() + 1 and x.dim() in (2, 3)
+    assert state.shape[1:] == (*x.shape[1:], dstate)
+    assert A.shape == ((nheads,) if x.dim() == 3 else (nheads, dstate))
+    assert dt.shape == (batch, nheads)
+    assert B.shape == (batch, ngroups, dstate)
+    assert C.shape == B.shape
+    if D is not None:
+        assert D.shape == (nheads,) or D.shape == x.shape[1:]
+    if z is not None:
+        assert z.shape == x.shape
+    if dt_bias is not None:
+        assert dt_bias.shape == (nheads,)
+    if state_indices is not None:
+        assert state_indices.shape == (batch,)
+    return _C.token_scan_step(state, x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus), float(dt_limit[0]), float(dt_limit[1]),
+                              state_indices)
