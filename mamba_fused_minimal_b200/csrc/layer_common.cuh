@@ -65,9 +65,26 @@ __device__ __forceinline__ float dsilu_f(float v) {
   const float g = sigmoid_f(v);
   return g * (1.0f + v * (1.0f - g));
 }
-// log(1 + exp(v)), exact to a few units in the last place also where it is small: the layer's steps
-// lie between 1e-4 and 1e-1, where log(exp(v) + 1) would keep three digits.
-__device__ __forceinline__ float softplus_f(float v) { return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v))); }
+// log(1 + exp(v)), exact to a few units in the last place also where it is small: the layer's steps lie
+// between 1e-4 and 1e-1, where log(exp(v) + 1) would keep three digits.  With e = exp(-|v|) <= 1,
+// log(1 + e) = 2 atanh(e / (2 + e)), whose argument is at most 1/3: seven terms of the series leave 2e-8.
+// The exponential's argument is rounded once in |v| log2 e; what the rounding lost is put back.
+__device__ __forceinline__ float softplus_f(float v) {
+  float m = fabsf(v);
+  m = m > 100.0f ? 100.0f : m;                 // exp(-100) is zero in fp32; a NaN passes
+  const float p = -m * 1.4426950408889634f;
+  const float lost = fmaf(-m, 1.4426950408889634f, -p) * 0.6931471805599453f;
+  float e = ex2_approx(p);
+  e = fmaf(e, lost, e);
+  const float s = __fdividef(e, 2.0f + e), s2 = s * s;
+  float r = fmaf(s2, 1.0f / 13.0f, 1.0f / 11.0f);
+  r = fmaf(s2, r, 1.0f / 9.0f);
+  r = fmaf(s2, r, 1.0f / 7.0f);
+  r = fmaf(s2, r, 1.0f / 5.0f);
+  r = fmaf(s2, r, 1.0f / 3.0f);
+  r = 2.0f * fmaf(s * s2, r, s);
+  return v > 0.0f ? v + r : r;
+}
 // dt' of one position and channel, and the factor of its gradient
 __device__ __forceinline__ float scan_dt(float raw, bool softplus, float lo, float hi) {
   const float v = softplus ? softplus_f(raw) : raw;

@@ -2,15 +2,15 @@
 //
 // Each (position, channel, component) needs one exponential and four multiply-adds, and nothing of it can
 // be shared between channels, so at dstate 16 the special function units (16 exponentials per clock and
-// SM) bound the kernel, ahead of memory (x, dt, z and out once).  A thread holds NS components of one
-// channel's state in registers and LPC adjacent lanes share a channel: the recurrence along the positions
-// never leaves a thread, and only y is summed over the LPC lanes, four positions at a time (the lanes trade
-// halves, so that four sums over four lanes take three exchanges).
+// SM) bound the kernel, ahead of memory (x, dt, z and out once).  A thread holds NS components of K
+// channels' states in registers and LPC adjacent lanes share a channel: the recurrence along the positions
+// never leaves a thread, and only y is summed over the LPC lanes.
 //
-// A block takes 16 channels and walks the positions in tiles of 32.  The tile's x, dt, B and C are turned
-// into fp32 with positions contiguous in shared memory, so that one 16-byte read gives a thread four
-// positions; dt' is formed once per position and channel there.  The next tile's loads are in flight while
-// this one is computed.
+// A block takes 16 channels and walks the positions in tiles of 32.  dt' is formed once per position and
+// channel and put beside dt' x in shared memory, B and C are widened there.  What a lane reads back per
+// component and position has to pass the shared memory's 128 bytes a clock whether it is broadcast or not;
+// K = 2 channels per thread share each B and C.  The multiply-adds work on pairs of components (packed
+// fp32), which halves their issue slots.
 //
 // Few channels and a long sequence: the sequence is cut into segments that run side by side.  A first pass
 // leaves each segment's state from a zero start and the sum of its dt'; since the decay over a segment is
@@ -18,221 +18,383 @@
 // exponentials are computed twice, so this is done only where the GPU would otherwise stand idle.
 #include "token_scan.cuh"
 
+#ifndef SSD_SCAN_K
+#define SSD_SCAN_K 1
+#endif
+#ifndef SSD_SCAN_UNROLL
+#define SSD_SCAN_UNROLL 1
+#endif
+
 namespace ssd {
 namespace {
 
+constexpr int kUnroll = SSD_SCAN_UNROLL;
 constexpr int kCh = 16;            // channels of a block
 constexpr int kTile = 32;          // positions of a tile
-constexpr int kLd = kTile + 4;     // row pitch in shared memory: 16-byte aligned, rows in different banks
+constexpr int kLdu = 2 * kTile + 4;   // row pitches in shared memory: a channel's rows start in different banks
+constexpr int kLdy = 4 * kTile + 4;
 
-template <typename T, int LPC, int NS, bool STATE>
-__global__ void __launch_bounds__(kCh* LPC) token_scan_kernel(ScanArgs a) {
-  constexpr int NT = kCh * LPC;          // threads
-  constexpr int EV = kTile / LPC;        // elements of x a thread loads per tile
-  constexpr int VPR = kCh / EV;          // such vectors per position
-  constexpr int NP = LPC * NS;           // components, padded
-  constexpr bool kAhead = NS <= 4;       // B and C of the next tile wait in registers too
+constexpr int kHelpers = 64;       // threads that load, prepare and store
+constexpr int kVec = kTile * kCh / kHelpers;   // elements of x such a thread loads per tile
+constexpr int kPerRow = kCh / kVec;            // such vectors per position
+
+// LPC lanes share a channel, a thread holds NS components of K channels.
+template <int LPC, int NS, int K>
+struct ScanShape {
+  static constexpr int kCompute = kCh * LPC / K;      // threads that hold states
+  static constexpr int kThreads = kCompute + kHelpers;
+  static constexpr int kState = LPC * NS;             // components, padded
+  static constexpr int kChunk = NS < 4 ? NS : 4;      // components that are read together
+  static constexpr int kGroups = NS / kChunk;
+  static constexpr int kRow = 2 * kState;             // a position's B and C
+  static constexpr int kItems = 2 * kTile * kState / kChunk;   // chunks of a tile's B and C
+  static constexpr int kPer = kItems / kHelpers;
+  static constexpr bool kAhead = kPer <= 16;          // B and C of the next tile wait in registers, too
+  static constexpr int kStage = kCh * (kLdu + kLdy) + kTile * kRow;   // floats of a tile in shared memory
+  static constexpr size_t kSmem = 2 * sizeof(float) * kStage;
+  // blocks an SM should hold: what leaves each thread about 100 registers
+  static constexpr int kResident = kThreads <= 128 ? 5 : kThreads <= 192 ? 3 : 1;
+};
+
+// Named barriers FIRST and FIRST + 1, one for each stage: COUNT threads meet, of which some only leave word
+// (arrive) and go on.  The numbers are constants: with computed ones the block would claim all sixteen
+// barriers, and an SM has enough for four such blocks.
+template <int FIRST, int COUNT>
+__device__ __forceinline__ void bar_sync(int stage) {
+  if (stage == 0)
+    asm volatile("bar.sync %0, %1;" ::"n"(FIRST), "n"(COUNT) : "memory");
+  else
+    asm volatile("bar.sync %0, %1;" ::"n"(FIRST + 1), "n"(COUNT) : "memory");
+}
+template <int FIRST, int COUNT>
+__device__ __forceinline__ void bar_arrive(int stage) {
+  if (stage == 0)
+    asm volatile("bar.arrive %0, %1;" ::"n"(FIRST), "n"(COUNT) : "memory");
+  else
+    asm volatile("bar.arrive %0, %1;" ::"n"(FIRST + 1), "n"(COUNT) : "memory");
+}
+
+template <typename T, int LPC, int NS, int K, bool STATE, bool VEC>
+__global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC, NS, K>::kResident) token_scan_kernel(ScanArgs a) {
+  using Sh = ScanShape<LPC, NS, K>;
+  constexpr int NT = Sh::kThreads, EV = kVec, CB = Sh::kChunk, GR = Sh::kGroups, CK = kCh / K;
   extern __shared__ float4 smem4[];
-  float* s_d = reinterpret_cast<float*>(smem4);       // [kCh][kLd] dt'
-  float* s_u = s_d + kCh * kLd;                       // dt' * x
-  float* s_y = s_u + kCh * kLd;
-  float* s_B = s_y + kCh * kLd;                       // [NP][kLd]
-  float* s_C = s_B + NP * kLd;
-  const int tid = threadIdx.x;
+  // a stage: du [kCh][kLdu], (dt', dt' x) of each position; y [kCh][kLdy], four shares of y of each
+  // position; bc [kTile][GR][LPC][B: CB, C: CB]
+  float* const s_stage = reinterpret_cast<float*>(smem4);
   const int g = blockIdx.x / a.tiles_per_group, tile_c = blockIdx.x % a.tiles_per_group;
   const int b = blockIdx.z, seg = blockIdx.y;
   const int c0 = g * a.per_group + tile_c * kCh;                     // first channel of the block
   const int nch = min(kCh, a.per_group - tile_c * kCh);
   const int t_begin = seg * a.seg_len, t_end = min(a.seqlen, t_begin + a.seg_len);
 
-  // what this thread loads and stores: EV channels of one position
-  const int lt = tid / VPR, lc = (tid % VPR) * EV;
-  const int lcount = max(0, min(EV, nch - lc));
-  const T* xp = static_cast<const T*>(a.x) + b * a.x_sb + c0 + lc;
-  const T* zp = static_cast<const T*>(a.z) + b * a.z_sb + c0 + lc;
-  const int64_t dt_off = b * a.dt_sb + c0 + lc;
-  const T* Bp = static_cast<const T*>(a.B) + b * a.B_sb + g * a.B_sg;
-  const T* Cp = static_cast<const T*>(a.C) + b * a.C_sb + g * a.C_sg;
-  float dv[EV], bv[EV];
+  const int tiles = (t_end - t_begin + kTile - 1) / kTile;
+  // The two kinds of threads meet twice a tile: barrier 1 + stage when the tile is prepared, barrier 3 + stage
+  // when it is computed.  The helpers prepare tile i + 2 only after they have stored tile i, so a stage is
+  // never written while it is read.
+  if (threadIdx.x >= Sh::kCompute) {
+    const int tid = threadIdx.x - Sh::kCompute;
+    // what this thread loads and stores: EV channels of one position
+    const int lt = tid / kPerRow, lc = (tid % kPerRow) * EV;
+    const int lcount = max(0, min(EV, nch - lc));
+    const int lfrom = c0 + (lcount > 0 ? lc : 0);
+    const T* xp = static_cast<const T*>(a.x) + b * a.x_sb + lfrom;
+    const T* zp = static_cast<const T*>(a.z) + b * a.z_sb + lfrom;
+    const int64_t dt_off = b * a.dt_sb + lfrom;
+    const T* Bp = static_cast<const T*>(a.B) + b * a.B_sb + g * a.B_sg;
+    const T* Cp = static_cast<const T*>(a.C) + b * a.C_sb + g * a.C_sg;
+    float dv[EV], bv[EV];
 #pragma unroll
-  for (int e = 0; e < EV; ++e) {
-    dv[e] = a.D && e < lcount ? load_f(a.D, a.D_dtype, c0 + lc + e) : 0.0f;
-    bv[e] = a.bias && e < lcount ? load_f(a.bias, a.bias_dtype, c0 + lc + e) : 0.0f;
+    for (int e = 0; e < EV; ++e) {
+      dv[e] = a.D && e < lcount ? load_f(a.D, a.D_dtype, c0 + lc + e) : 0.0f;
+      bv[e] = a.bias && e < lcount ? load_f(a.bias, a.bias_dtype, c0 + lc + e) : 0.0f;
+    }
+
+    Pack<T, EV> xr, dr16;
+    Pack<float, EV> dr32;
+    Pack<T, CB> bcr[Sh::kAhead ? Sh::kPer : 1];
+    // chunk k of this thread of the tile's B and C: CB components of one position
+    const auto load_bc = [&](int k, int t0) {
+      const int item = k * kHelpers + tid;
+      const int n = item % (GR * LPC) * CB, tb = min(t0 + item / (GR * LPC) % kTile, t_end - 1);
+      const T* src = item >= Sh::kItems / 2 ? Cp + (int64_t)tb * a.C_sl : Bp + (int64_t)tb * a.B_sl;
+      if constexpr (VEC)
+        return load_some<CB, true>(src + (n < a.dstate ? n : 0), CB);
+      else
+        return load_some<CB, false>(src + n, a.dstate - n);
+    };
+    const auto place_bc = [&](float* s_bc, int k, const Pack<T, CB>& r) {
+      const int item = k * kHelpers + tid;
+      const int gl = item % (GR * LPC), t = item / (GR * LPC) % kTile;
+      const int lane = gl / GR, grp = gl % GR;                       // component gl * CB = lane * NS + grp * CB
+      float v[CB];
+#pragma unroll
+      for (int i = 0; i < CB; ++i) v[i] = gl * CB + i < a.dstate ? widen(r.e[i]) : 0.0f;
+      store_vec<CB>(s_bc + t * Sh::kRow + (grp * LPC + lane) * 2 * CB + (item >= Sh::kItems / 2 ? CB : 0), v);
+    };
+    // The next tile's values, left as they are loaded.  Positions past the end read the last one's, channels
+    // past the group's the first one's; what is made of them is masked.
+    const auto fetch = [&](int t0) {
+      const int t = min(t0 + lt, t_end - 1), count = lcount;
+      xr = load_some<EV, VEC>(xp + (int64_t)t * a.x_sl, count);
+      if (a.dt_f32)
+        dr32 = load_some<EV, VEC>(static_cast<const float*>(a.dt) + dt_off + (int64_t)t * a.dt_sl, count);
+      else
+        dr16 = load_some<EV, VEC>(static_cast<const T*>(a.dt) + dt_off + (int64_t)t * a.dt_sl, count);
+      if constexpr (Sh::kAhead) {
+#pragma unroll
+        for (int k = 0; k < Sh::kPer; ++k)
+          if (!STATE || k * kHelpers < Sh::kItems / 2) bcr[k] = load_bc(k, t0);
+      }
+    };
+    const auto prepare = [&](int i) {
+      float* const s_du = s_stage + (i & 1) * Sh::kStage;
+      // positions past the end get dt' = dt' x = 0: they leave the state as it is
+      const int count = t_begin + i * kTile + lt < t_end ? lcount : 0;
+#pragma unroll
+      for (int e = 0; e < EV; ++e) {
+        const float raw = (a.dt_f32 ? dr32.e[e] : widen(dr16.e[e])) + bv[e];
+        const float d = e < count ? scan_dt(raw, a.softplus, a.dt_min, a.dt_max) : 0.0f;
+        const float u = e < count ? d * widen(xr.e[e]) : 0.0f;
+        *reinterpret_cast<float2*>(&s_du[(lc + e) * kLdu + 2 * lt]) = make_float2(d, u);
+      }
+      float* const s_bc = s_du + kCh * (kLdu + kLdy);
+      constexpr int kMine = STATE ? Sh::kPer / 2 : Sh::kPer;         // the second half is C
+      if constexpr (Sh::kAhead) {
+#pragma unroll
+        for (int k = 0; k < kMine; ++k) place_bc(s_bc, k, bcr[k]);
+      } else {
+#pragma unroll 8
+        for (int k = 0; k < kMine; ++k) place_bc(s_bc, k, load_bc(k, t_begin + i * kTile));
+      }
+      bar_arrive<1, NT>(i & 1);
+    };
+    fetch(t_begin);
+    prepare(0);
+    if (tiles > 1) fetch(t_begin + kTile);
+    for (int i = 0; i < tiles; ++i) {
+      const int t0 = t_begin + i * kTile;
+      if (i + 1 < tiles) prepare(i + 1);
+      if (i + 2 < tiles) fetch(t0 + 2 * kTile);
+      // x and z of the tile whose y is awaited, read (again) while it is computed
+      Pack<T, EV> xk, zk;
+      if (!STATE) {
+        const int t = min(t0 + lt, t_end - 1);
+        xk = load_some<EV, VEC>(xp + (int64_t)t * a.x_sl, lcount);
+        if (a.z) zk = load_some<EV, VEC>(zp + (int64_t)t * a.z_sl, lcount);
+      }
+      bar_sync<3, NT>(i & 1);
+      const int count = t0 + lt < t_end ? lcount : 0;
+      if (!STATE && count > 0) {
+        const float* s_y = s_stage + (i & 1) * Sh::kStage + kCh * kLdu;
+        const int64_t at = ((int64_t)b * a.seqlen + t0 + lt) * a.channels + c0 + lc;
+        float o[EV];
+#pragma unroll
+        for (int e = 0; e < EV; ++e) {
+          const float4 y4 = *reinterpret_cast<const float4*>(&s_y[(lc + e) * kLdy + 4 * lt]);
+          o[e] = fmaf(dv[e], widen(xk.e[e]), (y4.x + y4.y) + (y4.z + y4.w));
+        }
+        if (a.z) {
+          if (a.out_x) store_some<EV, VEC>(static_cast<T*>(a.out_x) + at, o, count);
+#pragma unroll
+          for (int e = 0; e < EV; ++e) o[e] *= silu_f(widen(zk.e[e]));
+        }
+        store_some<EV, VEC>(static_cast<T*>(a.out) + at, o, count);
+      }
+    }
+    return;
   }
 
-  // what this thread computes: components q, q + LPC, ... of channel ch
+  const int tid = threadIdx.x;
+  // what this thread computes: components n0 .. n0 + NS - 1, in pairs, of channels ch, ch + CK, ...
   const int q = tid % LPC, ch = tid / LPC;
-  const bool has = ch < nch;
-  float A2[NS], h[NS];
+  const int n0 = q * NS;
+  const int64_t state_at = ((int64_t)b * a.channels + c0 + ch) * a.dstate + n0;
+  f32x2 A2[K][NS / 2], h[K][NS / 2];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int n = s * LPC + q;
-    const bool in = has && n < a.dstate;
-    A2[s] = in ? load_f(a.A, a.A_dtype, (int64_t)(c0 + ch) * a.dstate + n) * kLog2e : 0.0f;
-    h[s] = in && a.init ? load_f(a.init, a.init_dtype, ((int64_t)b * a.channels + c0 + ch) * a.dstate + n) : 0.0f;
-    if (STATE && seg > 0) h[s] = 0.0f;
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int s = 0; s < NS; s += 2) {
+      float A[2], v[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool in = ch + k * CK < nch && n0 + s + i < a.dstate;
+        const int64_t at = (int64_t)k * CK * a.dstate + s + i;
+        A[i] = in ? load_f(a.A, a.A_dtype, (int64_t)(c0 + ch) * a.dstate + n0 + at) * kLog2e : 0.0f;
+        v[i] = in && a.init && seg == 0 ? load_f(a.init, a.init_dtype, state_at + at) : 0.0f;
+      }
+      A2[k][s / 2] = pack2(A[0], A[1]);
+      h[k][s / 2] = pack2(v[0], v[1]);
+    }
   }
+  // the states of the thread's channels into an array (..., channels, dstate) whose element of the block's
+  // first channel is at `base`
+  const auto store_state = [&](float* base) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (ch + k * CK >= nch) continue;
+      float* dst = base + (int64_t)(ch + k * CK) * a.dstate + n0;
+#pragma unroll
+      for (int s = 0; s < NS; s += 2) {
+        float v[2];
+        unpack2(h[k][s / 2], v[0], v[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (n0 + s + i < a.dstate) dst[s + i] = v[i];
+      }
+    }
+  };
   if (!STATE && seg > 0) {
     // the state this segment starts from: what the earlier ones leave, in order (the first of them
     // started from the initial state)
 #pragma unroll
-    for (int s = 0; s < NS; ++s) h[s] = 0.0f;
-    if (has) {
+    for (int k = 0; k < K; ++k) {
+      if (ch + k * CK >= nch) continue;
       for (int j = 0; j < seg; ++j) {
-        const int64_t at = ((int64_t)b * a.segments + j) * a.channels + c0 + ch;
+        const int64_t at = ((int64_t)b * a.segments + j) * a.channels + c0 + ch + k * CK;
         const float2 dec = a.seg_decay[at];
         const bool keeps = j > 0 && dec.y != 0.0f;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          const int n = s * LPC + q;
-          if (n < a.dstate) h[s] = (keeps ? ex2_approx(A2[s] * dec.x) * h[s] : 0.0f) + a.seg_state[at * a.dstate + n];
+        for (int s = 0; s < NS; s += 2) {
+          float A[2], v[2];
+          unpack2(A2[k][s / 2], A[0], A[1]);
+          unpack2(h[k][s / 2], v[0], v[1]);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (n0 + s + i < a.dstate) v[i] = (keeps ? ex2_approx(A[i] * dec.x) * v[i] : 0.0f) + a.seg_state[at * a.dstate + n0 + s + i];
+          }
+          h[k][s / 2] = pack2(v[0], v[1]);
         }
       }
     }
   }
-  float sum_dt = 0.0f;
+  float sum_dt[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) sum_dt[k] = 0.0f;
   bool dropped = false;
 
-  Pack<T, EV> xr, zr;
-  float dr[EV];
-  Pack<T, 4> bc[kAhead ? NS : 1];
-  const auto load_bc = [&](int k, int t0) {
-    const int item = k * NT + tid;
-    const bool is_c = item >= kTile * NP / 4;
-    const int r = is_c ? item - kTile * NP / 4 : item;
-    const int t = t0 + r / (NP / 4), n = (r % (NP / 4)) * 4;
-    const T* p = is_c ? Cp + (int64_t)t * a.C_sl : Bp + (int64_t)t * a.B_sl;
-    const bool want = t < t_end && !(STATE && is_c);
-    return load_some<4>(p + n, want ? a.dstate - n : 0, a.vec_bc);
-  };
-  const auto store_bc = [&](int k, const Pack<T, 4>& v) {
-    const int item = k * NT + tid;
-    const bool is_c = item >= kTile * NP / 4;
-    const int r = is_c ? item - kTile * NP / 4 : item;
-    const int t = r / (NP / 4), n = (r % (NP / 4)) * 4;
-    float* s = is_c ? s_C : s_B;
+  // four positions of the tile; RESET: `r4` says which of them drop the state before
+  const auto four = [&](int t, const float* s_du, const float* s_bc, float* s_y, auto reset, uint32_t r4) {
+    constexpr bool RESET = decltype(reset)::value;
+    float d[K][4], u[K][4], y[K][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[(n + i) * kLd + t] = widen(v.e[i]);
-  };
-  const auto fetch = [&](int t0) {
-    const int t = t0 + lt;
-    const int count = t < t_end ? lcount : 0;
-    xr = load_some<EV>(xp + (int64_t)t * a.x_sl, count, a.vec);
-    if (a.dt_f32) {
-      const Pack<float, EV> r = load_some<EV>(static_cast<const float*>(a.dt) + dt_off + (int64_t)t * a.dt_sl, count, a.vec);
-#pragma unroll
-      for (int e = 0; e < EV; ++e) dr[e] = r.e[e];
-    } else {
-      const Pack<T, EV> r = load_some<EV>(static_cast<const T*>(a.dt) + dt_off + (int64_t)t * a.dt_sl, count, a.vec);
-#pragma unroll
-      for (int e = 0; e < EV; ++e) dr[e] = widen(r.e[e]);
+    for (int k = 0; k < K; ++k) {
+      const float* du = &s_du[(ch + k * CK) * kLdu + 2 * t];
+      const float4 lo = *reinterpret_cast<const float4*>(du), hi = *reinterpret_cast<const float4*>(du + 4);
+      d[k][0] = lo.x, u[k][0] = lo.y, d[k][1] = lo.z, u[k][1] = lo.w;
+      d[k][2] = hi.x, u[k][2] = hi.y, d[k][3] = hi.z, u[k][3] = hi.w;
     }
-    if (!STATE && a.z) zr = load_some<EV>(zp + (int64_t)t * a.z_sl, count, a.vec);
-    if constexpr (kAhead) {
 #pragma unroll
-      for (int k = 0; k < NS; ++k) bc[k] = load_bc(k, t0);
-    }
-  };
-
-  fetch(t_begin);
-  for (int t0 = t_begin; t0 < t_end; t0 += kTile) {
-    // positions past the end get dt' = 0 and x = B = C = 0: they leave the state as it is
-    const int count = t0 + lt < t_end ? lcount : 0;
-    float xv[EV];
-    Pack<T, EV> zv = zr;
+    for (int i = 0; i < 4; ++i) {
+      f32x2 y2[K];
 #pragma unroll
-    for (int e = 0; e < EV; ++e) {
-      xv[e] = widen(xr.e[e]);
-      const float d = e < count ? scan_dt(dr[e] + bv[e], a.softplus, a.dt_min, a.dt_max) : 0.0f;
-      s_d[(lc + e) * kLd + lt] = d;
-      s_u[(lc + e) * kLd + lt] = d * xv[e];
-    }
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int k = 0; k < NS; ++k) store_bc(k, bc[k]);
-    } else {
-#pragma unroll 4
-      for (int k = 0; k < NS; ++k) store_bc(k, load_bc(k, t0));
-    }
-    const uint32_t resets = a.seq ? reset_mask(a, b, t0, tid & 31) : 0u;
-    __syncthreads();
-    if (t0 + kTile < t_end) fetch(t0 + kTile);
-
-    const int stop = min(kTile, t_end - t0);
-    for (int t = 0; t < stop; t += 4) {
-      if (!STATE && a.ckpt && (t & (SSD_TOKEN_SCAN_CHECKPOINT - 1)) == 0 && has) {
-        const int64_t nck = (a.seqlen + SSD_TOKEN_SCAN_CHECKPOINT - 1) / SSD_TOKEN_SCAN_CHECKPOINT;
-        float* dst = a.ckpt + (((int64_t)b * nck + (t0 + t) / SSD_TOKEN_SCAN_CHECKPOINT) * a.channels + c0 + ch) * a.dstate;
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-          if (s * LPC + q < a.dstate) dst[s * LPC + q] = h[s];
-      }
-      const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kLd + t]);
-      const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kLd + t]);
-      const float d[4] = {d4.x, d4.y, d4.z, d4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-      float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const uint32_t r4 = (resets >> t) & 15u;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const float4 B4 = *reinterpret_cast<const float4*>(&s_B[(s * LPC + q) * kLd + t]);
-        const float Bv[4] = {B4.x, B4.y, B4.z, B4.w};
-        float Cv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (!STATE) {
-          const float4 C4 = *reinterpret_cast<const float4*>(&s_C[(s * LPC + q) * kLd + t]);
-          Cv[0] = C4.x, Cv[1] = C4.y, Cv[2] = C4.z, Cv[3] = C4.w;
+      for (int m = 0; m < GR; ++m) {
+        const float* row = s_bc + (t + i) * Sh::kRow + (m * LPC + q) * 2 * CB;
+        f32x2 Bv[CB / 2], Cv[CB / 2];
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(row);
+        Bv[0] = v.x;
+        if constexpr (CB == 2) {
+          Cv[0] = v.y;
+        } else {
+          Bv[1] = v.y;
+          if (!STATE) {
+            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(row + CB);
+            Cv[0] = w.x, Cv[1] = w.y;
+          }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (r4 >> i & 1u) h[s] = 0.0f;
-          h[s] = fmaf(ex2_approx(d[i] * A2[s]), h[s], u[i] * Bv[i]);
-          if (!STATE) y[i] = fmaf(h[s], Cv[i], y[i]);
+        for (int k = 0; k < K; ++k) {
+          const f32x2 dd = pack2(d[k][i], d[k][i]), uu = pack2(u[k][i], u[k][i]);
+#pragma unroll
+          for (int s = 0; s < CB / 2; ++s) {
+            const int at = m * (CB / 2) + s;
+            f32x2& hh = h[k][at];
+            if (RESET && (r4 >> i & 1u)) hh = 0;
+            float e0, e1;
+            unpack2(mul2(dd, A2[k][at]), e0, e1);
+            hh = fma2(pack2(ex2_approx(e0), ex2_approx(e1)), hh, mul2(uu, Bv[s]));
+            if (!STATE) y2[k] = at == 0 ? mul2(hh, Cv[s]) : fma2(hh, Cv[s], y2[k]);
+          }
         }
       }
-      if (STATE) {
-        sum_dt += (d[0] + d[1]) + (d[2] + d[3]);
-        dropped |= r4 != 0u;
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        if (STATE) {
+          sum_dt[k] += d[k][i];
+        } else {
+          float lo, hi;
+          unpack2(y2[k], lo, hi);
+          y[k][i] = lo + hi;
+        }
+      }
+    }
+    if (STATE) return;
+    // y is summed over the channel's lanes: lanes beyond four trade halves until four shares are left, which
+    // go to shared memory and are added where y is used
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      float* dst = &s_y[(ch + k * CK) * kLdy + 4 * t + (q & 3)];
+      if constexpr (LPC == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[4 * i] = y[k][i];
       } else {
-        // four sums over the channel's lanes: lanes trade halves until each of four holds one position
-        const bool odd = q & 1, high = q & 2;
-        float y01 = odd ? y[1] : y[0], y23 = odd ? y[3] : y[2];
-        y01 += __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], 1);
-        y23 += __shfl_xor_sync(0xffffffffu, odd ? y[2] : y[3], 1);
-        float r = high ? y23 : y01;
-        r += __shfl_xor_sync(0xffffffffu, high ? y01 : y23, 2);
-#pragma unroll
-        for (int off = 4; off < LPC; off <<= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
-        if (q < 4) s_y[ch * kLd + t + q] = r;
+        const bool b2 = q & 4;
+        float y0 = b2 ? y[k][1] : y[k][0], y1 = b2 ? y[k][3] : y[k][2];
+        y0 += __shfl_xor_sync(0xffffffffu, b2 ? y[k][0] : y[k][1], 4);
+        y1 += __shfl_xor_sync(0xffffffffu, b2 ? y[k][2] : y[k][3], 4);
+        if constexpr (LPC == 8) {
+          dst[b2 ? 4 : 0] = y0;
+          dst[b2 ? 12 : 8] = y1;
+        } else {
+          const bool b3 = q & 8;
+          float r = b3 ? y1 : y0;
+          r += __shfl_xor_sync(0xffffffffu, b3 ? y0 : y1, 8);
+          dst[(b2 ? 4 : 0) + (b3 ? 8 : 0)] = r;
+        }
       }
     }
-    __syncthreads();
-    if (!STATE && count > 0) {
-      const int64_t at = ((int64_t)b * a.seqlen + t0 + lt) * a.channels + c0 + lc;
-      float o[EV];
-#pragma unroll
-      for (int e = 0; e < EV; ++e) o[e] = s_y[(lc + e) * kLd + lt] + dv[e] * xv[e];
-      if (a.z) {
-        if (a.out_x) store_some<EV>(static_cast<T*>(a.out_x) + at, o, count, a.vec);
-#pragma unroll
-        for (int e = 0; e < EV; ++e) o[e] *= silu_f(widen(zv.e[e]));
+  };
+
+  for (int i = 0; i < tiles; ++i) {
+    const int t0 = t_begin + i * kTile;
+    const float* const s_du = s_stage + (i & 1) * Sh::kStage;
+    float* const s_y = s_stage + (i & 1) * Sh::kStage + kCh * kLdu;
+    const float* const s_bc = s_y + kCh * kLdy;
+    const uint32_t resets = a.seq ? reset_mask(a, b, t0, tid & 31) : 0u;
+    bar_sync<1, NT>(i & 1);
+    const int stop = min(kTile, t_end - t0);
+    for (int half = 0; half < stop; half += SSD_TOKEN_SCAN_CHECKPOINT) {
+      if (!STATE && a.ckpt) {
+        const int64_t nck = (a.seqlen + SSD_TOKEN_SCAN_CHECKPOINT - 1) / SSD_TOKEN_SCAN_CHECKPOINT;
+        store_state(a.ckpt + (((int64_t)b * nck + (t0 + half) / SSD_TOKEN_SCAN_CHECKPOINT) * a.channels + c0) * a.dstate);
       }
-      store_some<EV>(static_cast<T*>(a.out) + at, o, count, a.vec);
+      const int end = min(stop, half + SSD_TOKEN_SCAN_CHECKPOINT);
+      if (resets == 0u) {
+#pragma unroll kUnroll
+        for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::false_type(), 0u);
+      } else {
+#pragma unroll 1
+        for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::true_type(), resets >> t);
+      }
     }
+    if (STATE) dropped |= resets != 0u;
+    bar_arrive<3, NT>(i & 1);
   }
 
-  if (!has) return;
-  float* dst = STATE ? a.seg_state + (((int64_t)b * a.segments + seg) * a.channels + c0 + ch) * a.dstate
-                     : a.final_states + ((int64_t)b * a.channels + c0 + ch) * a.dstate;
-  if (STATE || t_end == a.seqlen) {
+  if (STATE) {
+    const int64_t at = ((int64_t)b * a.segments + seg) * a.channels + c0;
+    store_state(a.seg_state + at * a.dstate);
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-      if (s * LPC + q < a.dstate) dst[s * LPC + q] = h[s];
+    for (int k = 0; k < K; ++k)
+      if (q == 0 && ch + k * CK < nch) a.seg_decay[at + ch + k * CK] = make_float2(sum_dt[k], dropped ? 0.0f : 1.0f);
+  } else if (t_end == a.seqlen) {
+    store_state(a.final_states + ((int64_t)b * a.channels + c0) * a.dstate);
   }
-  if (STATE && q == 0) a.seg_decay[((int64_t)b * a.segments + seg) * a.channels + c0 + ch] = make_float2(sum_dt, dropped ? 0.0f : 1.0f);
 }
 
 // How a problem is laid out over the GPU.
 struct ScanPlan {
-  int lpc, ns, tiles_per_group, segments, seg_len;
+  int lpc, ns, k, tiles_per_group, segments, seg_len;
 };
 
 ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
@@ -240,16 +402,13 @@ ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
   const int per_group = p.channels / p.ngroups;
   s.tiles_per_group = (per_group + kCh - 1) / kCh;
   const int64_t blocks = (int64_t)p.batch * p.ngroups * s.tiles_per_group;
-  // lanes per channel: more lanes give more threads, fewer lanes fewer exchanges and a smaller share of
-  // per-tile work; the fewest that leave each scheduler two warps
   const int n = p.dstate <= 8 ? 8 : p.dstate <= 16 ? 16 : p.dstate <= 32 ? 32 : p.dstate <= 64 ? 64 : p.dstate <= 128 ? 128 : 256;
   s.lpc = n <= 16 ? 4 : n <= 32 ? 8 : 16;
-  const int most = n < 16 ? n : 16;
-  while (s.lpc < most && blocks * s.lpc / 2 < 148 * 8) s.lpc *= 2;
+  s.k = SSD_SCAN_K;
   s.ns = n / s.lpc;
   // segments: only where the blocks leave most of the GPU idle, and none shorter than 256 positions
   s.segments = 1;
-  const int64_t warps = blocks * s.lpc / 2;
+  const int64_t warps = blocks * s.lpc / (2 * s.k);
   if (warps < 148 * 4) {
     const int64_t want = (148 * 12 + warps - 1) / warps, room = p.seqlen / 256;
     s.segments = (int)(want < room ? want : room);
@@ -261,23 +420,39 @@ ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
   return s;
 }
 
-template <typename T, int LPC, int NS>
-int launch_plan(const ScanArgs& a, int batch, cudaStream_t stream) {
-  const size_t smem = (3 * kCh + 2 * LPC * NS) * kLd * sizeof(float);
+template <typename T, int LPC, int NS, int K, bool VEC>
+int launch_vec(const ScanArgs& a, int batch, cudaStream_t stream) {
+  using Sh = ScanShape<LPC, NS, K>;
+  constexpr size_t smem = Sh::kSmem;
   dim3 grid(a.ngroups * a.tiles_per_group, a.segments, batch);
   if (smem > 48 * 1024) {
-    SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_kernel<T, LPC, NS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_kernel<T, LPC, NS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_kernel<T, LPC, NS, K, false, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_kernel<T, LPC, NS, K, true, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   }
   if (a.segments > 1) {
     grid.y = a.segments - 1;                     // nothing starts from the last segment's state
-    token_scan_kernel<T, LPC, NS, true><<<grid, kCh * LPC, smem, stream>>>(a);
+    token_scan_kernel<T, LPC, NS, K, true, VEC><<<grid, Sh::kThreads, smem, stream>>>(a);
     SSD_CUDA_OK(cudaGetLastError());
     grid.y = a.segments;
   }
-  token_scan_kernel<T, LPC, NS, false><<<grid, kCh * LPC, smem, stream>>>(a);
+  token_scan_kernel<T, LPC, NS, K, false, VEC><<<grid, Sh::kThreads, smem, stream>>>(a);
   SSD_CUDA_OK(cudaGetLastError());
   return SSD_OK;
+}
+
+template <typename T, int LPC, int NS, int K>
+int launch_plan(const ScanArgs& a, const ssd_token_scan_params_t& p, cudaStream_t stream) {
+  using Sh = ScanShape<LPC, NS, K>;
+  constexpr int CB = Sh::kChunk, EV = kVec;
+  // a thread's vector of channels begins at a multiple of its length within a group
+  constexpr size_t kMost = EV * sizeof(T) < 16 ? EV * sizeof(T) : 16;
+  const int ds = dtype_size(p.dt_dtype);
+  const size_t dt_most = EV * ds < 16 ? EV * ds : 16;
+  const bool vec = a.per_group % EV == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), kMost) && rows_aligned(p.dt, p.dt_stride, 2, ds, dt_most) &&
+                   (p.z == nullptr || rows_aligned(p.z, p.z_stride, 2, sizeof(T), kMost)) && aligned_to(p.out, kMost) && aligned_to(p.out_x, kMost) &&
+                   p.dstate % CB == 0 && rows_aligned(p.B, p.B_stride, 3, sizeof(T), CB * sizeof(T)) &&
+                   rows_aligned(p.C, p.C_stride, 3, sizeof(T), CB * sizeof(T));
+  return vec ? launch_vec<T, LPC, NS, K, true>(a, p.batch, stream) : launch_vec<T, LPC, NS, K, false>(a, p.batch, stream);
 }
 
 size_t seg_state_bytes(const ssd_token_scan_params_t& p, const ScanPlan& s) {
@@ -303,13 +478,6 @@ ScanArgs scan_args(const ssd_token_scan_params_t& p) {
   a.B_sb = p.B_stride[0], a.B_sl = p.B_stride[1], a.B_sg = p.B_stride[2];
   a.C_sb = p.C_stride[0], a.C_sl = p.C_stride[1], a.C_sg = p.C_stride[2];
   a.s_sb = p.seq_idx_stride[0], a.s_sl = p.seq_idx_stride[1];
-  const int es = dtype_size(p.x_dtype), ds = dtype_size(p.dt_dtype);
-  // a thread's vector of channels begins at a multiple of its own length within the group: aligned if
-  // groups and rows are aligned to 16 bytes of the type
-  a.vec = a.per_group % (16 / es) == 0 && p.channels % (16 / es) == 0 && rows_aligned(p.x, p.x_stride, 2, es, 16) &&
-          rows_aligned(p.dt, p.dt_stride, 2, ds, 16) && (p.z == nullptr || rows_aligned(p.z, p.z_stride, 2, es, 16)) &&
-          aligned_to(p.out, 16) && aligned_to(p.out_x, 16);
-  a.vec_bc = p.dstate % 4 == 0 && rows_aligned(p.B, p.B_stride, 3, es, 4 * es) && rows_aligned(p.C, p.C_stride, 3, es, 4 * es);
   a.seg_len = p.seqlen, a.segments = 1;
   return a;
 }
@@ -332,17 +500,19 @@ int launch_token_scan(const ssd_token_scan_params_t& p, cudaStream_t stream) {
   SSD_REQUIRE(p.batch <= 65535, SSD_ERR_UNSUPPORTED, "token scan: batch %d too large", p.batch);
   return with_type(p.x_dtype, [&](auto t) -> int {
     using T = decltype(t);
-    switch (s.lpc * 1000 + s.ns) {
-      case 4002: return launch_plan<T, 4, 2>(a, p.batch, stream);
-      case 8001: return launch_plan<T, 8, 1>(a, p.batch, stream);
-      case 4004: return launch_plan<T, 4, 4>(a, p.batch, stream);
-      case 8002: return launch_plan<T, 8, 2>(a, p.batch, stream);
-      case 16001: return launch_plan<T, 16, 1>(a, p.batch, stream);
-      case 8004: return launch_plan<T, 8, 4>(a, p.batch, stream);
-      case 16002: return launch_plan<T, 16, 2>(a, p.batch, stream);
-      case 16004: return launch_plan<T, 16, 4>(a, p.batch, stream);
-      case 16008: return launch_plan<T, 16, 8>(a, p.batch, stream);
-      default: return launch_plan<T, 16, 16>(a, p.batch, stream);
+    switch ((s.k * 100 + s.lpc) * 100 + s.ns) {
+      case 10402: return launch_plan<T, 4, 2, 1>(a, p, stream);
+      case 10404: return launch_plan<T, 4, 4, 1>(a, p, stream);
+      case 10804: return launch_plan<T, 8, 4, 1>(a, p, stream);
+      case 11604: return launch_plan<T, 16, 4, 1>(a, p, stream);
+      case 11608: return launch_plan<T, 16, 8, 1>(a, p, stream);
+      case 11616: return launch_plan<T, 16, 16, 1>(a, p, stream);
+      case 20402: return launch_plan<T, 4, 2, 2>(a, p, stream);
+      case 20404: return launch_plan<T, 4, 4, 2>(a, p, stream);
+      case 20804: return launch_plan<T, 8, 4, 2>(a, p, stream);
+      case 21604: return launch_plan<T, 16, 4, 2>(a, p, stream);
+      case 21608: return launch_plan<T, 16, 8, 2>(a, p, stream);
+      default: return launch_plan<T, 16, 16, 2>(a, p, stream);
     }
   });
 }

@@ -84,31 +84,38 @@ __global__ void __launch_bounds__(kBwdThreads) token_scan_bwd_kernel(ScanBwdArgs
   float sum_A = 0.0f;
 
   const int tiles = (a.seqlen + kT - 1) / kT;
-  float xr[PER], dr[PER], gr[PER], zr[PER], yr[PER], bcr[kAhead ? Sh::kPerBc : 1], h_next = 0.0f;
-  const auto read = [&](const void* base, int64_t at) { return widen(static_cast<const T*>(base)[at]); };
+  // as they were loaded: nothing waits for them before they are used
+  T xr[PER], dr[PER], gr[PER], zr[PER], yr[PER], bcr[kAhead ? Sh::kPerBc : 1];
+  float dr32[PER], h_next = 0.0f;
+  const T zero = narrow<T>(0.0f);
+  const auto read = [&](const void* base, int64_t at) { return static_cast<const T*>(base)[at]; };
   const auto load_bc = [&](int k, int t0) {
     const int item = k * kBwdThreads + tid;
-    if (Sh::kBc < kBwdThreads && item >= Sh::kBc) return 0.0f;
+    if (Sh::kBc < kBwdThreads && item >= Sh::kBc) return zero;
     const int nn = item % NP, t = t0 + (item / NP) % kT;
     const bool is_c = item >= kT * NP;
-    if (nn >= a.dstate || t >= a.seqlen) return 0.0f;
+    if (nn >= a.dstate || t >= a.seqlen) return zero;
     return is_c ? read(a.C, b * a.C_sb + (int64_t)t * a.C_sl + grp * a.C_sg + nn) : read(a.B, b * a.B_sb + (int64_t)t * a.B_sl + grp * a.B_sg + nn);
   };
-  const auto store_bc = [&](int k, float v) {
+  const auto store_bc = [&](int k, T v) {
     const int item = k * kBwdThreads + tid;
     if (Sh::kBc < kBwdThreads && item >= Sh::kBc) return;
-    (item >= kT * NP ? s_C : s_B)[(item % NP) * kPitch + (item / NP) % kT] = v;
+    (item >= kT * NP ? s_C : s_B)[(item % NP) * kPitch + (item / NP) % kT] = widen(v);
   };
   const auto fetch = [&](int t0) {
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
       const int item = e * kBwdThreads + tid, t = t0 + item / CH;
-      xr[e] = dr[e] = gr[e] = zr[e] = yr[e] = 0.0f;
+      xr[e] = dr[e] = gr[e] = zr[e] = yr[e] = zero;
+      dr32[e] = 0.0f;
       if (item >= Sh::kItems || t >= a.seqlen || lc >= nch) continue;
       const int64_t c = c0 + lc;
       xr[e] = read(a.x, b * a.x_sb + (int64_t)t * a.x_sl + c);
       const int64_t dat = b * a.dt_sb + (int64_t)t * a.dt_sl + c;
-      dr[e] = a.dt_f32 ? static_cast<const float*>(a.dt)[dat] : read(a.dt, dat);
+      if (a.dt_f32)
+        dr32[e] = static_cast<const float*>(a.dt)[dat];
+      else
+        dr[e] = read(a.dt, dat);
       gr[e] = read(q.dout, b * q.d_sb + (int64_t)t * q.d_sl + c);
       if (a.z) {
         zr[e] = read(a.z, b * a.z_sb + (int64_t)t * a.z_sl + c);
@@ -131,13 +138,14 @@ __global__ void __launch_bounds__(kBwdThreads) token_scan_bwd_kernel(ScanBwdArgs
       const int item = e * kBwdThreads + tid, lt = item / CH, t = t0 + lt;
       if (item >= Sh::kItems) continue;
       const bool in = t < a.seqlen && lc < nch;
-      x[e] = xr[e];
-      raw[e] = dr[e] + bias;
+      x[e] = widen(xr[e]);
+      raw[e] = (a.dt_f32 ? dr32[e] : widen(dr[e])) + bias;
       d[e] = in ? scan_dt(raw[e], a.softplus, a.dt_min, a.dt_max) : 0.0f;
-      dy[e] = gr[e];
+      dy[e] = widen(gr[e]);
       if (a.z) {
-        dy[e] = gr[e] * silu_f(zr[e]);
-        if (in) static_cast<T*>(q.dz)[((int64_t)b * a.seqlen + t) * a.channels + c0 + lc] = narrow<T>(gr[e] * yr[e] * dsilu_f(zr[e]));
+        const float zv = widen(zr[e]);
+        if (in) static_cast<T*>(q.dz)[((int64_t)b * a.seqlen + t) * a.channels + c0 + lc] = narrow<T>(dy[e] * widen(yr[e]) * dsilu_f(zv));
+        dy[e] *= silu_f(zv);
       }
       s_d[lc * kPitch + lt] = d[e];
       s_u[lc * kPitch + lt] = d[e] * x[e];
