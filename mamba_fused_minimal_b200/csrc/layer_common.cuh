@@ -58,7 +58,13 @@ __device__ __forceinline__ void load_param(const void* base, int dtype, int64_t 
 }
 
 // ---- activations -----------------------------------------------------------------------------------
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.0f, 1.0f + __expf(-v)); }
+__device__ __forceinline__ float rcp_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// 1 / (1 + exp(-v)): zero where the exponential overflows
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_approx(1.0f + ex2_approx(v * -1.4426950408889634f)); }
 __device__ __forceinline__ float silu_f(float v) { return v * sigmoid_f(v); }
 // d/dv of v * sigmoid(v)
 __device__ __forceinline__ float dsilu_f(float v) {
@@ -68,22 +74,16 @@ __device__ __forceinline__ float dsilu_f(float v) {
 // log(1 + exp(v)), exact to a few units in the last place also where it is small: the layer's steps lie
 // between 1e-4 and 1e-1, where log(exp(v) + 1) would keep three digits.  With e = exp(-|v|) <= 1,
 // log(1 + e) = 2 atanh(e / (2 + e)), whose argument is at most 1/3: seven terms of the series leave 2e-8.
-// The exponential's argument is rounded once in |v| log2 e; what the rounding lost is put back.
 __device__ __forceinline__ float softplus_f(float v) {
-  float m = fabsf(v);
-  m = m > 100.0f ? 100.0f : m;                 // exp(-100) is zero in fp32; a NaN passes
-  const float p = -m * 1.4426950408889634f;
-  const float lost = fmaf(-m, 1.4426950408889634f, -p) * 0.6931471805599453f;
-  float e = ex2_approx(p);
-  e = fmaf(e, lost, e);
-  const float s = __fdividef(e, 2.0f + e), s2 = s * s;
+  const float e = ex2_approx(fabsf(v) * -1.4426950408889634f);
+  const float s = e * rcp_approx(2.0f + e), s2 = s * s;
   float r = fmaf(s2, 1.0f / 13.0f, 1.0f / 11.0f);
   r = fmaf(s2, r, 1.0f / 9.0f);
   r = fmaf(s2, r, 1.0f / 7.0f);
   r = fmaf(s2, r, 1.0f / 5.0f);
   r = fmaf(s2, r, 1.0f / 3.0f);
-  r = 2.0f * fmaf(s * s2, r, s);
-  return v > 0.0f ? v + r : r;
+  r = fmaf(s * s2, r, s);
+  return fmaf(2.0f, r, fmaxf(v, 0.0f));          // r is a NaN where v is
 }
 // dt' of one position and channel, and the factor of its gradient
 __device__ __forceinline__ float scan_dt(float raw, bool softplus, float lo, float hi) {

@@ -7,10 +7,11 @@
 // never leaves a thread, and only y is summed over the LPC lanes.
 //
 // A block takes 16 channels and walks the positions in tiles of 32.  dt' is formed once per position and
-// channel and put beside dt' x in shared memory, B and C are widened there.  What a lane reads back per
-// component and position has to pass the shared memory's 128 bytes a clock whether it is broadcast or not;
-// K = 2 channels per thread share each B and C.  The multiply-adds work on pairs of components (packed
-// fp32), which halves their issue slots.
+// channel and put beside dt' x in shared memory, B and C are copied there as they are.  What a lane reads
+// back per component and position has to pass the shared memory's 128 bytes a clock, broadcast or not:
+// with B and C widened in shared memory that was the bound (17 of 19 cycles per 32 updates and
+// scheduler), so 16-bit ones are widened in registers.  The multiply-adds work on pairs of components
+// (packed fp32), which halves their issue slots.
 //
 // Few channels and a long sequence: the sequence is cut into segments that run side by side.  A first pass
 // leaves each segment's state from a zero start and the sum of its dt'; since the decay over a segment is
@@ -18,28 +19,29 @@
 // exponentials are computed twice, so this is done only where the GPU would otherwise stand idle.
 #include "token_scan.cuh"
 
-#ifndef SSD_SCAN_K
-#define SSD_SCAN_K 1
-#endif
-#ifndef SSD_SCAN_UNROLL
-#define SSD_SCAN_UNROLL 1
-#endif
-
 namespace ssd {
 namespace {
 
-constexpr int kUnroll = SSD_SCAN_UNROLL;
 constexpr int kCh = 16;            // channels of a block
 constexpr int kTile = 32;          // positions of a tile
-constexpr int kLdu = 2 * kTile + 4;   // row pitches in shared memory: a channel's rows start in different banks
-constexpr int kLdy = 4 * kTile + 4;
+// Rows in shared memory, in floats: dt' and dt' x of a channel by position, and its four shares of y by
+// position.  Eight channels' rows start four banks apart, and channels 8 to 15 sixteen banks further, so
+// neither the threads that compute nor those that prepare meet in a bank.
+constexpr int kLdu = kTile + 4, kDu = kCh * kLdu + 16;
+constexpr int kLdy = 4 * kTile + 4, kY = kCh * kLdy + 16;
+__device__ __forceinline__ int du_row(int ch) { return ch * kLdu + (ch >> 3) * 16; }
+__device__ __forceinline__ int y_row(int ch) { return ch * kLdy + (ch >> 3) * 16; }
 
 constexpr int kHelpers = 64;       // threads that load, prepare and store
 constexpr int kVec = kTile * kCh / kHelpers;   // elements of x such a thread loads per tile
 constexpr int kPerRow = kCh / kVec;            // such vectors per position
 
+constexpr int resident(int threads, int states) {
+  return threads <= 128 ? 5 : threads <= 192 ? (states <= 8 ? 3 : 2) : (states <= 4 ? 2 : 1);
+}
+
 // LPC lanes share a channel, a thread holds NS components of K channels.
-template <int LPC, int NS, int K>
+template <typename T, int LPC, int NS, int K>
 struct ScanShape {
   static constexpr int kCompute = kCh * LPC / K;      // threads that hold states
   static constexpr int kThreads = kCompute + kHelpers;
@@ -50,11 +52,36 @@ struct ScanShape {
   static constexpr int kItems = 2 * kTile * kState / kChunk;   // chunks of a tile's B and C
   static constexpr int kPer = kItems / kHelpers;
   static constexpr bool kAhead = kPer <= 16;          // B and C of the next tile wait in registers, too
-  static constexpr int kStage = kCh * (kLdu + kLdy) + kTile * kRow;   // floats of a tile in shared memory
+  static constexpr int kStage = 2 * kDu + kY + kTile * kRow * (int)sizeof(T) / 4;   // a tile in shared memory, in 4-byte words
   static constexpr size_t kSmem = 2 * sizeof(float) * kStage;
-  // blocks an SM should hold: what leaves each thread about 100 registers
-  static constexpr int kResident = kThreads <= 128 ? 5 : kThreads <= 192 ? 3 : 1;
+  // blocks an SM should hold, what leaves a thread the registers that its states need
+  static constexpr int kResident = resident(kThreads, NS * K);
 };
+
+// CB components of B and CB of C that lie side by side in shared memory, as pairs of fp32
+template <int CB, bool C>
+__device__ __forceinline__ void load_bc_pairs(const float* p, f32x2 (&B)[CB / 2], f32x2 (&Cv)[CB / 2]) {
+  const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(p);
+  B[0] = v.x;
+  if constexpr (CB == 2) {
+    Cv[0] = v.y;
+  } else {
+    B[1] = v.y;
+    if constexpr (C) {
+      const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p + 4);
+      Cv[0] = w.x, Cv[1] = w.y;
+    }
+  }
+}
+template <int CB, bool C, typename T>
+__device__ __forceinline__ void load_bc_pairs(const T* p, f32x2 (&B)[CB / 2], f32x2 (&Cv)[CB / 2]) {
+  const Pack<uint32_t, CB> w = *reinterpret_cast<const Pack<uint32_t, CB>*>(p);
+#pragma unroll
+  for (int i = 0; i < CB / 2; ++i) {
+    B[i] = widen_pair<T>(w.e[i]);
+    if constexpr (C) Cv[i] = widen_pair<T>(w.e[CB / 2 + i]);
+  }
+}
 
 // Named barriers FIRST and FIRST + 1, one for each stage: COUNT threads meet, of which some only leave word
 // (arrive) and go on.  The numbers are constants: with computed ones the block would claim all sixteen
@@ -75,12 +102,11 @@ __device__ __forceinline__ void bar_arrive(int stage) {
 }
 
 template <typename T, int LPC, int NS, int K, bool STATE, bool VEC>
-__global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC, NS, K>::kResident) token_scan_kernel(ScanArgs a) {
-  using Sh = ScanShape<LPC, NS, K>;
+__global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<T, LPC, NS, K>::kResident) token_scan_kernel(ScanArgs a) {
+  using Sh = ScanShape<T, LPC, NS, K>;
   constexpr int NT = Sh::kThreads, EV = kVec, CB = Sh::kChunk, GR = Sh::kGroups, CK = kCh / K;
   extern __shared__ float4 smem4[];
-  // a stage: du [kCh][kLdu], (dt', dt' x) of each position; y [kCh][kLdy], four shares of y of each
-  // position; bc [kTile][GR][LPC][B: CB, C: CB]
+  // a stage: dt' rows, dt' x rows, y rows, bc [kTile][GR][LPC][B: CB, C: CB]
   float* const s_stage = reinterpret_cast<float*>(smem4);
   const int g = blockIdx.x / a.tiles_per_group, tile_c = blockIdx.x % a.tiles_per_group;
   const int b = blockIdx.z, seg = blockIdx.y;
@@ -103,34 +129,41 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
     const int64_t dt_off = b * a.dt_sb + lfrom;
     const T* Bp = static_cast<const T*>(a.B) + b * a.B_sb + g * a.B_sg;
     const T* Cp = static_cast<const T*>(a.C) + b * a.C_sb + g * a.C_sg;
-    float dv[EV], bv[EV];
+    f32x2 dv[EV / 2], bv[EV / 2];
 #pragma unroll
-    for (int e = 0; e < EV; ++e) {
-      dv[e] = a.D && e < lcount ? load_f(a.D, a.D_dtype, c0 + lc + e) : 0.0f;
-      bv[e] = a.bias && e < lcount ? load_f(a.bias, a.bias_dtype, c0 + lc + e) : 0.0f;
+    for (int e = 0; e < EV; e += 2) {
+      float u[2], v[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        u[i] = a.D && e + i < lcount ? load_f(a.D, a.D_dtype, c0 + lc + e + i) : 0.0f;
+        v[i] = a.bias && e + i < lcount ? load_f(a.bias, a.bias_dtype, c0 + lc + e + i) : 0.0f;
+      }
+      dv[e / 2] = pack2(u[0], u[1]);
+      bv[e / 2] = pack2(v[0], v[1]);
     }
 
     Pack<T, EV> xr, dr16;
     Pack<float, EV> dr32;
     Pack<T, CB> bcr[Sh::kAhead ? Sh::kPer : 1];
-    // chunk k of this thread of the tile's B and C: CB components of one position
+    // Chunk k of this thread of a tile's B (first half) and C: CB components from `bn` on, of position
+    // bt + a multiple of kStep.  A chunk's lane and group: component gl * CB = lane * NS + grp * CB.
+    constexpr int kStep = kHelpers / (GR * LPC), kHalf = Sh::kPer / 2;
+    const int gl = tid % (GR * LPC), bt = tid / (GR * LPC), bn = gl * CB;
+    const bool bin = bn < a.dstate;
+    const T* const Bt = Bp + (VEC && !bin ? 0 : bn);
+    const T* const Ct = Cp + (VEC && !bin ? 0 : bn);
+    const int bc_at = bt * Sh::kRow + (gl % GR * LPC + gl / GR) * 2 * CB;
     const auto load_bc = [&](int k, int t0) {
-      const int item = k * kHelpers + tid;
-      const int n = item % (GR * LPC) * CB, tb = min(t0 + item / (GR * LPC) % kTile, t_end - 1);
-      const T* src = item >= Sh::kItems / 2 ? Cp + (int64_t)tb * a.C_sl : Bp + (int64_t)tb * a.B_sl;
-      if constexpr (VEC)
-        return load_some<CB, true>(src + (n < a.dstate ? n : 0), CB);
-      else
-        return load_some<CB, false>(src + n, a.dstate - n);
+      const int t = min(t0 + bt + k % kHalf * kStep, t_end - 1);
+      return load_some<CB, VEC>(k < kHalf ? Bt + t * a.B_sl : Ct + t * a.C_sl, a.dstate - bn);
     };
-    const auto place_bc = [&](float* s_bc, int k, const Pack<T, CB>& r) {
-      const int item = k * kHelpers + tid;
-      const int gl = item % (GR * LPC), t = item / (GR * LPC) % kTile;
-      const int lane = gl / GR, grp = gl % GR;                       // component gl * CB = lane * NS + grp * CB
-      float v[CB];
+    const auto place_bc = [&](T* s_bc, int k, Pack<T, CB> r) {
+      if (a.dstate < Sh::kState) {
 #pragma unroll
-      for (int i = 0; i < CB; ++i) v[i] = gl * CB + i < a.dstate ? widen(r.e[i]) : 0.0f;
-      store_vec<CB>(s_bc + t * Sh::kRow + (grp * LPC + lane) * 2 * CB + (item >= Sh::kItems / 2 ? CB : 0), v);
+        for (int i = 0; i < CB; ++i)
+          if (bn + i >= a.dstate) r.e[i] = narrow<T>(0.0f);
+      }
+      *reinterpret_cast<Pack<T, CB>*>(s_bc + bc_at + k % kHalf * kStep * Sh::kRow + (k < kHalf ? 0 : CB)) = r;
     };
     // The next tile's values, left as they are loaded.  Positions past the end read the last one's, channels
     // past the group's the first one's; what is made of them is masked.
@@ -144,22 +177,51 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
       if constexpr (Sh::kAhead) {
 #pragma unroll
         for (int k = 0; k < Sh::kPer; ++k)
-          if (!STATE || k * kHelpers < Sh::kItems / 2) bcr[k] = load_bc(k, t0);
+          if (!STATE || k < kHalf) bcr[k] = load_bc(k, t0);
       }
     };
     const auto prepare = [&](int i) {
-      float* const s_du = s_stage + (i & 1) * Sh::kStage;
-      // positions past the end get dt' = dt' x = 0: they leave the state as it is
-      const int count = t_begin + i * kTile + lt < t_end ? lcount : 0;
+      float* const s_d = s_stage + (i & 1) * Sh::kStage + du_row(lc) + lt;
+      if (t_begin + i * kTile + lt < t_end) {
+        // the branches stand outside the loops: the pairs' chains of operations run side by side
+        f32x2 d[EV / 2];
+        if (a.dt_f32) {
 #pragma unroll
-      for (int e = 0; e < EV; ++e) {
-        const float raw = (a.dt_f32 ? dr32.e[e] : widen(dr16.e[e])) + bv[e];
-        const float d = e < count ? scan_dt(raw, a.softplus, a.dt_min, a.dt_max) : 0.0f;
-        const float u = e < count ? d * widen(xr.e[e]) : 0.0f;
-        *reinterpret_cast<float2*>(&s_du[(lc + e) * kLdu + 2 * lt]) = make_float2(d, u);
+          for (int e = 0; e < EV / 2; ++e) d[e] = add2(pair_of(dr32, e), bv[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < EV / 2; ++e) d[e] = add2(pair_of(dr16, e), bv[e]);
+        }
+        if (a.softplus) {
+#pragma unroll
+          for (int e = 0; e < EV / 2; ++e) d[e] = softplus2(d[e]);
+        }
+        if (a.limits) {
+#pragma unroll
+          for (int e = 0; e < EV / 2; ++e) {
+            float v[2];
+            unpack2(d[e], v[0], v[1]);
+            d[e] = pack2(fminf(fmaxf(v[0], a.dt_min), a.dt_max), fminf(fmaxf(v[1], a.dt_min), a.dt_max));
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < EV / 2; ++e) {
+          float v[2], u[2];
+          unpack2(d[e], v[0], v[1]);
+          unpack2(mul2(d[e], pair_of(xr, e)), u[0], u[1]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            s_d[(2 * e + k) * kLdu] = v[k];
+            s_d[(2 * e + k) * kLdu + kDu] = u[k];
+          }
+        }
+      } else {
+        // positions past the end leave the state as it is
+#pragma unroll
+        for (int e = 0; e < EV; ++e) s_d[e * kLdu] = s_d[e * kLdu + kDu] = 0.0f;
       }
-      float* const s_bc = s_du + kCh * (kLdu + kLdy);
-      constexpr int kMine = STATE ? Sh::kPer / 2 : Sh::kPer;         // the second half is C
+      T* const s_bc = reinterpret_cast<T*>(s_stage + (i & 1) * Sh::kStage + 2 * kDu + kY);
+      constexpr int kMine = STATE ? kHalf : Sh::kPer;
       if constexpr (Sh::kAhead) {
 #pragma unroll
         for (int k = 0; k < kMine; ++k) place_bc(s_bc, k, bcr[k]);
@@ -174,30 +236,34 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
     if (tiles > 1) fetch(t_begin + kTile);
     for (int i = 0; i < tiles; ++i) {
       const int t0 = t_begin + i * kTile;
-      if (i + 1 < tiles) prepare(i + 1);
-      if (i + 2 < tiles) fetch(t0 + 2 * kTile);
-      // x and z of the tile whose y is awaited, read (again) while it is computed
+      // x and z of the tile whose y is awaited, read (again) before the next one is prepared
       Pack<T, EV> xk, zk;
       if (!STATE) {
         const int t = min(t0 + lt, t_end - 1);
         xk = load_some<EV, VEC>(xp + (int64_t)t * a.x_sl, lcount);
         if (a.z) zk = load_some<EV, VEC>(zp + (int64_t)t * a.z_sl, lcount);
       }
+      if (i + 1 < tiles) prepare(i + 1);
+      if (i + 2 < tiles) fetch(t0 + 2 * kTile);
       bar_sync<3, NT>(i & 1);
       const int count = t0 + lt < t_end ? lcount : 0;
       if (!STATE && count > 0) {
-        const float* s_y = s_stage + (i & 1) * Sh::kStage + kCh * kLdu;
+        const float* s_y = s_stage + (i & 1) * Sh::kStage + 2 * kDu + y_row(lc) + 4 * lt;
         const int64_t at = ((int64_t)b * a.seqlen + t0 + lt) * a.channels + c0 + lc;
         float o[EV];
 #pragma unroll
         for (int e = 0; e < EV; ++e) {
-          const float4 y4 = *reinterpret_cast<const float4*>(&s_y[(lc + e) * kLdy + 4 * lt]);
-          o[e] = fmaf(dv[e], widen(xk.e[e]), (y4.x + y4.y) + (y4.z + y4.w));
+          const ulonglong2 y4 = *reinterpret_cast<const ulonglong2*>(s_y + e * kLdy);
+          float lo, hi;
+          unpack2(add2(y4.x, y4.y), lo, hi);
+          o[e] = lo + hi;
         }
+#pragma unroll
+        for (int e = 0; e < EV; e += 2) unpack2(fma2(dv[e / 2], pair_of(xk, e / 2), pack2(o[e], o[e + 1])), o[e], o[e + 1]);
         if (a.z) {
           if (a.out_x) store_some<EV, VEC>(static_cast<T*>(a.out_x) + at, o, count);
 #pragma unroll
-          for (int e = 0; e < EV; ++e) o[e] *= silu_f(widen(zk.e[e]));
+          for (int e = 0; e < EV; e += 2) unpack2(mul2(pack2(o[e], o[e + 1]), silu2(pair_of(zk, e / 2))), o[e], o[e + 1]);
         }
         store_some<EV, VEC>(static_cast<T*>(a.out) + at, o, count);
       }
@@ -274,34 +340,24 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
   bool dropped = false;
 
   // four positions of the tile; RESET: `r4` says which of them drop the state before
-  const auto four = [&](int t, const float* s_du, const float* s_bc, float* s_y, auto reset, uint32_t r4) {
+  const auto four = [&](int t, const float* s_du, const T* s_bc, float* s_y, auto reset, uint32_t r4) {
     constexpr bool RESET = decltype(reset)::value;
     float d[K][4], u[K][4], y[K][4];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const float* du = &s_du[(ch + k * CK) * kLdu + 2 * t];
-      const float4 lo = *reinterpret_cast<const float4*>(du), hi = *reinterpret_cast<const float4*>(du + 4);
-      d[k][0] = lo.x, u[k][0] = lo.y, d[k][1] = lo.z, u[k][1] = lo.w;
-      d[k][2] = hi.x, u[k][2] = hi.y, d[k][3] = hi.z, u[k][3] = hi.w;
+      const float* du = s_du + du_row(ch + k * CK) + t;
+      const float4 dd = *reinterpret_cast<const float4*>(du), uu = *reinterpret_cast<const float4*>(du + kDu);
+      d[k][0] = dd.x, d[k][1] = dd.y, d[k][2] = dd.z, d[k][3] = dd.w;
+      u[k][0] = uu.x, u[k][1] = uu.y, u[k][2] = uu.z, u[k][3] = uu.w;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       f32x2 y2[K];
 #pragma unroll
       for (int m = 0; m < GR; ++m) {
-        const float* row = s_bc + (t + i) * Sh::kRow + (m * LPC + q) * 2 * CB;
+        const T* row = s_bc + (t + i) * Sh::kRow + (m * LPC + q) * 2 * CB;
         f32x2 Bv[CB / 2], Cv[CB / 2];
-        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(row);
-        Bv[0] = v.x;
-        if constexpr (CB == 2) {
-          Cv[0] = v.y;
-        } else {
-          Bv[1] = v.y;
-          if (!STATE) {
-            const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(row + CB);
-            Cv[0] = w.x, Cv[1] = w.y;
-          }
-        }
+        load_bc_pairs<CB, !STATE>(row, Bv, Cv);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
           const f32x2 dd = pack2(d[k][i], d[k][i]), uu = pack2(u[k][i], u[k][i]);
@@ -333,7 +389,7 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
     // go to shared memory and are added where y is used
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      float* dst = &s_y[(ch + k * CK) * kLdy + 4 * t + (q & 3)];
+      float* dst = s_y + y_row(ch + k * CK) + 4 * t + (q & 3);
       if constexpr (LPC == 4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) dst[4 * i] = y[k][i];
@@ -358,8 +414,8 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
   for (int i = 0; i < tiles; ++i) {
     const int t0 = t_begin + i * kTile;
     const float* const s_du = s_stage + (i & 1) * Sh::kStage;
-    float* const s_y = s_stage + (i & 1) * Sh::kStage + kCh * kLdu;
-    const float* const s_bc = s_y + kCh * kLdy;
+    float* const s_y = s_stage + (i & 1) * Sh::kStage + 2 * kDu;
+    const T* const s_bc = reinterpret_cast<const T*>(s_y + kY);
     const uint32_t resets = a.seq ? reset_mask(a, b, t0, tid & 31) : 0u;
     bar_sync<1, NT>(i & 1);
     const int stop = min(kTile, t_end - t0);
@@ -370,7 +426,7 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
       }
       const int end = min(stop, half + SSD_TOKEN_SCAN_CHECKPOINT);
       if (resets == 0u) {
-#pragma unroll kUnroll
+#pragma unroll 1
         for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::false_type(), 0u);
       } else {
 #pragma unroll 1
@@ -392,6 +448,11 @@ __global__ void __launch_bounds__(ScanShape<LPC, NS, K>::kThreads, ScanShape<LPC
   }
 }
 
+// fp32 B and C pass shared memory in fp32 and need the sharing between two channels of a thread (3 x 777 x
+// 1536 channels of 64: 115 us against 167); 16-bit ones need the threads more (2 x 4096 x 5120 channels of
+// 16: 387 us against 422).
+constexpr int channels_per_thread(int elem) { return elem == 4 ? 2 : 1; }
+
 // How a problem is laid out over the GPU.
 struct ScanPlan {
   int lpc, ns, k, tiles_per_group, segments, seg_len;
@@ -404,17 +465,14 @@ ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
   const int64_t blocks = (int64_t)p.batch * p.ngroups * s.tiles_per_group;
   const int n = p.dstate <= 8 ? 8 : p.dstate <= 16 ? 16 : p.dstate <= 32 ? 32 : p.dstate <= 64 ? 64 : p.dstate <= 128 ? 128 : 256;
   s.lpc = n <= 16 ? 4 : n <= 32 ? 8 : 16;
-  s.k = SSD_SCAN_K;
+  s.k = channels_per_thread(dtype_size(p.x_dtype));
   s.ns = n / s.lpc;
-  // segments: only where the blocks leave most of the GPU idle, and none shorter than 256 positions
-  s.segments = 1;
-  const int64_t warps = blocks * s.lpc / (2 * s.k);
-  if (warps < 148 * 4) {
-    const int64_t want = (148 * 12 + warps - 1) / warps, room = p.seqlen / 256;
-    s.segments = (int)(want < room ? want : room);
-    if (s.segments > 128) s.segments = 128;
-    if (s.segments < 3) s.segments = 1;          // the state pass doubles the work
-  }
+  // segments: only where less than half of the blocks that fit the GPU at once would run, as many as fill
+  // it, and none shorter than 256 positions
+  const int64_t fit = 148 * resident(kCh * s.lpc / s.k + kHelpers, s.ns * s.k);
+  const int64_t want = fit / blocks, room = p.seqlen / 256;
+  s.segments = (int)(want < room ? want : room);
+  if (s.segments < 3) s.segments = 1;            // the state pass doubles the work
   s.seg_len = ((p.seqlen + s.segments - 1) / s.segments + kTile - 1) / kTile * kTile;
   s.segments = (p.seqlen + s.seg_len - 1) / s.seg_len;
   return s;
@@ -422,7 +480,7 @@ ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
 
 template <typename T, int LPC, int NS, int K, bool VEC>
 int launch_vec(const ScanArgs& a, int batch, cudaStream_t stream) {
-  using Sh = ScanShape<LPC, NS, K>;
+  using Sh = ScanShape<T, LPC, NS, K>;
   constexpr size_t smem = Sh::kSmem;
   dim3 grid(a.ngroups * a.tiles_per_group, a.segments, batch);
   if (smem > 48 * 1024) {
@@ -442,7 +500,7 @@ int launch_vec(const ScanArgs& a, int batch, cudaStream_t stream) {
 
 template <typename T, int LPC, int NS, int K>
 int launch_plan(const ScanArgs& a, const ssd_token_scan_params_t& p, cudaStream_t stream) {
-  using Sh = ScanShape<LPC, NS, K>;
+  using Sh = ScanShape<T, LPC, NS, K>;
   constexpr int CB = Sh::kChunk, EV = kVec;
   // a thread's vector of channels begins at a multiple of its length within a group
   constexpr size_t kMost = EV * sizeof(T) < 16 ? EV * sizeof(T) : 16;
@@ -472,6 +530,8 @@ ScanArgs scan_args(const ssd_token_scan_params_t& p) {
   a.seqlen = p.seqlen, a.channels = p.channels, a.ngroups = p.ngroups, a.dstate = p.dstate;
   a.per_group = p.channels / p.ngroups, a.tiles_per_group = 0;
   a.softplus = p.dt_softplus, a.dt_min = p.dt_min, a.dt_max = p.dt_max;
+  // whether clamping changes anything (a softplus is not negative)
+  a.limits = p.dt_max < INFINITY || !(p.dt_softplus ? p.dt_min <= 0.0f : p.dt_min == -INFINITY);
   a.x_sb = p.x_stride[0], a.x_sl = p.x_stride[1];
   a.dt_sb = p.dt_stride[0], a.dt_sl = p.dt_stride[1];
   a.z_sb = p.z_stride[0], a.z_sl = p.z_stride[1];
@@ -500,19 +560,14 @@ int launch_token_scan(const ssd_token_scan_params_t& p, cudaStream_t stream) {
   SSD_REQUIRE(p.batch <= 65535, SSD_ERR_UNSUPPORTED, "token scan: batch %d too large", p.batch);
   return with_type(p.x_dtype, [&](auto t) -> int {
     using T = decltype(t);
-    switch ((s.k * 100 + s.lpc) * 100 + s.ns) {
-      case 10402: return launch_plan<T, 4, 2, 1>(a, p, stream);
-      case 10404: return launch_plan<T, 4, 4, 1>(a, p, stream);
-      case 10804: return launch_plan<T, 8, 4, 1>(a, p, stream);
-      case 11604: return launch_plan<T, 16, 4, 1>(a, p, stream);
-      case 11608: return launch_plan<T, 16, 8, 1>(a, p, stream);
-      case 11616: return launch_plan<T, 16, 16, 1>(a, p, stream);
-      case 20402: return launch_plan<T, 4, 2, 2>(a, p, stream);
-      case 20404: return launch_plan<T, 4, 4, 2>(a, p, stream);
-      case 20804: return launch_plan<T, 8, 4, 2>(a, p, stream);
-      case 21604: return launch_plan<T, 16, 4, 2>(a, p, stream);
-      case 21608: return launch_plan<T, 16, 8, 2>(a, p, stream);
-      default: return launch_plan<T, 16, 16, 2>(a, p, stream);
+    constexpr int K = channels_per_thread(sizeof(T));
+    switch (s.lpc * 100 + s.ns) {
+      case 402: return launch_plan<T, 4, 2, K>(a, p, stream);
+      case 404: return launch_plan<T, 4, 4, K>(a, p, stream);
+      case 804: return launch_plan<T, 8, 4, K>(a, p, stream);
+      case 1604: return launch_plan<T, 16, 4, K>(a, p, stream);
+      case 1608: return launch_plan<T, 16, 8, K>(a, p, stream);
+      default: return launch_plan<T, 16, 16, K>(a, p, stream);
     }
   });
 }

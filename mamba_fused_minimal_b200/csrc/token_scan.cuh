@@ -24,7 +24,7 @@ struct ScanArgs {
   float2* seg_decay;     // (b, segments, d): (sum of dt', 0 where the segment drops what it was given, else 1)
   int dt_f32, A_dtype, D_dtype, bias_dtype, init_dtype;
   int seqlen, channels, ngroups, dstate, per_group, tiles_per_group;
-  int softplus;
+  int softplus, limits;
   float dt_min, dt_max;
   int64_t x_sb, x_sl, dt_sb, dt_sl, z_sb, z_sl;
   int64_t B_sb, B_sl, B_sg, C_sb, C_sl, C_sg;
@@ -50,6 +50,53 @@ __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
+// softplus_f and silu_f of a pair: the same operations in the same order
+__device__ __forceinline__ f32x2 softplus2(f32x2 v) {
+  float a, b, c, d;
+  unpack2(v, a, b);
+  const f32x2 e = pack2(ex2_approx(fabsf(a) * -1.4426950408889634f), ex2_approx(fabsf(b) * -1.4426950408889634f));
+  unpack2(add2(e, both(2.0f)), c, d);
+  const f32x2 s = mul2(e, pack2(rcp_approx(c), rcp_approx(d))), s2 = mul2(s, s);
+  f32x2 r = fma2(s2, both(1.0f / 13.0f), both(1.0f / 11.0f));
+  r = fma2(s2, r, both(1.0f / 9.0f));
+  r = fma2(s2, r, both(1.0f / 7.0f));
+  r = fma2(s2, r, both(1.0f / 5.0f));
+  r = fma2(s2, r, both(1.0f / 3.0f));
+  r = fma2(mul2(s, s2), r, s);
+  return fma2(both(2.0f), r, pack2(fmaxf(a, 0.0f), fmaxf(b, 0.0f)));
+}
+__device__ __forceinline__ f32x2 silu2(f32x2 v) {
+  float a, b;
+  unpack2(mul2(v, both(-1.4426950408889634f)), a, b);
+  unpack2(add2(both(1.0f), pack2(ex2_approx(a), ex2_approx(b))), a, b);
+  return mul2(v, pack2(rcp_approx(a), rcp_approx(b)));
+}
+// the two 16-bit elements of a word as fp32
+template <typename T> __device__ __forceinline__ f32x2 widen_pair(uint32_t w);
+template <> __device__ __forceinline__ f32x2 widen_pair<__nv_bfloat16>(uint32_t w) {
+  return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ f32x2 widen_pair<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pack2(f.x, f.y);
+}
+
+// elements 2 i and 2 i + 1 of a vector as fp32
+template <int V>
+__device__ __forceinline__ f32x2 pair_of(const Pack<float, V>& p, int i) { return pack2(p.e[2 * i], p.e[2 * i + 1]); }
+template <int V, typename T>
+__device__ __forceinline__ f32x2 pair_of(const Pack<T, V>& p, int i) {
+  uint32_t w;
+  memcpy(&w, &p.e[2 * i], 4);
+  return widen_pair<T>(w);
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 
 // V consecutive elements.  VEC: the vector is aligned and read as a whole, `count` or not -- the caller
@@ -68,10 +115,29 @@ __device__ __forceinline__ Pack<T, V> load_some(const T* p, int count) {
   }
   return t;
 }
+template <typename T> struct Pairs;
+template <> struct Pairs<float> {
+  static __device__ __forceinline__ void put(float* e, float a, float b) { e[0] = a, e[1] = b; }
+};
+template <> struct Pairs<__nv_bfloat16> {
+  static __device__ __forceinline__ void put(__nv_bfloat16* e, float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    memcpy(e, &v, 4);
+  }
+};
+template <> struct Pairs<__half> {
+  static __device__ __forceinline__ void put(__half* e, float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    memcpy(e, &v, 4);
+  }
+};
 template <int V, bool VEC, typename T>
 __device__ __forceinline__ void store_some(T* p, const float (&v)[V], int count) {
   if constexpr (VEC) {
-    if (count > 0) store_vec<V>(p, v);
+    Pack<T, V> t;
+#pragma unroll
+    for (int i = 0; i < V; i += 2) Pairs<T>::put(&t.e[i], v[i], v[i + 1]);
+    if (count > 0) *reinterpret_cast<Pack<T, V>*>(p) = t;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
