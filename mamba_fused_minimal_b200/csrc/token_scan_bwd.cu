@@ -16,7 +16,7 @@
 namespace ssd {
 namespace {
 
-constexpr int kBwdThreads = 512;
+constexpr int kBwdThreads = 256;      // two blocks an SM: one loads and sums while the other computes
 constexpr int kBwdWarps = kBwdThreads / 32;
 constexpr int kT = SSD_TOKEN_SCAN_CHECKPOINT;     // positions of a tile
 constexpr int kPitch = kT + 4;                    // row pitch in shared memory
@@ -34,9 +34,10 @@ struct ScanBwdArgs {
   float* part_D;       // (b, d)
   float* part_bias;    // (b, d)
   int64_t d_sb, d_sl;
+  int unit, unit32, unit_bc, unit_ck;   // bytes copied at a time of x and the like, of an fp32 dt, of B and C, of the states
 };
 
-template <int NP>
+template <typename T, int NP>
 struct BwdShape {
   static constexpr int kChannels = kBwdThreads / NP;              // channels of a block
   static constexpr int kSlabs = NP > 32 ? NP / 32 : 1;            // warps that share a channel
@@ -45,17 +46,54 @@ struct BwdShape {
   static constexpr int kPer = kItems > kBwdThreads ? kItems / kBwdThreads : 1;
   static constexpr int kBc = 2 * kT * NP;
   static constexpr int kPerBc = kBc > kBwdThreads ? kBc / kBwdThreads : 1;
-  static constexpr size_t kSmem = sizeof(float) * ((3 * kChannels + 2 * NP) * kPitch + 2 * kChannels * kSlabs * kPitch + kBwdWarps * kT * kRow);
+  // a tile as it lies in memory: x, dout, z, out_x (kItems elements each), B and C (kT rows of dstate), dt and
+  // the states before the tile (in 4 bytes)
+  static constexpr int kRaw16 = 4 * kItems + 2 * kT * NP, kRaw32 = kItems + kBwdThreads;
+  static constexpr size_t kRaw = (kRaw16 * sizeof(T) + kRaw32 * 4 + 15) / 16 * 16;
+  static constexpr size_t kSmem = 2 * kRaw + sizeof(float) * ((3 * kChannels + 2 * NP) * kPitch + 2 * kChannels * kSlabs * kPitch + kBwdWarps * kT * kRow);
 };
 
+// One warp copies `rows` rows of `bytes` bytes, `pitch` bytes apart, to rows of `to_pitch` bytes in shared
+// memory: asynchronously where rows and sizes are multiples of 4, 8 or 16 bytes (`unit`), else by elements
+// of `elem` bytes.  Row r stands for row min(r, last).
+__device__ __forceinline__ void copy_rows(char* to, int to_pitch, const char* from, int64_t pitch, int rows, int last, int bytes, int unit, int elem,
+                                          int lane) {
+  if (unit >= 4) {
+    const int per = bytes / unit;
+    for (int i = lane; i < rows * per; i += 32) {
+      const int r = i / per, k = (i - r * per) * unit;
+      const char* src = from + min(r, last) * pitch + k;
+      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to + r * to_pitch + k));
+      if (unit == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+      else if (unit == 8)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+      else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+    }
+  } else {
+    const int per = bytes / elem;
+    for (int i = lane; i < rows * per; i += 32) {
+      const int r = i / per, k = (i - r * per) * elem;
+      const char* src = from + min(r, last) * pitch + k;
+      char* dst = to + r * to_pitch + k;
+      if (elem == 4)
+        *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+      else
+        *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+    }
+  }
+}
+
 template <typename T, int NP>
-__global__ void __launch_bounds__(kBwdThreads) token_scan_bwd_kernel(ScanBwdArgs q) {
-  using Sh = BwdShape<NP>;
-  constexpr int CH = Sh::kChannels, SL = Sh::kSlabs, ROW = Sh::kRow, PER = Sh::kPer;
-  constexpr bool kAhead = NP <= 64;      // the tile before waits in registers while this one is computed
+__global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdArgs q) {
+  using Sh = BwdShape<T, NP>;
+  constexpr int NT = kBwdThreads, CH = Sh::kChannels, SL = Sh::kSlabs, ROW = Sh::kRow, PER = Sh::kPer, NBC = Sh::kPerBc;
+  constexpr int ES = sizeof(T);
   const ScanArgs& a = q.f;
   extern __shared__ float4 smem4[];
-  float* s_d = reinterpret_cast<float*>(smem4);      // [CH][kPitch] dt'
+  char* const s_raw = reinterpret_cast<char*>(smem4);        // [2][Sh::kRaw]
+  float* s_d = reinterpret_cast<float*>(s_raw + 2 * Sh::kRaw);      // [CH][kPitch] dt'
   float* s_u = s_d + CH * kPitch;                    // dt' x
   float* s_g = s_u + CH * kPitch;                    // dy
   float* s_B = s_g + CH * kPitch;                    // [NP][kPitch]
@@ -67,240 +105,284 @@ __global__ void __launch_bounds__(kBwdThreads) token_scan_bwd_kernel(ScanBwdArgs
   const int b = blockIdx.y;
   const int c0 = grp * a.per_group + tile_c * CH;
   const int nch = min(CH, a.per_group - tile_c * CH);
+  const int tiles = (a.seqlen + kT - 1) / kT;
+  const int last = (tiles - 1) * kT;                 // first position of the tile the walk begins with
 
-  // what this thread loads and stores: item i is position i / CH, channel i % CH
-  const int lc = tid % CH;
-  const float Dv = a.D && lc < nch ? load_f(a.D, a.D_dtype, c0 + lc) : 0.0f;
-  const float bias = a.bias && lc < nch ? load_f(a.bias, a.bias_dtype, c0 + lc) : 0.0f;
+  // The tiles' values come through two buffers of shared memory: the copies of the next tile are in flight
+  // while one is walked (held in registers they did not fit beside the walk: what was loaded was spilled,
+  // and so waited for at once).  A warp copies one tensor.
+  const auto fetch = [&](int t0, int buf) {
+    char* const raw = s_raw + buf * Sh::kRaw;
+    constexpr int kOne = Sh::kItems * ES, kBC = kT * NP * ES;
+    const int tail = a.seqlen - 1 - t0;
+    const int64_t row = (int64_t)b * a.seqlen + t0;
+    const auto rows = [&](int at, const void* base, int64_t off, int64_t sl, int es, int unit) {
+      copy_rows(raw + at, CH * es, static_cast<const char*>(base) + (off + (int64_t)t0 * sl + c0) * es, sl * es, kT, tail, nch * es, unit, es, lane);
+    };
+    if (warp == 0) rows(0, a.x, b * a.x_sb, a.x_sl, ES, q.unit);
+    if (warp == 1) rows(kOne, q.dout, b * q.d_sb, q.d_sl, ES, q.unit);
+    if (warp == 2 && a.z) rows(2 * kOne, a.z, b * a.z_sb, a.z_sl, ES, q.unit);
+    if (warp == 3 && a.z) rows(3 * kOne, a.out_x, (row - t0) * a.channels, a.channels, ES, q.unit);
+    if (warp == 4) rows(4 * kOne + 2 * kBC, a.dt, b * a.dt_sb, a.dt_sl, a.dt_f32 ? 4 : ES, a.dt_f32 ? q.unit32 : q.unit);
+    const int nb = a.dstate * ES;
+    if (warp == 5)
+      copy_rows(raw + 4 * kOne, NP * ES, static_cast<const char*>(a.B) + (b * a.B_sb + (int64_t)t0 * a.B_sl + grp * a.B_sg) * ES, a.B_sl * ES, kT,
+                tail, nb, q.unit_bc, ES, lane);
+    if (warp == 6)
+      copy_rows(raw + 4 * kOne + kBC, NP * ES, static_cast<const char*>(a.C) + (b * a.C_sb + (int64_t)t0 * a.C_sl + grp * a.C_sg) * ES, a.C_sl * ES,
+                kT, tail, nb, q.unit_bc, ES, lane);
+    if (warp == 7)
+      copy_rows(raw + Sh::kRaw16 * ES + Sh::kItems * 4, NP * 4,
+                reinterpret_cast<const char*>(a.ckpt + (((int64_t)b * tiles + t0 / kT) * a.channels + c0) * a.dstate), (int64_t)a.dstate * 4, nch, nch,
+                a.dstate * 4, q.unit_ck, 4, lane);
+  };
+
+  // what this thread prepares and stores: positions lt, lt + kStep, ... of the tile, channel lc
+  constexpr int kStep = NT / CH;
+  const int lt = tid / CH, lc = tid % CH;
+  const bool mine = Sh::kItems >= NT || tid < Sh::kItems, inc = lc < nch;
+  const int c = c0 + (inc ? lc : 0);
+  const float Dv = a.D ? load_f(a.D, a.D_dtype, c) : 0.0f;
+  const float bias = a.bias ? load_f(a.bias, a.bias_dtype, c) : 0.0f;
   float sum_D = 0.0f, sum_bias = 0.0f;
+  const int64_t own = (int64_t)b * a.seqlen * a.channels;       // of the contiguous tensors
 
   // what this thread computes
   const int n = tid % NP, ch = tid / NP;
   const bool has = ch < nch && n < a.dstate;
-  const float A = has ? load_f(a.A, a.A_dtype, (int64_t)(c0 + ch) * a.dstate + n) : 0.0f;
-  const float A2 = A * kLog2e;
-  const int64_t state_at = ((int64_t)b * a.channels + c0 + ch) * a.dstate + n;
-  float carry = has && q.dfinal ? q.dfinal[state_at] : 0.0f;      // a_{t+1} g_{t+1}
+  const int at_n = has ? (c0 + ch) * a.dstate + n : 0;            // of a (channels, dstate) tensor
+  const int64_t ck_step = (int64_t)a.channels * a.dstate;
+  const float A = has ? load_f(a.A, a.A_dtype, at_n) : 0.0f;
+  float carry = has && q.dfinal ? q.dfinal[b * ck_step + at_n] : 0.0f;      // a_{t+1} g_{t+1}
   float sum_A = 0.0f;
 
-  const int tiles = (a.seqlen + kT - 1) / kT;
-  // as they were loaded: nothing waits for them before they are used
-  T xr[PER], dr[PER], gr[PER], zr[PER], yr[PER], bcr[kAhead ? Sh::kPerBc : 1];
-  float dr32[PER], h_next = 0.0f;
-  const T zero = narrow<T>(0.0f);
-  const auto read = [&](const void* base, int64_t at) { return static_cast<const T*>(base)[at]; };
-  const auto load_bc = [&](int k, int t0) {
-    const int item = k * kBwdThreads + tid;
-    if (Sh::kBc < kBwdThreads && item >= Sh::kBc) return zero;
-    const int nn = item % NP, t = t0 + (item / NP) % kT;
-    const bool is_c = item >= kT * NP;
-    if (nn >= a.dstate || t >= a.seqlen) return zero;
-    return is_c ? read(a.C, b * a.C_sb + (int64_t)t * a.C_sl + grp * a.C_sg + nn) : read(a.B, b * a.B_sb + (int64_t)t * a.B_sl + grp * a.B_sg + nn);
-  };
-  const auto store_bc = [&](int k, T v) {
-    const int item = k * kBwdThreads + tid;
-    if (Sh::kBc < kBwdThreads && item >= Sh::kBc) return;
-    (item >= kT * NP ? s_C : s_B)[(item % NP) * kPitch + (item / NP) % kT] = widen(v);
-  };
-  const auto fetch = [&](int t0) {
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      const int item = e * kBwdThreads + tid, t = t0 + item / CH;
-      xr[e] = dr[e] = gr[e] = zr[e] = yr[e] = zero;
-      dr32[e] = 0.0f;
-      if (item >= Sh::kItems || t >= a.seqlen || lc >= nch) continue;
-      const int64_t c = c0 + lc;
-      xr[e] = read(a.x, b * a.x_sb + (int64_t)t * a.x_sl + c);
-      const int64_t dat = b * a.dt_sb + (int64_t)t * a.dt_sl + c;
-      if (a.dt_f32)
-        dr32[e] = static_cast<const float*>(a.dt)[dat];
-      else
-        dr[e] = read(a.dt, dat);
-      gr[e] = read(q.dout, b * q.d_sb + (int64_t)t * q.d_sl + c);
-      if (a.z) {
-        zr[e] = read(a.z, b * a.z_sb + (int64_t)t * a.z_sl + c);
-        yr[e] = read(a.out_x, ((int64_t)b * a.seqlen + t) * a.channels + c);
-      }
-    }
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int k = 0; k < Sh::kPerBc; ++k) bcr[k] = load_bc(k, t0);
-    }
-    if (has) h_next = a.ckpt[(((int64_t)b * tiles + t0 / kT) * a.channels + c0 + ch) * a.dstate + n];
-  };
+  // B and C: component bn of positions bt, bt + kBcStep, ...; the first half of the items is B (with eight
+  // components the first half of the threads takes B and the other C)
+  constexpr bool kOnce = NT / NP > kT;
+  constexpr int kBcStep = kOnce ? kT : NT / NP, kHalf = kT / kBcStep;
+  static_assert(kOnce ? NBC == 1 && NT / NP == 2 * kT : NBC == 2 * kHalf, "every component of a tile's B and C is taken once");
+  const int bn = tid % NP, bt = tid / NP % kT;
+  const bool second = kOnce && tid / NP >= kT;
+  const bool bin = bn < a.dstate;
 
-  fetch((tiles - 1) * kT);
-  for (int tile = tiles - 1; tile >= 0; --tile) {
-    const int t0 = tile * kT;
-    float d[PER], x[PER], dy[PER], raw[PER];
+  // the block's share of dB and dC: outputs o = k NT + tid; component on of kind oj, in the slabs and
+  // positions that k walks through
+  constexpr int kOuts = kT * SL * ROW / NT, kQ = NT / ROW, kSum = kBwdWarps / SL;
+  const int oq = tid / ROW, oj = tid % ROW;
+  const int64_t out_row = (int64_t)a.ngroups * a.tiles_per_group * 2 * a.dstate;
+  float* const part = q.part_bc + ((int64_t)b * a.seqlen * a.ngroups + grp) * a.tiles_per_group * (2 * a.dstate) + (int64_t)tile_c * 2 * a.dstate;
+  const int part_at = (oj / (ROW / 2)) * a.dstate + oj % (ROW / 2);
+
+  fetch(last, 0);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  int buf = 0;
+  for (int t0 = last; t0 >= 0; t0 -= kT, buf ^= 1) {
+    const T* const raw = reinterpret_cast<const T*>(s_raw + buf * Sh::kRaw);
+    const float* const raw32 = reinterpret_cast<const float*>(s_raw + buf * Sh::kRaw + Sh::kRaw16 * ES);
+    float d[PER], x[PER], dy[PER], slope[PER];         // slope: d dt' / d dt
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const int item = e * kBwdThreads + tid, lt = item / CH, t = t0 + lt;
-      if (item >= Sh::kItems) continue;
-      const bool in = t < a.seqlen && lc < nch;
-      x[e] = widen(xr[e]);
-      raw[e] = (a.dt_f32 ? dr32[e] : widen(dr[e])) + bias;
-      d[e] = in ? scan_dt(raw[e], a.softplus, a.dt_min, a.dt_max) : 0.0f;
-      dy[e] = widen(gr[e]);
-      if (a.z) {
-        const float zv = widen(zr[e]);
-        if (in) static_cast<T*>(q.dz)[((int64_t)b * a.seqlen + t) * a.channels + c0 + lc] = narrow<T>(dy[e] * widen(yr[e]) * dsilu_f(zv));
-        dy[e] *= silu_f(zv);
+      const int t = t0 + lt + e * kStep;
+      const bool in = mine && inc && t < a.seqlen;
+      const int item = mine ? (lt + e * kStep) * CH + lc : 0;
+      x[e] = in ? widen(raw[item]) : 0.0f;
+      d[e] = (a.dt_f32 ? raw32[item] : widen(reinterpret_cast<const T*>(raw32)[item])) + bias;
+      slope[e] = 1.0f;
+      if (a.softplus) {
+        slope[e] = sigmoid_f(d[e]);
+        d[e] = softplus_f(d[e]);
       }
-      s_d[lc * kPitch + lt] = d[e];
-      s_u[lc * kPitch + lt] = d[e] * x[e];
-      s_g[lc * kPitch + lt] = dy[e];
+      if (a.limits) {
+        if (d[e] < a.dt_min || d[e] > a.dt_max) slope[e] = 0.0f;
+        d[e] = fminf(fmaxf(d[e], a.dt_min), a.dt_max);
+      }
+      if (!in) d[e] = 0.0f;
+      dy[e] = in ? widen(raw[Sh::kItems + item]) : 0.0f;
+      if (a.z) {
+        const float zv = widen(raw[2 * Sh::kItems + item]), s = sigmoid_f(zv);
+        if (in) static_cast<T*>(q.dz)[own + (int64_t)t * a.channels + c] = 
+            narrow<T>(dy[e] * widen(raw[3 * Sh::kItems + item]) * (s * (1.0f + zv * (1.0f - s))));
+        dy[e] = in ? dy[e] * (zv * s) : 0.0f;
+      }
+      if (mine) {
+        const int at = lc * kPitch + lt + e * kStep;
+        s_d[at] = d[e];
+        s_u[at] = d[e] * x[e];
+        s_g[at] = dy[e];
+      }
       sum_D += dy[e] * x[e];
     }
-    if constexpr (kAhead) {
 #pragma unroll
-      for (int k = 0; k < Sh::kPerBc; ++k) store_bc(k, bcr[k]);
-    } else {
-#pragma unroll 4
-      for (int k = 0; k < Sh::kPerBc; ++k) store_bc(k, load_bc(k, t0));
+    for (int k = 0; k < NBC; ++k) {
+      const bool is_b = k < kHalf && !second;
+      const int t = bt + k % kHalf * kBcStep;
+      (is_b ? s_B : s_C)[bn * kPitch + t] = bin ? widen(raw[4 * Sh::kItems + (is_b ? t : kT + t) * NP + bn]) : 0.0f;
     }
-    float h = h_next;
+    float h = has ? raw32[Sh::kItems + ch * NP + n] : 0.0f;
     const uint32_t resets = a.seq ? reset_mask(a, b, t0, lane) : 0u;
     __syncthreads();
-    if (tile > 0) fetch(t0 - kT);
+    if (t0 > 0) fetch(t0 - kT, buf ^ 1);
 
-    // forwards through the tile: the decays, and what of the state before reaches each position
-    float dec[kT], kept[kT];
+    const auto walk = [&](auto reset) {
+      constexpr bool RESET = decltype(reset)::value;
+      // forwards through the tile: the decays, and what of the state before reaches each position
+      float dec[kT], kept[kT];
 #pragma unroll
-    for (int t = 0; t < kT; t += 4) {
-      const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
-      const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kPitch + t]);
-      const float4 B4 = *reinterpret_cast<const float4*>(&s_B[n * kPitch + t]);
-      const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w}, BB[4] = {B4.x, B4.y, B4.z, B4.w};
+      for (int t = 0; t < kT; t += 4) {
+        const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
+        const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kPitch + t]);
+        const float4 B4 = *reinterpret_cast<const float4*>(&s_B[n * kPitch + t]);
+        const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w}, BB[4] = {B4.x, B4.y, B4.z, B4.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        dec[t + i] = resets >> (t + i) & 1u ? 0.0f : ex2_approx(dd[i] * A2);
-        kept[t + i] = resets >> (t + i) & 1u ? 0.0f : dec[t + i] * h;
-        h = fmaf(uu[i], BB[i], kept[t + i]);
-      }
-    }
-    // and backwards
-#pragma unroll
-    for (int t = kT - 4; t >= 0; t -= 4) {
-      const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
-      const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kPitch + t]);
-      const float4 g4 = *reinterpret_cast<const float4*>(&s_g[ch * kPitch + t]);
-      const float4 B4 = *reinterpret_cast<const float4*>(&s_B[n * kPitch + t]);
-      const float4 C4 = *reinterpret_cast<const float4*>(&s_C[n * kPitch + t]);
-      const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w}, yy[4] = {g4.x, g4.y, g4.z, g4.w};
-      const float BB[4] = {B4.x, B4.y, B4.z, B4.w}, CC[4] = {C4.x, C4.y, C4.z, C4.w};
-      float p1[4], p2[4];
-#pragma unroll
-      for (int i = 3; i >= 0; --i) {
-        const float g = fmaf(CC[i], yy[i], carry);
-        const float vC = yy[i] * fmaf(uu[i], BB[i], kept[t + i]);
-        const float vB = g * uu[i];
-        const float m = g * kept[t + i];
-        p1[i] = g * BB[i];
-        p2[i] = m * A;
-        sum_A = fmaf(m, dd[i], sum_A);
-        carry = g * dec[t + i];
-        float* row = s_bc + (warp * kT + t + i) * ROW;
-        if constexpr (NP >= 32) {
-          row[lane] = vB;
-          row[32 + lane] = vC;
-        } else {
-          // lanes 0..15 keep dB, lanes 16..31 dC, of the channels 16 lanes apart
-          float v = (lane < 16 ? vB : vC) + __shfl_xor_sync(0xffffffffu, lane < 16 ? vC : vB, 16);
-          if constexpr (NP == 8) {
-            v += __shfl_xor_sync(0xffffffffu, v, 8);
-            if ((lane & 8) == 0) row[(lane >> 4) * 8 + (lane & 7)] = v;
-          } else {
-            row[lane] = v;
-          }
+        for (int i = 0; i < 4; ++i) {
+          dec[t + i] = ex2_approx(dd[i] * (A * kLog2e));
+          kept[t + i] = dec[t + i] * h;
+          if (RESET && (resets >> (t + i) & 1u)) dec[t + i] = kept[t + i] = 0.0f;
+          h = fmaf(uu[i], BB[i], kept[t + i]);
         }
       }
-      // eight sums (two kinds, four positions) over the channel's lanes: the lanes trade halves until each
-      // of eight holds one sum
-      const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
-      float w[4];
+      // and backwards
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = (b0 ? p2[i] : p1[i]) + __shfl_xor_sync(0xffffffffu, b0 ? p1[i] : p2[i], 1);
-      float v0 = (b1 ? w[1] : w[0]) + __shfl_xor_sync(0xffffffffu, b1 ? w[0] : w[1], 2);
-      float v1 = (b1 ? w[3] : w[2]) + __shfl_xor_sync(0xffffffffu, b1 ? w[2] : w[3], 2);
-      float r = (b2 ? v1 : v0) + __shfl_xor_sync(0xffffffffu, b2 ? v0 : v1, 4);
+      for (int t = kT - 4; t >= 0; t -= 4) {
+        const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
+        const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kPitch + t]);
+        const float4 g4 = *reinterpret_cast<const float4*>(&s_g[ch * kPitch + t]);
+        const float4 B4 = *reinterpret_cast<const float4*>(&s_B[n * kPitch + t]);
+        const float4 C4 = *reinterpret_cast<const float4*>(&s_C[n * kPitch + t]);
+        const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w}, yy[4] = {g4.x, g4.y, g4.z, g4.w};
+        const float BB[4] = {B4.x, B4.y, B4.z, B4.w}, CC[4] = {C4.x, C4.y, C4.z, C4.w};
+        float p1[4], p2[4];
 #pragma unroll
-      for (int off = 8; off < (NP < 32 ? NP : 32); off <<= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
-      if ((n & 31) < 8) s_p[(((lane & 1) * CH + ch) * SL + n / 32) * kPitch + t + ((lane >> 1) & 3)] = r;
-    }
+        for (int i = 3; i >= 0; --i) {
+          const float g = fmaf(CC[i], yy[i], carry);
+          const float vC = yy[i] * fmaf(uu[i], BB[i], kept[t + i]);
+          const float vB = g * uu[i];
+          const float m = g * kept[t + i];
+          p1[i] = g * BB[i];
+          p2[i] = m * A;
+          sum_A = fmaf(m, dd[i], sum_A);
+          carry = g * dec[t + i];
+          float* row = s_bc + (warp * kT + t + i) * ROW;
+          if constexpr (NP >= 32) {
+            row[lane] = vB;
+            row[32 + lane] = vC;
+          } else {
+            // lanes 0..15 keep dB, lanes 16..31 dC, of the channels 16 lanes apart
+            float v = (lane < 16 ? vB : vC) + __shfl_xor_sync(0xffffffffu, lane < 16 ? vC : vB, 16);
+            if constexpr (NP == 8) {
+              v += __shfl_xor_sync(0xffffffffu, v, 8);
+              if ((lane & 8) == 0) row[(lane >> 4) * 8 + (lane & 7)] = v;
+            } else {
+              row[lane] = v;
+            }
+          }
+        }
+        // eight sums (two kinds, four positions) over the channel's lanes: the lanes trade halves until each
+        // of eight holds one sum
+        const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (b0 ? p2[i] : p1[i]) + __shfl_xor_sync(0xffffffffu, b0 ? p1[i] : p2[i], 1);
+        float v0 = (b1 ? w[1] : w[0]) + __shfl_xor_sync(0xffffffffu, b1 ? w[0] : w[1], 2);
+        float v1 = (b1 ? w[3] : w[2]) + __shfl_xor_sync(0xffffffffu, b1 ? w[2] : w[3], 2);
+        float r = (b2 ? v1 : v0) + __shfl_xor_sync(0xffffffffu, b2 ? v0 : v1, 4);
+#pragma unroll
+        for (int off = 8; off < (NP < 32 ? NP : 32); off <<= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
+        if ((n & 31) < 8) s_p[(((lane & 1) * CH + ch) * SL + n / 32) * kPitch + t + ((lane >> 1) & 3)] = r;
+      }
+    };
+    if (resets == 0u)
+      walk(std::false_type());
+    else
+      walk(std::true_type());
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
 
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
-      const int item = e * kBwdThreads + tid, lt = item / CH, t = t0 + lt;
-      if (item >= Sh::kItems || t >= a.seqlen || lc >= nch) continue;
+      const int t = t0 + lt + e * kStep;
+      if (!mine || !inc || t >= a.seqlen) continue;
       float gB = 0.0f, gA = 0.0f;
 #pragma unroll
       for (int s = 0; s < SL; ++s) {
-        gB += s_p[(lc * SL + s) * kPitch + lt];
-        gA += s_p[((CH + lc) * SL + s) * kPitch + lt];
+        gB += s_p[(lc * SL + s) * kPitch + lt + e * kStep];
+        gA += s_p[((CH + lc) * SL + s) * kPitch + lt + e * kStep];
       }
-      float dd = x[e] * gB + gA;
-      if (a.softplus || a.dt_min > -INFINITY || a.dt_max < INFINITY) {
-        const float v = a.softplus ? softplus_f(raw[e]) : raw[e];
-        if (v < a.dt_min || v > a.dt_max) dd = 0.0f;
-        if (a.softplus) dd *= sigmoid_f(raw[e]);
-      }
+      const float dd = fmaf(x[e], gB, gA) * slope[e];
       sum_bias += dd;
-      const int64_t at = ((int64_t)b * a.seqlen + t) * a.channels + c0 + lc;
+      const int64_t at = own + (int64_t)t * a.channels + c;
       static_cast<T*>(q.dx)[at] = narrow<T>(fmaf(d[e], gB, Dv * dy[e]));
       if (a.dt_f32)
         static_cast<float*>(q.ddt)[at] = dd;
       else
         static_cast<T*>(q.ddt)[at] = narrow<T>(dd);
     }
-    // the block's share of dB and dC: over the warps (their channels) in order
-    constexpr int kOuts = kT * SL * ROW, kSum = kBwdWarps / SL;
-#pragma unroll 1
-    for (int o = tid; o < kOuts; o += kBwdThreads) {
-      const int j = o % ROW, slab = (o / ROW) % SL, t = o / (ROW * SL);
-      const int nn = slab * 32 + j % (ROW / 2);
-      if (nn >= a.dstate || t0 + t >= a.seqlen) continue;
+    // over the warps (their channels) in order
+#pragma unroll
+    for (int k = 0; k < kOuts; ++k) {
+      int slab, t;
+      if constexpr (kQ % SL == 0) {
+        slab = oq % SL;
+        t = k * (kQ / SL) + oq / SL;
+      } else {
+        constexpr int kTurn = SL / kQ;
+        slab = k % kTurn * kQ + oq;
+        t = k / kTurn;
+      }
+      if (slab * 32 + oj % (ROW / 2) >= a.dstate || t0 + t >= a.seqlen) continue;
       float v = 0.0f;
 #pragma unroll
-      for (int s = 0; s < kSum; ++s) v += s_bc[((s * SL + slab) * kT + t) * ROW + j];
-      q.part_bc[((((int64_t)b * a.seqlen + t0 + t) * a.ngroups + grp) * a.tiles_per_group + tile_c) * (2 * a.dstate) +
-                (j / (ROW / 2)) * a.dstate + nn] = v;
+      for (int s = 0; s < kSum; ++s) v += s_bc[((s * SL + slab) * kT + t) * ROW + oj];
+      part[(int64_t)(t0 + t) * out_row + part_at + slab * 32] = v;
     }
   }
 
   if (has) {
-    q.part_A[state_at] = sum_A;
-    if (q.dinit) q.dinit[state_at] = carry;
+    q.part_A[b * ck_step + at_n] = sum_A;
+    if (q.dinit) q.dinit[b * ck_step + at_n] = carry;
   }
   // dD and the bias's gradient: over the threads of a channel in order
   __syncthreads();
   s_bc[tid] = sum_D;
-  s_bc[kBwdThreads + tid] = sum_bias;
+  s_bc[NT + tid] = sum_bias;
   __syncthreads();
   if (tid < nch) {
     float u = 0.0f, v = 0.0f;
-    for (int s = tid; s < min(kBwdThreads, Sh::kItems); s += CH) u += s_bc[s], v += s_bc[kBwdThreads + s];
+    for (int s = tid; s < min(NT, Sh::kItems); s += CH) u += s_bc[s], v += s_bc[NT + s];
     q.part_D[(int64_t)b * a.channels + c0 + tid] = u;
     q.part_bias[(int64_t)b * a.channels + c0 + tid] = v;
   }
 }
 
-// dB and dC: over the blocks' shares in order.  One thread per (position, group, kind, component).
+// dB and dC of one (position, group): over the blocks' shares in order, eight strides of blocks side by side
+// joined in order (one thread a sum was bound by the latency of its chain of loads: 160 us for 4096
+// positions of 320 blocks).
 template <typename T>
 __global__ void __launch_bounds__(256) sum_bc_kernel(const float* part, T* dB, T* dC, int64_t rows, int tiles, int dstate) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= rows * 2 * dstate) return;
-  const int64_t row = i / (2 * dstate);
-  const int j = (int)(i - row * 2 * dstate);
-  const float* p = part + row * tiles * (2 * dstate) + j;
-  float v = 0.0f;
+  __shared__ float s[8][33];
+  const int64_t row = blockIdx.x;
+  const float* p = part + row * tiles * (2 * dstate);
+  for (int j0 = 0; j0 < 2 * dstate; j0 += 32) {
+    const int j = j0 + threadIdx.x;
+    float v = 0.0f;
+    if (j < 2 * dstate) {
 #pragma unroll 8
-  for (int k = 0; k < tiles; ++k) v += p[(int64_t)k * 2 * dstate];
-  if (j < dstate)
-    dB[row * dstate + j] = narrow<T>(v);
-  else
-    dC[row * dstate + j - dstate] = narrow<T>(v);
+      for (int k = threadIdx.y; k < tiles; k += 8) v += p[(int64_t)k * 2 * dstate + j];
+    }
+    s[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0 && j < 2 * dstate) {
+      float u = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u += s[k][threadIdx.x];
+      if (j < dstate)
+        dB[row * dstate + j] = narrow<T>(u);
+      else
+        dC[row * dstate + j - dstate] = narrow<T>(u);
+    }
+    __syncthreads();
+  }
 }
 
 // dA, dD and the bias's gradient: over the batch in order.
@@ -345,9 +427,28 @@ BwdWorkspace bwd_workspace(const ssd_token_scan_params_t& p) {
   return w;
 }
 
+// the largest of 16, 8 and 4 bytes that `bytes` is a multiple of, else 0
+int copy_unit(int64_t bytes) { return bytes % 16 == 0 ? 16 : bytes % 8 == 0 ? 8 : bytes % 4 == 0 ? 4 : 0; }
+template <typename... Ts>
+int copy_unit(int64_t first, int64_t second, Ts... more) {
+  const int u = copy_unit(first), v = copy_unit(second, more...);
+  return u < v ? u : v;
+}
+
 template <typename T, int NP>
-int launch_bwd(const ScanBwdArgs& q, int batch, cudaStream_t stream) {
-  constexpr size_t smem = BwdShape<NP>::kSmem;
+int launch_bwd(ScanBwdArgs& q, int batch, cudaStream_t stream) {
+  using Sh = BwdShape<T, NP>;
+  constexpr size_t smem = Sh::kSmem;
+  const ScanArgs& a = q.f;
+  const auto at = [](const void* p) { return (int64_t)(reinterpret_cast<uintptr_t>(p) & 15); };
+  constexpr int64_t es = sizeof(T);
+  // a block's channels begin at a multiple of its own within the group, and its last block ends with it
+  const int64_t ch = Sh::kChannels * es, pg = (int64_t)a.per_group * es;
+  q.unit = copy_unit(ch, pg, at(a.x), a.x_sb * es, a.x_sl * es, at(q.dout), q.d_sb * es, q.d_sl * es, at(a.z), a.z ? a.z_sb * es : 0, a.z ? a.z_sl * es : 0,
+                     at(a.out_x), a.channels * es, a.dt_f32 ? 0 : at(a.dt), a.dt_f32 ? 0 : a.dt_sb * es, a.dt_f32 ? 0 : a.dt_sl * es);
+  q.unit32 = copy_unit(Sh::kChannels * 4, (int64_t)a.per_group * 4, at(a.dt), a.dt_sb * 4, a.dt_sl * 4);
+  q.unit_bc = copy_unit(a.dstate * es, at(a.B), a.B_sb * es, a.B_sl * es, a.B_sg * es, at(a.C), a.C_sb * es, a.C_sl * es, a.C_sg * es);
+  q.unit_ck = copy_unit(a.dstate * 4, at(a.ckpt));
   if (smem > 48 * 1024)
     SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_bwd_kernel<T, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   token_scan_bwd_kernel<T, NP><<<dim3(q.f.ngroups * q.f.tiles_per_group, batch), kBwdThreads, smem, stream>>>(q);
@@ -374,7 +475,9 @@ int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t str
   q.part_D = ws + w.D;
   q.part_bias = q.part_D + (size_t)p.batch * p.channels;
   q.d_sb = r.dout_stride[0], q.d_sl = r.dout_stride[1];
-  SSD_REQUIRE(p.batch <= 65535, SSD_ERR_UNSUPPORTED, "token scan: batch %d too large", p.batch);
+  SSD_REQUIRE(p.batch <= 65535 && (int64_t)p.batch * p.seqlen * p.ngroups <= 0x7fffffff, SSD_ERR_UNSUPPORTED,
+              "token scan: batch %d, seqlen %d or ngroups %d too large", p.batch, p.seqlen, p.ngroups);
+  SSD_REQUIRE((int64_t)p.channels * p.dstate <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "token scan: %d channels of %d too many", p.channels, p.dstate);
   return with_type(p.x_dtype, [&](auto t) -> int {
     using T = decltype(t);
     int rc;
@@ -387,9 +490,9 @@ int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t str
       default: rc = launch_bwd<T, 256>(q, p.batch, stream); break;
     }
     if (rc != SSD_OK) return rc;
-    const int64_t rows = (int64_t)p.batch * p.seqlen * p.ngroups, outs = rows * 2 * p.dstate;
-    sum_bc_kernel<T><<<(unsigned)((outs + 255) / 256), 256, 0, stream>>>(q.part_bc, static_cast<T*>(r.dB), static_cast<T*>(r.dC), rows,
-                                                                       q.f.tiles_per_group, p.dstate);
+    const int64_t rows = (int64_t)p.batch * p.seqlen * p.ngroups;
+    sum_bc_kernel<T><<<(unsigned)rows, dim3(32, 8), 0, stream>>>(q.part_bc, static_cast<T*>(r.dB), static_cast<T*>(r.dC), rows,
+                                                               q.f.tiles_per_group, p.dstate);
     SSD_CUDA_OK(cudaGetLastError());
     const int64_t par = (int64_t)p.channels * (p.dstate + 2);
     sum_batch_kernel<<<(unsigned)((par + 255) / 256), 256, 0, stream>>>(q, p.batch, r.dA, r.dD, r.ddt_bias);
