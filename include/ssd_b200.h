@@ -609,7 +609,7 @@ SSD_API int ssd_token_scan_bwd(const ssd_token_scan_bwd_params_t* prm, ssd_strea
  *    final_states of the chunk kernels) and a decay for each channel and component (headdim 1).
  *    state_indices: as for ssd_short_conv_step. */
 typedef struct {
-  void* state;               /* (slots, h, p, n) of state_dtype, n contiguous */
+  void* state;               /* (slots, h, p, n) of state_dtype (x_dtype or SSD_F32), n contiguous */
   const void* x;             /* (b, h, p) of x_dtype */
   const void* dt;            /* (b, h) of dt_dtype */
   const void* A;             /* (h, n) of A_dtype */

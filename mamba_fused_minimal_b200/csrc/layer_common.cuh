@@ -57,6 +57,21 @@ __device__ __forceinline__ void load_param(const void* base, int dtype, int64_t 
   for (int i = 0; i < V; ++i) v[i] = load_f(base, dtype, idx + i);
 }
 
+// One parameter of any of the three types in two steps: `load` issues it -- into one register or the other,
+// with no branch that would wait for it -- and `value` converts it where it is used.
+struct AnyParam {
+  uint32_t w = 0;
+  uint16_t h = 0;
+  __device__ __forceinline__ void load(const void* base, int dtype, int64_t idx) {
+    if (dtype == SSD_F32) w = static_cast<const uint32_t*>(base)[idx];
+    if (dtype != SSD_F32) h = static_cast<const uint16_t*>(base)[idx];
+  }
+  __device__ __forceinline__ float value(int dtype) const {
+    const float b = __uint_as_float((uint32_t)h << 16), f = __half2float(__ushort_as_half(h));
+    return dtype == SSD_F32 ? __uint_as_float(w) : dtype == SSD_BF16 ? b : f;
+  }
+};
+
 // ---- activations -----------------------------------------------------------------------------------
 __device__ __forceinline__ float rcp_approx(float v) {
   float r;
@@ -85,7 +100,7 @@ __device__ __forceinline__ float softplus_f(float v) {
   r = fmaf(s * s2, r, s);
   return fmaf(2.0f, r, fmaxf(v, 0.0f));          // r is a NaN where v is
 }
-// dt' of one position and channel, and the factor of its gradient
+// dt' of one position and channel
 __device__ __forceinline__ float scan_dt(float raw, bool softplus, float lo, float hi) {
   const float v = softplus ? softplus_f(raw) : raw;
   return fminf(fmaxf(v, lo), hi);

@@ -13,9 +13,10 @@ namespace ssd {
 namespace {
 
 constexpr int kConvThreads = 128;
-constexpr int kFwdStrip = 32;     // positions of a forward strip
-constexpr int kBwdStrip = 64;     // positions of a gradient strip: fewer partial sums of the weights
-constexpr int kAhead = 8;         // positions whose loads are in flight together
+constexpr int kGroup = 8;         // positions whose loads are issued together, one group ahead of their use
+constexpr int kFwdStrip = 64;     // positions of a forward strip
+// positions of a gradient strip: with the width - 1 behind it a whole number of groups
+__host__ __device__ constexpr int bwd_strip(int width) { return 64 - (width - 1); }
 
 struct ConvArgs {
   const void* x;
@@ -61,6 +62,9 @@ __device__ __forceinline__ void load_input(const ConvArgs& a, const T* x, int b,
   }
 }
 
+// Channels are contiguous, so a thread takes V of them; 8 bytes a load leave the registers for eight loads in
+// flight and the next eight behind them.  Every load is unconditional (the position is clamped to the strip):
+// one under a condition would be waited for at once.
 template <typename T, int W, int V, bool SEQ>
 __global__ void __launch_bounds__(kConvThreads) short_conv_fwd_kernel(ConvArgs a) {
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
@@ -70,61 +74,75 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_fwd_kernel(ConvArgs a
   const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
   T* out = static_cast<T*>(a.out) + ((int64_t)b * a.seqlen) * a.channels + c;
   const int64_t sbase = SEQ ? b * a.s_sb : 0;
+  Pack<T, V> next[kGroup];
+  int next_id[kGroup];
+  const auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) {
+      const int at = min(t + u, t1 - 1);
+      next[u] = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)at * a.x_sl);
+      next_id[u] = SEQ ? seq_at(a, sbase, at) : 0;
+    }
+  };
+  fetch(t0);
   float wr[W][V], bs[V];
   load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, c, wr, bs);
-  float win[W - 1][V];                 // win[j] = x[t - 1 - j]
-  int id[W - 1];
+  float v[W - 1 + kGroup][V];          // v[W - 1 + u] = x[t + u], before it the last width - 1 inputs
+  int id[W - 1 + kGroup];
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    load_input<T, W, V>(a, x, b, c, t0 - 1 - j, win[j]);
-    id[j] = SEQ ? seq_at(a, sbase, t0 - 1 - j) : 0;
+    load_input<T, W, V>(a, x, b, c, t0 - (W - 1) + j, v[j]);
+    id[j] = SEQ ? seq_at(a, sbase, t0 - (W - 1) + j) : 0;
   }
-  for (int t = t0; t < t1; t += kAhead) {
-    float cur[kAhead][V];
-    int cid[kAhead];
+  for (int t = t0; t < t1; t += kGroup) {
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (t + u < t1) {
-        load_vec<V>(x + (int64_t)(t + u) * a.x_sl, cur[u]);
-        cid[u] = SEQ ? seq_at(a, sbase, t + u) : 0;
-      }
+    for (int u = 0; u < kGroup; ++u) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[W - 1 + u][i] = widen(next[u].e[i]);
+      id[W - 1 + u] = next_id[u];
     }
+    if (t + kGroup < t1) fetch(t + kGroup);
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (t + u >= t1) break;
+    for (int u = 0; u < kGroup; ++u) {
       float y[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        float acc = fmaf(wr[0][i], cur[u][i], bs[i]);
+        float acc = fmaf(wr[0][i], v[W - 1 + u][i], bs[i]);
 #pragma unroll
         for (int j = 1; j < W; ++j) {
           // the value j positions back, masked where it belongs to another sequence (a select: what is
           // masked may be an infinity or a NaN)
-          const float past = !SEQ || id[j - 1] == cid[u] ? win[j - 1][i] : 0.0f;
+          const float past = !SEQ || id[W - 1 + u - j] == id[W - 1 + u] ? v[W - 1 + u - j][i] : 0.0f;
           acc = fmaf(wr[j][i], past, acc);
         }
-        y[i] = a.silu ? silu_f(acc) : acc;
+        y[i] = acc;
       }
-      store_vec<V>(out + (int64_t)(t + u) * a.channels, y);
+      if (a.silu) {
 #pragma unroll
-      for (int j = W - 2; j > 0; --j) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) win[j][i] = win[j - 1][i];
-        id[j] = id[j - 1];
+        for (int i = 0; i < V; ++i) y[i] = silu_f(y[i]);
       }
+      if (t + u < t1) store_vec<V>(out + (int64_t)(t + u) * a.channels, y);
+    }
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[0][i] = cur[u][i];
-      id[0] = cid[u];
+    for (int j = 0; j < W - 1; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = v[kGroup + j][i];
+      id[j] = id[kGroup + j];
     }
   }
   if (a.final_states != nullptr && t1 == a.seqlen) {
     T* fin = static_cast<T*>(a.final_states) + (int64_t)b * (W - 1) * a.channels + c;
+    const int last = SEQ ? seq_at(a, sbase, a.seqlen - 1) : 0;
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) {          // win[j] = x[seqlen - 1 - j]
-      float v[V];
+    for (int j = 0; j < W - 1; ++j) {
+      const int t = a.seqlen - (W - 1) + j;
+      float y[V];
+      load_input<T, W, V>(a, x, b, c, t, y);
+      if (SEQ && seq_at(a, sbase, t) != last) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] = !SEQ || id[j] == id[0] ? win[j][i] : 0.0f;
-      store_vec<V>(fin + (int64_t)(W - 2 - j) * a.channels, v);
+        for (int i = 0; i < V; ++i) y[i] = 0.0f;
+      }
+      store_vec<V>(fin + (int64_t)j * a.channels, y);
     }
   }
 }
@@ -140,100 +158,118 @@ struct ConvBwdArgs {
   int64_t d_sb, d_sl;
 };
 
-// A strip walks its positions and the width - 1 behind it (whose dpre its last dx need); dx of a
-// position is complete once dpre of the width - 1 positions after it is known.
+// A strip walks its positions and the width - 1 behind it (whose dpre its last dx need), in groups whose
+// loads are issued one group ahead; dx of a position is complete once dpre of the width - 1 positions after it
+// is known.
 template <typename T, int W, int V, bool SEQ>
 __global__ void __launch_bounds__(kConvThreads) short_conv_bwd_kernel(ConvBwdArgs g) {
   const ConvArgs& a = g.f;
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
   const int b = blockIdx.z;
-  const int t0 = blockIdx.y * kBwdStrip, t1 = min(t0 + kBwdStrip, a.seqlen);
+  const int t0 = blockIdx.y * bwd_strip(W), t1 = min(t0 + bwd_strip(W), a.seqlen);
   const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
   const T* dout = static_cast<const T*>(g.dout) + b * g.d_sb + c;
   T* dx = static_cast<T*>(g.dx) + ((int64_t)b * a.seqlen) * a.channels + c;
   const int64_t sbase = SEQ ? b * a.s_sb : 0;
   const int last_id = SEQ ? seq_at(a, sbase, a.seqlen - 1) : 0;
-  float wr[W][V], bs[V];
+  Pack<T, V> next[kGroup], next_d[kGroup];
+  int next_id[kGroup];
+  const auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) {
+      const int at = min(t + u, a.seqlen - 1);
+      next[u] = *reinterpret_cast<const Pack<T, V>*>(x + (int64_t)at * a.x_sl);
+      next_d[u] = *reinterpret_cast<const Pack<T, V>*>(dout + (int64_t)at * g.d_sl);
+      next_id[u] = SEQ ? seq_at(a, sbase, at) : 0;
+    }
+  };
+  fetch(t0);
+  float wr[W][V], bs[V], dw[W][V], db[V];
   load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, c, wr, bs);
-  float win[W][V], dp[W][V], dw[W][V], db[V];       // win[j] = x[t - j], dp[j] = dpre[t - j]
-  int id[W];
+  float v[W - 1 + kGroup][V], dp[W - 1 + kGroup][V];       // x and dpre; [W - 1 + u] is position t + u
+  int id[W - 1 + kGroup];
   const bool first = t0 == 0;
 #pragma unroll
-  for (int j = 0; j < W; ++j) {
+  for (int i = 0; i < V; ++i) {
+    db[i] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) dp[j][i] = dw[j][i] = win[j][i] = 0.0f;
-    id[j] = 0;
+    for (int j = 0; j < W; ++j) dw[j][i] = 0.0f;
   }
-#pragma unroll
-  for (int i = 0; i < V; ++i) db[i] = 0.0f;
 #pragma unroll
   for (int j = 0; j < W - 1; ++j) {
-    load_input<T, W, V>(a, x, b, c, t0 - 1 - j, win[j]);
-    id[j] = SEQ ? seq_at(a, sbase, t0 - 1 - j) : 0;
+    load_input<T, W, V>(a, x, b, c, t0 - (W - 1) + j, v[j]);
+    id[j] = SEQ ? seq_at(a, sbase, t0 - (W - 1) + j) : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) dp[j][i] = 0.0f;           // not of this strip, and zero before the first position
   }
-  // t runs width - 1 positions past the strip, to its end or the sequence's: behind the sequence's end
-  // dpre is zero
-  for (int t = t0; t < t1 + W - 1; ++t) {
-    float in[V], d[V];
-    int now = 0;
-    const bool inside = t < a.seqlen;
-    if (inside) {
-      load_vec<V>(x + (int64_t)t * a.x_sl, in);
-      load_vec<V>(dout + (int64_t)t * g.d_sl, d);
-      now = SEQ ? seq_at(a, sbase, t) : 0;
-    } else {
+  for (int t = t0; t < t1 + W - 1; t += kGroup) {
+    Pack<T, V> d[kGroup];
 #pragma unroll
-      for (int i = 0; i < V; ++i) in[i] = d[i] = 0.0f;
+    for (int u = 0; u < kGroup; ++u) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[W - 1 + u][i] = widen(next[u].e[i]);
+      d[u] = next_d[u];
+      id[W - 1 + u] = next_id[u];
     }
+    if (t + kGroup < t1 + W - 1) fetch(t + kGroup);
 #pragma unroll
-    for (int j = W - 1; j > 0; --j) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) win[j][i] = win[j - 1][i], dp[j][i] = dp[j - 1][i];
-      id[j] = id[j - 1];
-    }
-    id[0] = now;
-#pragma unroll
-    for (int i = 0; i < V; ++i) win[0][i] = in[i];
-    const bool own = t < t1;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float acc = fmaf(wr[0][i], in[i], bs[i]);
-#pragma unroll
-      for (int j = 1; j < W; ++j) acc = fmaf(wr[j][i], !SEQ || id[j] == now ? win[j][i] : 0.0f, acc);
-      const float v = inside ? (a.silu ? d[i] * dsilu_f(acc) : d[i]) : 0.0f;
-      dp[0][i] = v;
-      if (own) {
-        db[i] += v;
-        dw[0][i] += v * in[i];
-#pragma unroll
-        for (int j = 1; j < W; ++j) dw[j][i] += v * (!SEQ || id[j] == now ? win[j][i] : 0.0f);
-      }
-    }
-    // the position width - 1 back: dx[s] = sum_j wr[j] dpre[s + j]; s + j lies j behind s in the window
-    const int s = t - (W - 1);
-    if (s >= t0 || (first && g.dinit != nullptr)) {
-      float r[V];
+    for (int u = 0; u < kGroup; ++u) {
+      const int at = W - 1 + u, now = t + u;
+      float pre[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        r[i] = 0.0f;
+        pre[i] = fmaf(wr[0][i], v[at][i], bs[i]);
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          // before the first position there is no dpre, and behind the last one it is zero
-          if (s + j >= 0 && s + j < a.seqlen && (!SEQ || id[W - 1] == id[W - 1 - j])) r[i] = fmaf(wr[j][i], dp[W - 1 - j][i], r[i]);
+        for (int j = 1; j < W; ++j) pre[i] = fmaf(wr[j][i], !SEQ || id[at - j] == id[at] ? v[at - j][i] : 0.0f, pre[i]);
+        dp[at][i] = widen(d[u].e[i]);
+      }
+      if (a.silu) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) dp[at][i] *= dsilu_f(pre[i]);
+      }
+      if (now >= a.seqlen) {                               // behind the last position there is no dpre
+#pragma unroll
+        for (int i = 0; i < V; ++i) dp[at][i] = 0.0f;
+      }
+      if (now < t1) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          db[i] += dp[at][i];
+          dw[0][i] = fmaf(dp[at][i], v[at][i], dw[0][i]);
+#pragma unroll
+          for (int j = 1; j < W; ++j) dw[j][i] = fmaf(dp[at][i], !SEQ || id[at - j] == id[at] ? v[at - j][i] : 0.0f, dw[j][i]);
         }
       }
-      const int k = s - (a.seqlen - (W - 1));
-      if (g.dfinal != nullptr && k >= 0 && (!SEQ || id[W - 1] == last_id)) {
-        float u[V];
-        load_vec<V>(static_cast<const T*>(g.dfinal) + ((int64_t)b * (W - 1) + k) * a.channels + c, u);
+      // the position width - 1 back, s, at u in the window: dx[s] = sum_j wr[j] dpre[s + j]
+      const int s = now - (W - 1);
+      if ((s >= t0 || (first && g.dinit != nullptr)) && s < t1) {
+        float r[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) r[i] += u[i];
+        for (int i = 0; i < V; ++i) {
+          r[i] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < W; ++j)
+            if (!SEQ || s + j >= a.seqlen || id[u] == id[u + j]) r[i] = fmaf(wr[j][i], dp[u + j][i], r[i]);
+        }
+        const int k = s - (a.seqlen - (W - 1));
+        if (g.dfinal != nullptr && k >= 0 && (!SEQ || id[u] == last_id)) {
+          float f[V];
+          load_vec<V>(static_cast<const T*>(g.dfinal) + ((int64_t)b * (W - 1) + k) * a.channels + c, f);
+#pragma unroll
+          for (int i = 0; i < V; ++i) r[i] += f[i];
+        }
+        if (s >= 0)
+          store_vec<V>(dx + (int64_t)s * a.channels, r);
+        else
+          store_vec<V>(static_cast<T*>(g.dinit) + ((int64_t)b * (W - 1) + (s + W - 1)) * a.channels + c, r);
       }
-      if (s >= 0)
-        store_vec<V>(dx + (int64_t)s * a.channels, r);
-      else
-        store_vec<V>(static_cast<T*>(g.dinit) + ((int64_t)b * (W - 1) + (s + W - 1)) * a.channels + c, r);
+    }
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[j][i] = v[kGroup + j][i], dp[j][i] = dp[kGroup + j][i];
+      id[j] = id[kGroup + j];
     }
   }
   float* part = g.partial + ((int64_t)(blockIdx.z * gridDim.y + blockIdx.y) * (W + 1)) * a.channels + c;
@@ -356,9 +392,10 @@ int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream)
   SSD_REQUIRE(strips <= 65535 && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv: seqlen %d or batch %d too large", p.seqlen, p.batch);
   return with_type(p.x_dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = p.channels % V == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), 16) && aligned_to(p.out, 16) &&
-                     aligned_to(p.initial_states, 16) && aligned_to(p.final_states, 16);
+    constexpr int V = 4;
+    constexpr size_t kBytes = V * sizeof(T);
+    const bool vec = p.channels % V == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), kBytes) && aligned_to(p.out, kBytes) &&
+                     aligned_to(p.initial_states, kBytes) && aligned_to(p.final_states, kBytes);
     return with_width(p.width, [&](auto w) {
       constexpr int W = decltype(w)::value;
       const auto go = [&](auto v, auto s) -> int {
@@ -377,7 +414,7 @@ int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream)
 }
 
 size_t short_conv_bwd_workspace(const ssd_short_conv_bwd_params_t& p) {
-  return (size_t)p.conv.batch * strips_of(p.conv.seqlen, kBwdStrip) * (p.conv.width + 1) * p.conv.channels * sizeof(float);
+  return (size_t)p.conv.batch * strips_of(p.conv.seqlen, bwd_strip(p.conv.width)) * (p.conv.width + 1) * p.conv.channels * sizeof(float);
 }
 
 int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& q, cudaStream_t stream) {
@@ -390,11 +427,11 @@ int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& q, cudaStream_t str
   g.dinit = q.dinitial_states;
   g.partial = static_cast<float*>(q.workspace);
   g.d_sb = q.dout_stride[0], g.d_sl = q.dout_stride[1];
-  const int strips = strips_of(p.seqlen, kBwdStrip);
+  const int strips = strips_of(p.seqlen, bwd_strip(p.width));
   SSD_REQUIRE(strips <= 65535 && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv: seqlen %d or batch %d too large", p.seqlen, p.batch);
   return with_type(p.x_dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = 4;
+    constexpr int V = 2;
     constexpr size_t kBytes = V * sizeof(T);
     const bool vec = p.channels % V == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), kBytes) &&
                      rows_aligned(q.dout, q.dout_stride, 2, sizeof(T), kBytes) && aligned_to(q.dx, kBytes) &&

@@ -524,6 +524,7 @@ int ssd_token_scan_step(const ssd_token_scan_step_params_t* prm, ssd_stream_t st
   SSD_REQUIRE(valid_dtype(p.state_dtype) && valid_dtype(p.x_dtype) && valid_dtype(p.dt_dtype) && valid_dtype(p.A_dtype) &&
                   absent_or_valid(p.D, p.D_dtype) && absent_or_valid(p.dt_bias, p.bias_dtype),
               SSD_ERR_BAD_ARGUMENT, "bad dtype");
+  SSD_REQUIRE(p.state_dtype == p.x_dtype || p.state_dtype == SSD_F32, SSD_ERR_UNSUPPORTED, "the state must have x's dtype or be fp32");
   SSD_REQUIRE(p.batch > 0 && p.slots > 0 && p.nheads > 0 && p.headdim > 0 && p.ngroups > 0 && p.dstate > 0, SSD_ERR_BAD_ARGUMENT,
               "sizes must be positive");
   SSD_REQUIRE(p.nheads % p.ngroups == 0, SSD_ERR_BAD_ARGUMENT, "nheads %d not a multiple of ngroups %d", p.nheads, p.ngroups);
