@@ -40,12 +40,35 @@ __device__ __forceinline__ void store_out(void* base, int64_t idx, const float (
     for (int i = 0; i < V; ++i) t.e[i] = (int8_t)max(-127, min(127, __float2int_rn(y[i] * inv)));
     *reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(base) + idx) = t;
   } else if constexpr (std::is_same<O, E4M3>::value) {
-    Pack<uint8_t, V> t;
+    float q[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) t.e[i] = __nv_cvt_float_to_fp8(y[i] * inv, __NV_SATFINITE, __NV_E4M3);
-    *reinterpret_cast<Pack<uint8_t, V>*>(static_cast<uint8_t*>(base) + idx) = t;
+    for (int i = 0; i < V; ++i) q[i] = inv;
+    vec_mul(q, y);
+    if constexpr (V % 2 == 0) {
+      Pack<uint16_t, V / 2> t;
+#pragma unroll
+      for (int i = 0; i < V; i += 2) t.e[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(q[i], q[i + 1]), __NV_SATFINITE, __NV_E4M3);
+      *reinterpret_cast<Pack<uint16_t, V / 2>*>(static_cast<uint8_t*>(base) + idx) = t;
+    } else {
+      static_cast<uint8_t*>(base)[idx] = __nv_cvt_float_to_fp8(q[0], __NV_SATFINITE, __NV_E4M3);
+    }
   } else {
     store_vec<V>(static_cast<O*>(base) + idx, y);
+  }
+}
+
+// w = v rounded to R
+template <typename R, int V>
+__device__ __forceinline__ void round_all(const float (&v)[V], float (&w)[V]) {
+  Pack<R, V> t;
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      Pairs<R>::put(&t.e[i], v[i], v[i + 1]);
+      unpack2(pair_of(t, i / 2), w[i], w[i + 1]);
+    }
+  } else {
+    w[0] = widen(narrow<R>(v[0]));
   }
 }
 
@@ -68,43 +91,57 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
     if (res) {
       float u[V];
       load_vec<V>(res + col, u);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] += u[i];
+      vec_add(v, u);
     }
   };
   // two sums of squares: of t, which y is made of, and of t as it is kept, whose rstd the gradients use
   // (they see nothing but what was kept)
-  float sum = 0.0f, kept = 0.0f;
+  float sums[V], kepts[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[i] = kepts[i] = 0.0f;
   constexpr bool kRounds = sizeof(R) < 4;
   const auto square = [&](const float (&v)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      sum += v[i] * v[i];
-      if (kRounds) {
-        const float w = widen(narrow<R>(v[i]));
-        kept += w * w;
-      }
+    vec_fma(v, v, sums);
+    if constexpr (kRounds) {
+      float w[V];
+      round_all<R>(v, w);
+      vec_fma(w, w, kepts);
     }
   };
-  if (kHold) {
+  if constexpr (kHold) {
+    // all of the row's loads first, none of them under a condition that would be waited for: columns past
+    // the end read the last ones and become zero
+    Pack<T, V> xr[VPT];
+    Pack<R, V> rr[VPT];
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) xr[k] = *reinterpret_cast<const Pack<T, V>*>(x + min((int)(k * blockDim.x + threadIdx.x) * V, a.dim - V));
+    if (res) {
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) rr[k] = *reinterpret_cast<const Pack<R, V>*>(res + min((int)(k * blockDim.x + threadIdx.x) * V, a.dim - V));
+    }
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int col = (k * blockDim.x + threadIdx.x) * V;
-      if (col < a.dim) {
-        fetch(col, t[k]);
-      } else {
+      widen_all(xr[k], t[k]);
+      if (res) {
+        float u[V];
+        widen_all(rr[k], u);
+        vec_add(t[k], u);
+      }
+      if ((int)(k * blockDim.x + threadIdx.x) * V >= a.dim) {
 #pragma unroll
         for (int i = 0; i < V; ++i) t[k][i] = 0.0f;
       }
+      square(t[k]);
     }
-#pragma unroll
-    for (int k = 0; k < VPT; ++k) square(t[k]);
   } else {
     for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
       fetch(col, t[0]);
       square(t[0]);
     }
   }
+  float sum = sums[0], kept = kepts[0];
+#pragma unroll
+  for (int i = 1; i < V; ++i) sum += sums[i], kept += kepts[i];
   if (kRounds) {
     block_reduce2(sum, kept, slots);
   } else {
@@ -118,8 +155,11 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
     if (keep && a.residual_out) store_vec<V>(static_cast<R*>(a.residual_out) + obase + col, v);
     float w[V];
     load_param<V>(a.weight, a.weight_dtype, col, w);
+    float rr[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = v[i] * r * w[i];
+    for (int i = 0; i < V; ++i) rr[i] = r;
+    vec_mul(v, rr);
+    vec_mul(v, w);
   };
   if constexpr (!kScaled) {
     if (kHold) {
@@ -280,13 +320,17 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_bwd_kernel(NormBwdAr
     }
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
+      float s[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        hat[k][i] *= r;
-        dw[k][i] += g[k][i] * hat[k][i];
-        g[k][i] *= w[k][i];
-        sum += g[k][i] * hat[k][i];
-      }
+      for (int i = 0; i < V; ++i) s[i] = r;
+      vec_mul(hat[k], s);
+      vec_fma(g[k], hat[k], dw[k]);
+      vec_mul(g[k], w[k]);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = 0.0f;
+      vec_fma(g[k], hat[k], s);
+#pragma unroll
+      for (int i = 0; i < V; ++i) sum += s[i];
     }
     const float mean = block_reduce<false>(sum, slots[turn]) / (float)a.dim;
     const int64_t obase = row * a.dim;
@@ -298,8 +342,11 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_bwd_kernel(NormBwdAr
 #pragma unroll
       for (int i = 0; i < V; ++i) u[i] = 0.0f;
       if (dres) load_vec<V>(dres + col, u);
+      float m[V], s[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) u[i] += r * (g[k][i] - hat[k][i] * mean);
+      for (int i = 0; i < V; ++i) m[i] = -mean, s[i] = r;
+      vec_fma(hat[k], m, g[k]);
+      vec_fma(g[k], s, u);
       store_vec<V>(static_cast<T*>(a.dx) + obase + col, u);
       if (a.dresidual_in) store_vec<V>(static_cast<S*>(a.dresidual_in) + obase + col, u);
     }

@@ -5,6 +5,7 @@
 
 #include <cuda_fp8.h>
 
+#include <cstring>
 #include <type_traits>
 
 #include "ssd_common.cuh"
@@ -27,20 +28,126 @@ template <> __device__ __forceinline__ float narrow<float>(float v) { return v; 
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 
+// ---- two fp32 numbers in one 64-bit register: the packed multiply-adds issue once for both -----------
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
+// the two 16-bit elements of a word as fp32
+template <typename T> __device__ __forceinline__ f32x2 widen_pair(uint32_t w);
+template <> __device__ __forceinline__ f32x2 widen_pair<__nv_bfloat16>(uint32_t w) {
+  return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ f32x2 widen_pair<__half>(uint32_t w) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return pack2(f.x, f.y);
+}
+
+// elements 2 i and 2 i + 1 of a vector as fp32
+template <int V>
+__device__ __forceinline__ f32x2 pair_of(const Pack<float, V>& p, int i) { return pack2(p.e[2 * i], p.e[2 * i + 1]); }
+template <int V, typename T>
+__device__ __forceinline__ f32x2 pair_of(const Pack<T, V>& p, int i) {
+  uint32_t w;
+  memcpy(&w, &p.e[2 * i], 4);
+  return widen_pair<T>(w);
+}
+
+template <typename T> struct Pairs;
+template <> struct Pairs<float> {
+  static __device__ __forceinline__ void put(float* e, float a, float b) { e[0] = a, e[1] = b; }
+};
+template <> struct Pairs<__nv_bfloat16> {
+  static __device__ __forceinline__ void put(__nv_bfloat16* e, float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    memcpy(e, &v, 4);
+  }
+};
+template <> struct Pairs<__half> {
+  static __device__ __forceinline__ void put(__half* e, float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    memcpy(e, &v, 4);
+  }
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void widen_all(const Pack<T, V>& p, float (&v)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) unpack2(pair_of(p, i / 2), v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = widen(p.e[i]);
+  }
+}
 template <int V, typename T>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
-  const Pack<T, V> t = *reinterpret_cast<const Pack<T, V>*>(p);
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = widen(t.e[i]);
+  widen_all(*reinterpret_cast<const Pack<T, V>*>(p), v);
 }
 template <int V, typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
   Pack<T, V> t;
+  if constexpr (V % 2 == 0) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) t.e[i] = narrow<T>(v[i]);
+    for (int i = 0; i < V; i += 2) Pairs<T>::put(&t.e[i], v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) t.e[i] = narrow<T>(v[i]);
+  }
   *reinterpret_cast<Pack<T, V>*>(p) = t;
 }
 
+// v = f(v, w) element by element; pairs go through one packed operation
+template <int V>
+__device__ __forceinline__ void vec_add(float (&v)[V], const float (&w)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) unpack2(add2(pack2(v[i], v[i + 1]), pack2(w[i], w[i + 1])), v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] += w[i];
+  }
+}
+template <int V>
+__device__ __forceinline__ void vec_mul(float (&v)[V], const float (&w)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) unpack2(mul2(pack2(v[i], v[i + 1]), pack2(w[i], w[i + 1])), v[i], v[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] *= w[i];
+  }
+}
+// c = a * b + c
+template <int V>
+__device__ __forceinline__ void vec_fma(const float (&a)[V], const float (&b)[V], float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) unpack2(fma2(pack2(a[i], a[i + 1]), pack2(b[i], b[i + 1]), pack2(c[i], c[i + 1])), c[i], c[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] = fmaf(a[i], b[i], c[i]);
+  }
+}
 // V parameters (weights, biases) of any of the three types, always read as V separate elements or, in
 // fp32 and aligned, as 16-byte vectors; read once per thread, so the branch costs nothing.
 template <int V>
@@ -85,6 +192,22 @@ __device__ __forceinline__ float silu_f(float v) { return v * sigmoid_f(v); }
 __device__ __forceinline__ float dsilu_f(float v) {
   const float g = sigmoid_f(v);
   return g * (1.0f + v * (1.0f - g));
+}
+template <int V>
+__device__ __forceinline__ void vec_silu(float (&v)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      float a, b;
+      const f32x2 w = pack2(v[i], v[i + 1]);
+      unpack2(mul2(w, both(-1.4426950408889634f)), a, b);
+      unpack2(add2(both(1.0f), pack2(ex2_approx(a), ex2_approx(b))), a, b);
+      unpack2(mul2(w, pack2(rcp_approx(a), rcp_approx(b))), v[i], v[i + 1]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = silu_f(v[i]);
+  }
 }
 // log(1 + exp(v)), exact to a few units in the last place also where it is small: the layer's steps lie
 // between 1e-4 and 1e-1, where log(exp(v) + 1) would keep three digits.  With e = exp(-|v|) <= 1,

@@ -62,6 +62,27 @@ __device__ __forceinline__ void load_input(const ConvArgs& a, const T* x, int b,
   }
 }
 
+// The value j positions before position `at` of the window, masked where it belongs to another sequence (a
+// select: what is masked may be an infinity or a NaN).
+template <int V, bool SEQ, int N>
+__device__ __forceinline__ void masked(const float (&v)[N][V], const int (&id)[N], int at, int j, float (&past)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) past[i] = !SEQ || id[at - j] == id[at] ? v[at - j][i] : 0.0f;
+}
+// the pre-activation of position `at` of the window
+template <int W, int V, bool SEQ, int N>
+__device__ __forceinline__ void tap(const float (&wr)[W][V], const float (&bs)[V], const float (&v)[N][V], const int (&id)[N], int at, float (&y)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) y[i] = bs[i];
+  vec_fma(wr[0], v[at], y);
+#pragma unroll
+  for (int j = 1; j < W; ++j) {
+    float past[V];
+    masked<V, SEQ>(v, id, at, j, past);
+    vec_fma(wr[j], past, y);
+  }
+}
+
 // Channels are contiguous, so a thread takes V of them; 8 bytes a load leave the registers for eight loads in
 // flight and the next eight behind them.  Every load is unconditional (the position is clamped to the strip):
 // one under a condition would be waited for at once.
@@ -97,30 +118,15 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_fwd_kernel(ConvArgs a
   for (int t = t0; t < t1; t += kGroup) {
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[W - 1 + u][i] = widen(next[u].e[i]);
+      widen_all(next[u], v[W - 1 + u]);
       id[W - 1 + u] = next_id[u];
     }
     if (t + kGroup < t1) fetch(t + kGroup);
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
       float y[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float acc = fmaf(wr[0][i], v[W - 1 + u][i], bs[i]);
-#pragma unroll
-        for (int j = 1; j < W; ++j) {
-          // the value j positions back, masked where it belongs to another sequence (a select: what is
-          // masked may be an infinity or a NaN)
-          const float past = !SEQ || id[W - 1 + u - j] == id[W - 1 + u] ? v[W - 1 + u - j][i] : 0.0f;
-          acc = fmaf(wr[j][i], past, acc);
-        }
-        y[i] = acc;
-      }
-      if (a.silu) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) y[i] = silu_f(y[i]);
-      }
+      tap<W, V, SEQ>(wr, bs, v, id, W - 1 + u, y);
+      if (a.silu) vec_silu(y);
       if (t + u < t1) store_vec<V>(out + (int64_t)(t + u) * a.channels, y);
     }
 #pragma unroll
@@ -207,8 +213,7 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_bwd_kernel(ConvBwdArg
     Pack<T, V> d[kGroup];
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[W - 1 + u][i] = widen(next[u].e[i]);
+      widen_all(next[u], v[W - 1 + u]);
       d[u] = next_d[u];
       id[W - 1 + u] = next_id[u];
     }
@@ -217,28 +222,25 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_bwd_kernel(ConvBwdArg
     for (int u = 0; u < kGroup; ++u) {
       const int at = W - 1 + u, now = t + u;
       float pre[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        pre[i] = fmaf(wr[0][i], v[at][i], bs[i]);
-#pragma unroll
-        for (int j = 1; j < W; ++j) pre[i] = fmaf(wr[j][i], !SEQ || id[at - j] == id[at] ? v[at - j][i] : 0.0f, pre[i]);
-        dp[at][i] = widen(d[u].e[i]);
-      }
+      tap<W, V, SEQ>(wr, bs, v, id, at, pre);
+      widen_all(d[u], dp[at]);
       if (a.silu) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) dp[at][i] *= dsilu_f(pre[i]);
+        for (int i = 0; i < V; ++i) pre[i] = dsilu_f(pre[i]);
+        vec_mul(dp[at], pre);
       }
       if (now >= a.seqlen) {                               // behind the last position there is no dpre
 #pragma unroll
         for (int i = 0; i < V; ++i) dp[at][i] = 0.0f;
       }
       if (now < t1) {
+        vec_add(db, dp[at]);
+        vec_fma(dp[at], v[at], dw[0]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          db[i] += dp[at][i];
-          dw[0][i] = fmaf(dp[at][i], v[at][i], dw[0][i]);
-#pragma unroll
-          for (int j = 1; j < W; ++j) dw[j][i] = fmaf(dp[at][i], !SEQ || id[at - j] == id[at] ? v[at - j][i] : 0.0f, dw[j][i]);
+        for (int j = 1; j < W; ++j) {
+          float past[V];
+          masked<V, SEQ>(v, id, at, j, past);
+          vec_fma(dp[at], past, dw[j]);
         }
       }
       // the position width - 1 back, s, at u in the window: dx[s] = sum_j wr[j] dpre[s + j]
@@ -246,11 +248,13 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_bwd_kernel(ConvBwdArg
       if ((s >= t0 || (first && g.dinit != nullptr)) && s < t1) {
         float r[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          r[i] = 0.0f;
+        for (int i = 0; i < V; ++i) r[i] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < W; ++j)
-            if (!SEQ || s + j >= a.seqlen || id[u] == id[u + j]) r[i] = fmaf(wr[j][i], dp[u + j][i], r[i]);
+        for (int j = 0; j < W; ++j) {
+          float after[V];
+#pragma unroll
+          for (int i = 0; i < V; ++i) after[i] = !SEQ || id[u] == id[u + j] ? dp[u + j][i] : 0.0f;
+          vec_fma(wr[j], after, r);
         }
         const int k = s - (a.seqlen - (W - 1));
         if (g.dfinal != nullptr && k >= 0 && (!SEQ || id[u] == last_id)) {

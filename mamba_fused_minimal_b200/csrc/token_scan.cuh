@@ -32,30 +32,6 @@ struct ScanArgs {
   int seg_len, segments; // positions of a segment (a multiple of the tile's), segments of a sequence
 };
 
-// ---- two fp32 numbers in one 64-bit register: the packed multiply-adds issue once for both -----------
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 both(float v) { return pack2(v, v); }
 // softplus_f and silu_f of a pair: the same operations in the same order
 __device__ __forceinline__ f32x2 softplus2(f32x2 v) {
   float a, b, c, d;
@@ -77,26 +53,6 @@ __device__ __forceinline__ f32x2 silu2(f32x2 v) {
   unpack2(add2(both(1.0f), pack2(ex2_approx(a), ex2_approx(b))), a, b);
   return mul2(v, pack2(rcp_approx(a), rcp_approx(b)));
 }
-// the two 16-bit elements of a word as fp32
-template <typename T> __device__ __forceinline__ f32x2 widen_pair(uint32_t w);
-template <> __device__ __forceinline__ f32x2 widen_pair<__nv_bfloat16>(uint32_t w) {
-  return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <> __device__ __forceinline__ f32x2 widen_pair<__half>(uint32_t w) {
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return pack2(f.x, f.y);
-}
-
-// elements 2 i and 2 i + 1 of a vector as fp32
-template <int V>
-__device__ __forceinline__ f32x2 pair_of(const Pack<float, V>& p, int i) { return pack2(p.e[2 * i], p.e[2 * i + 1]); }
-template <int V, typename T>
-__device__ __forceinline__ f32x2 pair_of(const Pack<T, V>& p, int i) {
-  uint32_t w;
-  memcpy(&w, &p.e[2 * i], 4);
-  return widen_pair<T>(w);
-}
-
 constexpr float kLog2e = 1.4426950408889634f;
 
 // V consecutive elements.  VEC: the vector is aligned and read as a whole, `count` or not -- the caller
@@ -115,22 +71,6 @@ __device__ __forceinline__ Pack<T, V> load_some(const T* p, int count) {
   }
   return t;
 }
-template <typename T> struct Pairs;
-template <> struct Pairs<float> {
-  static __device__ __forceinline__ void put(float* e, float a, float b) { e[0] = a, e[1] = b; }
-};
-template <> struct Pairs<__nv_bfloat16> {
-  static __device__ __forceinline__ void put(__nv_bfloat16* e, float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    memcpy(e, &v, 4);
-  }
-};
-template <> struct Pairs<__half> {
-  static __device__ __forceinline__ void put(__half* e, float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    memcpy(e, &v, 4);
-  }
-};
 template <int V, bool VEC, typename T>
 __device__ __forceinline__ void store_some(T* p, const float (&v)[V], int count) {
   if constexpr (VEC) {

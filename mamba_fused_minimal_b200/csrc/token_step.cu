@@ -56,7 +56,7 @@ __device__ __forceinline__ int first_row(int lane) {
 }
 
 template <typename T, typename S, int VS, int LPR, int U, bool PER_HEAD>
-__global__ void __launch_bounds__(kStepThreads) token_step_kernel(StepArgs args) {
+__global__ void __launch_bounds__(kStepThreads, 5) token_step_kernel(StepArgs args) {
   const ssd_token_scan_step_params_t& p = args.p;
   constexpr int kGroups = kStepThreads / LPR;        // rows side by side
   constexpr int R = U / LPR > 1 ? U / LPR : 1;       // rows a lane finishes
@@ -67,14 +67,12 @@ __global__ void __launch_bounds__(kStepThreads) token_step_kernel(StepArgs args)
   const int heads_per_group = p.nheads / p.ngroups;
 
   // row u of the thread's, clamped to one that exists
-  const int64_t rows = PER_HEAD ? P : (int64_t)p.nheads * P;
-  const int64_t r0 = PER_HEAD ? (int64_t)(blockIdx.x % args.row_blocks) * (kGroups * U) : (int64_t)blockIdx.x * (kGroups * U);
-  const auto head_of = [&](int64_t r) { return PER_HEAD ? (int)(blockIdx.x / args.row_blocks) : P == 1 ? (int)r : (int)(r / P); };
-  const auto p_of = [&](int64_t r) { return PER_HEAD ? (int)r : P == 1 ? 0 : (int)(r % P); };
-  const auto row_of = [&](int u) {
-    const int64_t r = r0 + u * kGroups + grp;
-    return r < rows ? r : rows - 1;
-  };
+  const int rows = PER_HEAD ? P : p.nheads * P;
+  const int r0 = (PER_HEAD ? blockIdx.x % args.row_blocks : blockIdx.x) * (kGroups * U) + grp;
+  const int block_head = PER_HEAD ? blockIdx.x / args.row_blocks : 0;
+  const auto head_of = [&](int r) { return PER_HEAD ? block_head : P == 1 ? r : r / P; };
+  const auto p_of = [&](int r) { return PER_HEAD ? r : P == 1 ? 0 : r % P; };
+  const auto row_of = [&](int u) { return min(r0 + u * kGroups, rows - 1); };
   const bool live = slot >= 0;
   S* const state = static_cast<S*>(p.state) + (int64_t)max(slot, 0) * p.state_stride[0];
   const T* const xb = static_cast<const T*>(p.x) + b * p.x_stride[0];
@@ -83,13 +81,14 @@ __global__ void __launch_bounds__(kStepThreads) token_step_kernel(StepArgs args)
   T x[U], xf[R], zf[R];
   AnyParam dtr[H], br[H], ar[H], Df[R];
   Pack<S, VS> st[U];
+  int64_t at[U];
   float acc[U];
   const int mine0 = lane * VS < n ? lane * VS : 0;   // this lane's first components, clamped
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t r = row_of(u);
-    const int h = head_of(r), pp = p_of(r);
-    st[u] = *reinterpret_cast<const Pack<S, VS>*>(state + h * p.state_stride[1] + pp * p.state_stride[2] + mine0);
+    const int r = row_of(u), h = head_of(r), pp = p_of(r);
+    at[u] = h * p.state_stride[1] + pp * p.state_stride[2];
+    st[u] = *reinterpret_cast<const Pack<S, VS>*>(state + at[u] + mine0);
     x[u] = xb[h * p.x_stride[1] + pp * p.x_stride[2]];
     if (u < H) {
       dtr[u].load(p.dt, p.dt_dtype, b * p.dt_stride[0] + h * p.dt_stride[1]);
@@ -102,8 +101,7 @@ __global__ void __launch_bounds__(kStepThreads) token_step_kernel(StepArgs args)
   const int uf = first_row<LPR, U>(lane);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int64_t r = row_of(uf + i);
-    const int h = head_of(r), pp = p_of(r);
+    const int r = row_of(uf + i), h = head_of(r), pp = p_of(r);
     xf[i] = xb[h * p.x_stride[1] + pp * p.x_stride[2]];
     if (p.z) zf[i] = zb[h * p.z_stride[1] + pp * p.z_stride[2]];
     if (p.D) Df[i].load(p.D, p.D_dtype, h * p.D_stride[0] + pp * p.D_stride[1]);
@@ -137,12 +135,10 @@ __global__ void __launch_bounds__(kStepThreads) token_step_kernel(StepArgs args)
     if (PER_HEAD) load_bc(head_of(0));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t r = row_of(u);
-      const int h = head_of(r), pp = p_of(r);
-      S* const at = state + h * p.state_stride[1] + pp * p.state_stride[2] + nn;
-      float v[VS], Av[VS];
-      if (n0 > 0 && in) st[u] = *reinterpret_cast<const Pack<S, VS>*>(at);
+      float v[VS], Av[VS], w[VS];
+      if (n0 > 0 && in) st[u] = *reinterpret_cast<const Pack<S, VS>*>(state + at[u] + nn);
       if (!PER_HEAD) {
+        const int h = head_of(row_of(u));
         load_bc(h);
         const int64_t a0 = h * p.A_stride[0] + (in ? nn : 0) * p.A_stride[1];
         if (args.vec_A) {
@@ -155,17 +151,23 @@ __global__ void __launch_bounds__(kStepThreads) token_step_kernel(StepArgs args)
       const float d = dt[PER_HEAD ? 0 : u], ux = d * widen(x[u]);
 #pragma unroll
       for (int i = 0; i < VS; ++i) {
-        const float a = PER_HEAD ? decay[0] : ex2_approx(d * (Av[i] * 1.4426950408889634f));
-        v[i] = fmaf(a, widen(st[u].e[i]), ux * Bv[i]);
-        if (in) acc[u] = fmaf(v[i], Cv[i], acc[u]);      // y sees the state before it is rounded to its type
+        Av[i] = PER_HEAD ? decay[0] : ex2_approx(d * (Av[i] * 1.4426950408889634f));
+        v[i] = ux;
+        w[i] = widen(st[u].e[i]);
       }
-      if (in && !idle && r0 + u * kGroups + grp < rows) store_vec<VS>(at, v);
+      vec_mul(v, Bv);
+      vec_fma(Av, w, v);
+      if (in) {
+#pragma unroll
+        for (int i = 0; i < VS; ++i) acc[u] = fmaf(v[i], Cv[i], acc[u]);      // y sees the state before it is rounded to its type
+        if (!idle && r0 + u * kGroups < rows) store_vec<VS>(state + at[u] + nn, v);
+      }
     }
   }
   sum_rows<LPR, U>(acc, lane);
 #pragma unroll
   for (int i = 0; i < R; ++i) {
-    const int64_t r = r0 + (uf + i) * kGroups + grp;
+    const int r = r0 + (uf + i) * kGroups;
     // with more lanes than rows several lanes hold a row's sum: the first of them writes
     if (r >= rows || (LPR > U && (lane & (LPR / U - 1)) != 0)) continue;
     const int h = head_of(r), pp = p_of(r);
@@ -187,7 +189,7 @@ int launch_step(const ssd_token_scan_step_params_t& p, cudaStream_t stream) {
   a.vec_bc = rows_aligned(p.B, p.B_stride, 2, sizeof(T), kBytes) && rows_aligned(p.C, p.C_stride, 2, sizeof(T), kBytes) && p.dstate % VS == 0;
   a.vec_A = p.A_dtype == SSD_F32 && p.A_stride[1] == 1 && rows_aligned(p.A, p.A_stride, 1, 4, VS * 4 < 16 ? VS * 4 : 16) && p.dstate % VS == 0;
   const int64_t blocks = PER_HEAD ? (int64_t)a.row_blocks * p.nheads : ((int64_t)p.nheads * p.headdim + kRows - 1) / kRows;
-  SSD_REQUIRE(blocks <= 0x7fffffff && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "token scan step: too many rows or batch %d too large", p.batch);
+  SSD_REQUIRE((int64_t)p.nheads * p.headdim <= 0x7fffffff - kRows && blocks <= 0x7fffffff && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "token scan step: too many rows or batch %d too large", p.batch);
   token_step_kernel<T, S, VS, LPR, U, PER_HEAD><<<dim3((unsigned)blocks, p.batch), kStepThreads, 0, stream>>>(a);
   SSD_CUDA_OK(cudaGetLastError());
   return SSD_OK;
