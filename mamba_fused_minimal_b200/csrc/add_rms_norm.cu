@@ -287,76 +287,85 @@ struct NormBwdArgs {
 // A block walks rows blockIdx.x, + gridDim.x, ...; each thread keeps its columns' share of the weight
 // gradient in registers and writes it once, as the block's row of `partial`.  The second kernel adds the
 // rows of `partial` in a fixed order, so the result does not depend on which block ran first.
-template <typename T, typename S, int V, int VPT>
-__global__ void __launch_bounds__(kMaxThreads) add_rms_norm_bwd_kernel(NormBwdArgs a) {
+// The next row's loads are issued before this row's sum is joined, so the barrier's wait is theirs too.
+template <typename T, typename S, int V, int VPT, int THREADS>
+__global__ void __launch_bounds__(THREADS) add_rms_norm_bwd_kernel(NormBwdArgs a) {
   __shared__ float slots[2][32];
   float w[VPT][V], dw[VPT][V];
+  int col[VPT];
+  bool in[VPT];
 #pragma unroll
   for (int k = 0; k < VPT; ++k) {
-    const int col = (k * blockDim.x + threadIdx.x) * V;
+    col[k] = (int)(k * blockDim.x + threadIdx.x) * V;
+    in[k] = col[k] < a.dim;
+    col[k] = min(col[k], a.dim - V);       // past the end: the last columns, masked by w = 0 and not stored
+    load_param<V>(a.weight, a.weight_dtype, col[k], w[k]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) w[k][i] = dw[k][i] = 0.0f;
-    if (col < a.dim) load_param<V>(a.weight, a.weight_dtype, col, w[k]);
+    for (int i = 0; i < V; ++i) {
+      dw[k][i] = 0.0f;
+      if (!in[k]) w[k][i] = 0.0f;
+    }
   }
-  int turn = 0;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+  Pack<T, V> gr[VPT];
+  Pack<S, V> tr[VPT], rr[VPT];
+  float r_next;
+  const auto fetch = [&](int64_t row) {
     const int b = (int)(row / a.seqlen), l = (int)(row - (int64_t)b * a.seqlen);
     const T* dout = static_cast<const T*>(a.dout) + b * a.d_sb + l * a.d_sl;
     const S* total = static_cast<const S*>(a.total) + b * a.t_sb + l * a.t_sl;
-    const S* dres = a.dresidual ? static_cast<const S*>(a.dresidual) + b * a.r_sb + l * a.r_sl : nullptr;
-    const float r = a.rstd[row];
-    float g[VPT][V], hat[VPT][V];
-    float sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int col = (k * blockDim.x + threadIdx.x) * V;
-      if (col < a.dim) {
-        load_vec<V>(dout + col, g[k]);
-        load_vec<V>(total + col, hat[k]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) g[k][i] = hat[k][i] = 0.0f;
-      }
+      gr[k] = *reinterpret_cast<const Pack<T, V>*>(dout + col[k]);
+      tr[k] = *reinterpret_cast<const Pack<S, V>*>(total + col[k]);
     }
+    if (a.dresidual) {
+      const S* dres = static_cast<const S*>(a.dresidual) + b * a.r_sb + l * a.r_sl;
+#pragma unroll
+      for (int k = 0; k < VPT; ++k) rr[k] = *reinterpret_cast<const Pack<S, V>*>(dres + col[k]);
+    }
+    r_next = a.rstd[row];
+  };
+  fetch(blockIdx.x);
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const float r = r_next;
+    float g[VPT][V], hat[VPT][V], u[VPT][V], sums[V], s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[i] = 0.0f, s[i] = r;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      float s[V];
+      widen_all(gr[k], g[k]);
+      widen_all(tr[k], hat[k]);
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = r;
+      for (int i = 0; i < V; ++i) u[k][i] = 0.0f;
+      if (a.dresidual) widen_all(rr[k], u[k]);
       vec_mul(hat[k], s);
       vec_fma(g[k], hat[k], dw[k]);
       vec_mul(g[k], w[k]);
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = 0.0f;
-      vec_fma(g[k], hat[k], s);
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += s[i];
+      vec_fma(g[k], hat[k], sums);
     }
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) sum += sums[i];
+    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
     const float mean = block_reduce<false>(sum, slots[turn]) / (float)a.dim;
+    float m[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) m[i] = -mean;
     const int64_t obase = row * a.dim;
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
-      const int col = (k * blockDim.x + threadIdx.x) * V;
-      if (col >= a.dim) continue;
-      float u[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) u[i] = 0.0f;
-      if (dres) load_vec<V>(dres + col, u);
-      float m[V], s[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) m[i] = -mean, s[i] = r;
+      if (!in[k]) continue;
       vec_fma(hat[k], m, g[k]);
-      vec_fma(g[k], s, u);
-      store_vec<V>(static_cast<T*>(a.dx) + obase + col, u);
-      if (a.dresidual_in) store_vec<V>(static_cast<S*>(a.dresidual_in) + obase + col, u);
+      vec_fma(g[k], s, u[k]);
+      store_vec<V>(static_cast<T*>(a.dx) + obase + col[k], u[k]);
+      if (a.dresidual_in) store_vec<V>(static_cast<S*>(a.dresidual_in) + obase + col[k], u[k]);
     }
   }
   float* part = a.partial + (int64_t)blockIdx.x * a.dim;
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) {
-    const int col = (k * blockDim.x + threadIdx.x) * V;
-    if (col < a.dim) store_vec<V>(part + col, dw[k]);
-  }
+  for (int k = 0; k < VPT; ++k)
+    if (in[k]) store_vec<V>(part + col[k], dw[k]);
 }
 
 // The same for rows longer than a block's registers hold: every row is read twice and the weight
@@ -425,10 +434,16 @@ int launch_norm_bwd_v(const NormBwdArgs& a, cudaStream_t stream) {
   row_shape((a.dim + V - 1) / V, 0, V == 8 ? 2 : 4, &threads, &vpt);
   const int parts = bwd_parts(a.rows);
   switch (vpt) {
-    case 1: add_rms_norm_bwd_kernel<T, S, V, 1><<<parts, threads, 0, stream>>>(a); break;
-    case 2: add_rms_norm_bwd_kernel<T, S, V, 2><<<parts, threads, 0, stream>>>(a); break;
+    case 1:
+      // up to 512 threads have the registers for the next row's values
+      if (threads <= 512)
+        add_rms_norm_bwd_kernel<T, S, V, 1, 512><<<parts, threads, 0, stream>>>(a);
+      else
+        add_rms_norm_bwd_kernel<T, S, V, 1, kMaxThreads><<<parts, threads, 0, stream>>>(a);
+      break;
+    case 2: add_rms_norm_bwd_kernel<T, S, V, 2, kMaxThreads><<<parts, threads, 0, stream>>>(a); break;
     case 4:
-      if constexpr (V < 8) add_rms_norm_bwd_kernel<T, S, V, 4><<<parts, threads, 0, stream>>>(a);
+      if constexpr (V < 8) add_rms_norm_bwd_kernel<T, S, V, 4, kMaxThreads><<<parts, threads, 0, stream>>>(a);
       break;
     default:
       add_rms_norm_bwd_long_kernel<T, S><<<(unsigned)a.rows, 1024, 0, stream>>>(a);

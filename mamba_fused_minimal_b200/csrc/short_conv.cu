@@ -326,16 +326,17 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvStepA
   const int row = blockIdx.y;
   const int slot = step_slot(a.indices, row, a.slots);
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
+  // every load is issued before anything is used, clamped instead of under a condition
   const bool inside = c < a.channels;
-  T* out = static_cast<T*>(a.out) + (int64_t)row * a.channels + c;
-  T* st = static_cast<T*>(a.state) + (int64_t)max(slot, 0) * a.st_ss + c;
-  float y[V], in[V], past[W - 1][V], wr[W][V], bs[V];
-  if (inside && slot >= 0) {
-    load_vec<V>(static_cast<const T*>(a.x) + row * a.x_sb + c, in);
+  const int cc = inside ? c : 0;
+  T* out = static_cast<T*>(a.out) + (int64_t)row * a.channels + cc;
+  T* st = static_cast<T*>(a.state) + (int64_t)max(slot, 0) * a.st_ss + cc;
+  const Pack<T, V> xr = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.x) + row * a.x_sb + cc);
+  Pack<T, V> old[W - 1];
 #pragma unroll
-    for (int j = 0; j < W - 1; ++j) load_vec<V>(st + (int64_t)j * a.st_sp, past[j]);    // oldest first
-    load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, c, wr, bs);
-  }
+  for (int j = 0; j < W - 1; ++j) old[j] = *reinterpret_cast<const Pack<T, V>*>(st + (int64_t)j * a.st_sp);    // oldest first
+  float y[V], in[V], past[W - 1][V], wr[W][V], bs[V];
+  load_filter<W, V>(a.weight, a.weight_dtype, a.bias, a.bias_dtype, cc, wr, bs);
   const bool taken = step_taken(a.indices, row, slot);
   if (!inside) return;
   if (slot < 0 || taken) {
@@ -344,6 +345,9 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvStepA
     store_vec<V>(out, y);
     return;
   }
+  widen_all(xr, in);
+#pragma unroll
+  for (int j = 0; j < W - 1; ++j) widen_all(old[j], past[j]);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     float acc = fmaf(wr[0][i], in[i], bs[i]);
@@ -353,8 +357,8 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvStepA
   }
   store_vec<V>(out, y);
 #pragma unroll
-  for (int j = 0; j < W - 2; ++j) store_vec<V>(st + (int64_t)j * a.st_sp, past[j + 1]);
-  store_vec<V>(st + (int64_t)(W - 2) * a.st_sp, in);
+  for (int j = 0; j < W - 2; ++j) *reinterpret_cast<Pack<T, V>*>(st + (int64_t)j * a.st_sp) = old[j + 1];
+  *reinterpret_cast<Pack<T, V>*>(st + (int64_t)(W - 2) * a.st_sp) = xr;
 }
 
 ConvArgs conv_args(const ssd_short_conv_params_t& p) {
@@ -478,9 +482,10 @@ int launch_short_conv_step(const ssd_short_conv_step_params_t& p, cudaStream_t s
   SSD_REQUIRE(p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv step: batch %d too large", p.batch);
   return with_type(p.x_dtype, [&](auto t) {
     using T = decltype(t);
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = p.channels % V == 0 && rows_aligned(p.x, &p.x_stride, 1, sizeof(T), 16) &&
-                     rows_aligned(p.conv_state, p.state_stride, 2, sizeof(T), 16) && aligned_to(p.out, 16);
+    constexpr int V = 4;
+    constexpr size_t kBytes = V * sizeof(T);
+    const bool vec = p.channels % V == 0 && rows_aligned(p.x, &p.x_stride, 1, sizeof(T), kBytes) &&
+                     rows_aligned(p.conv_state, p.state_stride, 2, sizeof(T), kBytes) && aligned_to(p.out, kBytes);
     return with_width(p.width, [&](auto w) {
       constexpr int W = decltype(w)::value;
       const auto go = [&](auto v) -> int {
