@@ -432,7 +432,8 @@ typedef struct {
   const void* weight;        /* (dim,) of weight_dtype, contiguous */
   void* out;                 /* (b, l, dim) of out_dtype */
   void* residual_out;        /* (b, l, dim) of residual_dtype, or NULL */
-  float* rstd;               /* (b, l): (mean of the squares of t as kept, or of x + eps)^(-1/2), for the gradients */
+  float* rstd;               /* (b, l): (mean of the squares of t as kept, or of x, + eps)^(-1/2), for the gradients;
+                                not written with an 8-bit out */
   float* scales;             /* (b, l); required for an 8-bit out */
   int32_t x_dtype, residual_dtype, weight_dtype, out_dtype;
   int32_t batch, seqlen, dim;

@@ -32,18 +32,29 @@ template <typename O> struct OutKind { static constexpr float kMost = 0.0f; };
 template <> struct OutKind<I8> { static constexpr float kMost = 127.0f; };
 template <> struct OutKind<E4M3> { static constexpr float kMost = 448.0f; };
 
+// y / scale, rounded as a division rounds: the product with the reciprocal, and what it left over
+template <int V>
+__device__ __forceinline__ void quotients(const float (&y)[V], float scale, float inv, float (&q)[V]) {
+  float left[V], iv[V], sc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) q[i] = iv[i] = inv, sc[i] = -scale, left[i] = y[i];
+  vec_mul(q, y);
+  vec_fma(q, sc, left);
+  vec_fma(left, iv, q);
+}
+
 template <typename O, int V>
-__device__ __forceinline__ void store_out(void* base, int64_t idx, const float (&y)[V], float inv) {
+__device__ __forceinline__ void store_out(void* base, int64_t idx, const float (&y)[V], float scale, float inv) {
   if constexpr (std::is_same<O, I8>::value) {
     Pack<int8_t, V> t;
+    float q[V];
+    quotients(y, scale, inv, q);
 #pragma unroll
-    for (int i = 0; i < V; ++i) t.e[i] = (int8_t)max(-127, min(127, __float2int_rn(y[i] * inv)));
+    for (int i = 0; i < V; ++i) t.e[i] = (int8_t)max(-127, min(127, __float2int_rn(q[i])));
     *reinterpret_cast<Pack<int8_t, V>*>(static_cast<int8_t*>(base) + idx) = t;
   } else if constexpr (std::is_same<O, E4M3>::value) {
     float q[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) q[i] = inv;
-    vec_mul(q, y);
+    quotients(y, scale, inv, q);
     if constexpr (V % 2 == 0) {
       Pack<uint16_t, V / 2> t;
 #pragma unroll
@@ -99,7 +110,8 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
   float sums[V], kepts[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) sums[i] = kepts[i] = 0.0f;
-  constexpr bool kRounds = sizeof(R) < 4;
+  // an 8-bit output has no gradients
+  constexpr bool kRounds = sizeof(R) < 4 && !kScaled;
   const auto square = [&](const float (&v)[V]) {
     vec_fma(v, v, sums);
     if constexpr (kRounds) {
@@ -148,7 +160,7 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
     kept = sum = block_reduce<false>(sum, slots[0]);
   }
   const float r = rsqrtf(sum / (float)a.dim + a.eps);
-  if (threadIdx.x == 0) a.rstd[row] = rsqrtf(kept / (float)a.dim + a.eps);
+  if (!kScaled && threadIdx.x == 0) a.rstd[row] = rsqrtf(kept / (float)a.dim + a.eps);
 
   // y of one vector; `keep` writes the sum beside it
   const auto finish = [&](int col, float (&v)[V], bool keep) {
@@ -168,14 +180,14 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
         const int col = (k * blockDim.x + threadIdx.x) * V;
         if (col < a.dim) {
           finish(col, t[k], true);
-          store_out<O, V>(a.out, obase + col, t[k], 0.0f);
+          store_out<O, V>(a.out, obase + col, t[k], 0.0f, 0.0f);
         }
       }
     } else {
       for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
         fetch(col, t[0]);
         finish(col, t[0], true);
-        store_out<O, V>(a.out, obase + col, t[0], 0.0f);
+        store_out<O, V>(a.out, obase + col, t[0], 0.0f, 0.0f);
       }
     }
   } else {
@@ -203,18 +215,18 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
     const float scale = most <= 3.4028235e38f ? most / OutKind<O>::kMost : __int_as_float(0x7fc00000);
     if (threadIdx.x == 0) a.scales[row] = scale;
     // zero for a row of zeros; finite for the smallest rows
-    const float inv = most > 0.0f ? fminf(OutKind<O>::kMost / most, 3.4028235e38f) : 0.0f;
+    const float inv = most > 0.0f ? fminf(OutKind<O>::kMost / most, 1e38f) : 0.0f;
     if (kHold) {
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int col = (k * blockDim.x + threadIdx.x) * V;
-        if (col < a.dim) store_out<O, V>(a.out, obase + col, t[k], inv);
+        if (col < a.dim) store_out<O, V>(a.out, obase + col, t[k], scale, inv);
       }
     } else {
       for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
         fetch(col, t[0]);
         finish(col, t[0], false);
-        store_out<O, V>(a.out, obase + col, t[0], inv);
+        store_out<O, V>(a.out, obase + col, t[0], scale, inv);
       }
     }
   }

@@ -414,13 +414,14 @@ int ssd_add_rms_norm_fwd(const ssd_add_rms_norm_params_t* prm, ssd_stream_t stre
   NvtxRange nvtx_range("ssd_add_rms_norm_fwd");
   SSD_REQUIRE(prm != nullptr, SSD_ERR_BAD_ARGUMENT, "params is NULL");
   const ssd_add_rms_norm_params_t& p = *prm;
-  SSD_REQUIRE(p.x && p.weight && p.out && p.rstd, SSD_ERR_BAD_ARGUMENT, "x, weight, out and rstd must not be NULL");
+  SSD_REQUIRE(p.x && p.weight && p.out, SSD_ERR_BAD_ARGUMENT, "x, weight and out must not be NULL");
   SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
   SSD_REQUIRE((p.residual == nullptr && p.residual_out == nullptr) || p.residual_dtype == p.x_dtype || p.residual_dtype == SSD_F32,
               SSD_ERR_UNSUPPORTED, "the residual must have x's dtype or be fp32");
   SSD_REQUIRE(p.out_dtype == p.x_dtype || p.out_dtype == SSD_I8 || p.out_dtype == SSD_E4M3, SSD_ERR_UNSUPPORTED,
               "out must have x's dtype, int8 or e4m3");
-  SSD_REQUIRE(p.out_dtype == p.x_dtype || p.scales != nullptr, SSD_ERR_BAD_ARGUMENT, "an 8-bit out needs scales");
+  SSD_REQUIRE(p.out_dtype == p.x_dtype ? p.rstd != nullptr : p.scales != nullptr, SSD_ERR_BAD_ARGUMENT,
+              "rstd must not be NULL, nor scales with an 8-bit out");
   SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.dim > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
   SSD_REQUIRE((int64_t)p.batch * p.seqlen <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   return launch_add_rms_norm(p, reinterpret_cast<cudaStream_t>(stream));

@@ -53,36 +53,36 @@ struct BwdShape {
   static constexpr size_t kSmem = 2 * kRaw + sizeof(float) * ((3 * kChannels + 2 * NP) * kPitch + 2 * kChannels * kSlabs * kPitch + kBwdWarps * kT * kRow);
 };
 
-// One warp copies `rows` rows of `bytes` bytes, `pitch` bytes apart, to rows of `to_pitch` bytes in shared
-// memory: asynchronously where rows and sizes are multiples of 4, 8 or 16 bytes (`unit`), else by elements
-// of `elem` bytes.  Row r stands for row min(r, last).
-__device__ __forceinline__ void copy_rows(char* to, int to_pitch, const char* from, int64_t pitch, int rows, int last, int bytes, int unit, int elem,
-                                          int lane) {
-  if (unit >= 4) {
-    const int per = bytes / unit;
-    for (int i = lane; i < rows * per; i += 32) {
-      const int r = i / per, k = (i - r * per) * unit;
-      const char* src = from + min(r, last) * pitch + k;
-      const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to + r * to_pitch + k));
-      if (unit == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-      else if (unit == 8)
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
-      else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-    }
-  } else {
-    const int per = bytes / elem;
-    for (int i = lane; i < rows * per; i += 32) {
-      const int r = i / per, k = (i - r * per) * elem;
-      const char* src = from + min(r, last) * pitch + k;
-      char* dst = to + r * to_pitch + k;
-      if (elem == 4)
-        *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
-      else
-        *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
-    }
+// One warp copies `rows` rows of `bytes` bytes, `pitch` bytes apart, to rows of TO bytes in shared memory:
+// asynchronously where rows and sizes are multiples of 4, 8 or 16 bytes (`unit`), else by elements of `elem`
+// bytes.  Row r stands for row min(r, last).
+template <int TO>
+__device__ __forceinline__ void copy_rows(char* to, const char* from, int64_t pitch, int rows, int last, int bytes, int unit, int elem, int lane) {
+  const int step = unit >= 4 ? unit : elem, shift = __ffs(step) - 1;
+  // lanes go over whole rows of TO bytes, a power of two, so that no division is needed
+  for (int i = lane << shift; i < rows * TO; i += 32 << shift) {
+    const int r = i / TO, k = i % TO;
+    if (k >= bytes) continue;
+    const char* src = from + min(r, last) * pitch + k;
+    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(to + i));
+    if (unit == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else if (unit == 8)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+    else if (unit == 4)
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+    else if (elem == 4)
+      *reinterpret_cast<uint32_t*>(to + i) = *reinterpret_cast<const uint32_t*>(src);
+    else
+      *reinterpret_cast<uint16_t*>(to + i) = *reinterpret_cast<const uint16_t*>(src);
   }
+}
+
+// sum += v with the rounding error carried along: the parameters' gradients are sums over every position
+__device__ __forceinline__ void add_to(float& sum, float& lost, float v) {
+  const float y = v - lost, t = sum + y;
+  lost = (t - sum) - y;
+  sum = t;
 }
 
 template <typename T, int NP>
@@ -116,25 +116,35 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
     constexpr int kOne = Sh::kItems * ES, kBC = kT * NP * ES;
     const int tail = a.seqlen - 1 - t0;
     const int64_t row = (int64_t)b * a.seqlen + t0;
-    const auto rows = [&](int at, const void* base, int64_t off, int64_t sl, int es, int unit) {
-      copy_rows(raw + at, CH * es, static_cast<const char*>(base) + (off + (int64_t)t0 * sl + c0) * es, sl * es, kT, tail, nch * es, unit, es, lane);
+    const auto rows = [&](int at, const void* base, int64_t off, int64_t sl) {
+      copy_rows<CH * ES>(raw + at, static_cast<const char*>(base) + (off + (int64_t)t0 * sl + c0) * ES, sl * ES, kT, tail, nch * ES, q.unit, ES, lane);
     };
-    if (warp == 0) rows(0, a.x, b * a.x_sb, a.x_sl, ES, q.unit);
-    if (warp == 1) rows(kOne, q.dout, b * q.d_sb, q.d_sl, ES, q.unit);
-    if (warp == 2 && a.z) rows(2 * kOne, a.z, b * a.z_sb, a.z_sl, ES, q.unit);
-    if (warp == 3 && a.z) rows(3 * kOne, a.out_x, (row - t0) * a.channels, a.channels, ES, q.unit);
-    if (warp == 4) rows(4 * kOne + 2 * kBC, a.dt, b * a.dt_sb, a.dt_sl, a.dt_f32 ? 4 : ES, a.dt_f32 ? q.unit32 : q.unit);
-    const int nb = a.dstate * ES;
-    if (warp == 5)
-      copy_rows(raw + 4 * kOne, NP * ES, static_cast<const char*>(a.B) + (b * a.B_sb + (int64_t)t0 * a.B_sl + grp * a.B_sg) * ES, a.B_sl * ES, kT,
-                tail, nb, q.unit_bc, ES, lane);
-    if (warp == 6)
-      copy_rows(raw + 4 * kOne + kBC, NP * ES, static_cast<const char*>(a.C) + (b * a.C_sb + (int64_t)t0 * a.C_sl + grp * a.C_sg) * ES, a.C_sl * ES,
-                kT, tail, nb, q.unit_bc, ES, lane);
-    if (warp == 7)
-      copy_rows(raw + Sh::kRaw16 * ES + Sh::kItems * 4, NP * 4,
-                reinterpret_cast<const char*>(a.ckpt + (((int64_t)b * tiles + t0 / kT) * a.channels + c0) * a.dstate), (int64_t)a.dstate * 4, nch, nch,
-                a.dstate * 4, q.unit_ck, 4, lane);
+    const auto states = [&](int at, const void* base, int64_t off, int64_t sl) {
+      copy_rows<NP * ES>(raw + at, static_cast<const char*>(base) + (off + (int64_t)t0 * sl) * ES, sl * ES, kT, tail, a.dstate * ES, q.unit_bc, ES, lane);
+    };
+    switch (warp) {
+      case 0: rows(0, a.x, b * a.x_sb, a.x_sl); break;
+      case 1: rows(kOne, q.dout, b * q.d_sb, q.d_sl); break;
+      case 2:
+        if (a.z) rows(2 * kOne, a.z, b * a.z_sb, a.z_sl);
+        break;
+      case 3:
+        if (a.z) rows(3 * kOne, a.out_x, (row - t0) * a.channels, a.channels);
+        break;
+      case 4:
+        if (a.dt_f32)
+          copy_rows<CH * 4>(raw + 4 * kOne + 2 * kBC, static_cast<const char*>(a.dt) + (b * a.dt_sb + (int64_t)t0 * a.dt_sl + c0) * 4, a.dt_sl * 4, kT, tail,
+                            nch * 4, q.unit32, 4, lane);
+        else
+          rows(4 * kOne + 2 * kBC, a.dt, b * a.dt_sb, a.dt_sl);
+        break;
+      case 5: states(4 * kOne, a.B, b * a.B_sb + grp * a.B_sg, a.B_sl); break;
+      case 6: states(4 * kOne + kBC, a.C, b * a.C_sb + grp * a.C_sg, a.C_sl); break;
+      default:
+        copy_rows<NP * 4>(raw + Sh::kRaw16 * ES + Sh::kItems * 4,
+                          reinterpret_cast<const char*>(a.ckpt + (((int64_t)b * tiles + t0 / kT) * a.channels + c0) * a.dstate), (int64_t)a.dstate * 4, nch,
+                          nch, a.dstate * 4, q.unit_ck, 4, lane);
+    }
   };
 
   // what this thread prepares and stores: positions lt, lt + kStep, ... of the tile, channel lc
@@ -144,7 +154,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   const int c = c0 + (inc ? lc : 0);
   const float Dv = a.D ? load_f(a.D, a.D_dtype, c) : 0.0f;
   const float bias = a.bias ? load_f(a.bias, a.bias_dtype, c) : 0.0f;
-  float sum_D = 0.0f, sum_bias = 0.0f;
+  float sum_D = 0.0f, sum_bias = 0.0f, lost_D = 0.0f, lost_bias = 0.0f;
   const int64_t own = (int64_t)b * a.seqlen * a.channels;       // of the contiguous tensors
 
   // what this thread computes
@@ -154,7 +164,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   const int64_t ck_step = (int64_t)a.channels * a.dstate;
   const float A = has ? load_f(a.A, a.A_dtype, at_n) : 0.0f;
   float carry = has && q.dfinal ? q.dfinal[b * ck_step + at_n] : 0.0f;      // a_{t+1} g_{t+1}
-  float sum_A = 0.0f;
+  float sum_A = 0.0f, lost_A = 0.0f;
 
   // B and C: component bn of positions bt, bt + kBcStep, ...; the first half of the items is B (with eight
   // components the first half of the threads takes B and the other C)
@@ -211,7 +221,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
         s_u[at] = d[e] * x[e];
         s_g[at] = dy[e];
       }
-      sum_D += dy[e] * x[e];
+      add_to(sum_D, lost_D, dy[e] * x[e]);
     }
 #pragma unroll
     for (int k = 0; k < NBC; ++k) {
@@ -226,55 +236,71 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
 
     const auto walk = [&](auto reset) {
       constexpr bool RESET = decltype(reset)::value;
-      // forwards through the tile: the decays, and what of the state before reaches each position
-      float dec[kT], kept[kT];
+      // forwards through the tile: the decays, and what of the state before reaches each position; pairs are
+      // two neighbouring positions
+      f32x2 dec[kT / 2], kept[kT / 2];
 #pragma unroll
       for (int t = 0; t < kT; t += 4) {
-        const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
-        const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kPitch + t]);
-        const float4 B4 = *reinterpret_cast<const float4*>(&s_B[n * kPitch + t]);
-        const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w}, BB[4] = {B4.x, B4.y, B4.z, B4.w};
+        const ulonglong2 d4 = *reinterpret_cast<const ulonglong2*>(&s_d[ch * kPitch + t]);
+        const ulonglong2 u4 = *reinterpret_cast<const ulonglong2*>(&s_u[ch * kPitch + t]);
+        const ulonglong2 B4 = *reinterpret_cast<const ulonglong2*>(&s_B[n * kPitch + t]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          dec[t + i] = ex2_approx(dd[i] * (A * kLog2e));
-          kept[t + i] = dec[t + i] * h;
-          if (RESET && (resets >> (t + i) & 1u)) dec[t + i] = kept[t + i] = 0.0f;
-          h = fmaf(uu[i], BB[i], kept[t + i]);
+        for (int i = 0; i < 2; ++i) {
+          float e[2], k[2], v[2];
+          unpack2(mul2(i ? d4.y : d4.x, both(A * kLog2e)), e[0], e[1]);
+          unpack2(mul2(i ? u4.y : u4.x, i ? B4.y : B4.x), v[0], v[1]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            e[j] = ex2_approx(e[j]);
+            k[j] = e[j] * h;
+            if (RESET && (resets >> (t + 2 * i + j) & 1u)) e[j] = k[j] = 0.0f;
+            h = k[j] + v[j];
+          }
+          dec[t / 2 + i] = pack2(e[0], e[1]);
+          kept[t / 2 + i] = pack2(k[0], k[1]);
         }
       }
       // and backwards
+      f32x2 sum_A2 = 0;
 #pragma unroll
       for (int t = kT - 4; t >= 0; t -= 4) {
-        const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
-        const float4 u4 = *reinterpret_cast<const float4*>(&s_u[ch * kPitch + t]);
-        const float4 g4 = *reinterpret_cast<const float4*>(&s_g[ch * kPitch + t]);
-        const float4 B4 = *reinterpret_cast<const float4*>(&s_B[n * kPitch + t]);
-        const float4 C4 = *reinterpret_cast<const float4*>(&s_C[n * kPitch + t]);
-        const float dd[4] = {d4.x, d4.y, d4.z, d4.w}, uu[4] = {u4.x, u4.y, u4.z, u4.w}, yy[4] = {g4.x, g4.y, g4.z, g4.w};
-        const float BB[4] = {B4.x, B4.y, B4.z, B4.w}, CC[4] = {C4.x, C4.y, C4.z, C4.w};
+        const ulonglong2 d4 = *reinterpret_cast<const ulonglong2*>(&s_d[ch * kPitch + t]);
+        const ulonglong2 u4 = *reinterpret_cast<const ulonglong2*>(&s_u[ch * kPitch + t]);
+        const ulonglong2 g4 = *reinterpret_cast<const ulonglong2*>(&s_g[ch * kPitch + t]);
+        const ulonglong2 B4 = *reinterpret_cast<const ulonglong2*>(&s_B[n * kPitch + t]);
+        const ulonglong2 C4 = *reinterpret_cast<const ulonglong2*>(&s_C[n * kPitch + t]);
         float p1[4], p2[4];
 #pragma unroll
-        for (int i = 3; i >= 0; --i) {
-          const float g = fmaf(CC[i], yy[i], carry);
-          const float vC = yy[i] * fmaf(uu[i], BB[i], kept[t + i]);
-          const float vB = g * uu[i];
-          const float m = g * kept[t + i];
-          p1[i] = g * BB[i];
-          p2[i] = m * A;
-          sum_A = fmaf(m, dd[i], sum_A);
-          carry = g * dec[t + i];
-          float* row = s_bc + (warp * kT + t + i) * ROW;
-          if constexpr (NP >= 32) {
-            row[lane] = vB;
-            row[32 + lane] = vC;
-          } else {
-            // lanes 0..15 keep dB, lanes 16..31 dC, of the channels 16 lanes apart
-            float v = (lane < 16 ? vB : vC) + __shfl_xor_sync(0xffffffffu, lane < 16 ? vC : vB, 16);
-            if constexpr (NP == 8) {
-              v += __shfl_xor_sync(0xffffffffu, v, 8);
-              if ((lane & 8) == 0) row[(lane >> 4) * 8 + (lane & 7)] = v;
+        for (int i = 1; i >= 0; --i) {
+          const f32x2 dd = i ? d4.y : d4.x, uu = i ? u4.y : u4.x, yy = i ? g4.y : g4.x, BB = i ? B4.y : B4.x, CC = i ? C4.y : C4.x;
+          float from[2], e[2], g[2], vB[2], vC[2];
+          unpack2(mul2(CC, yy), from[0], from[1]);
+          unpack2(dec[t / 2 + i], e[0], e[1]);
+          g[1] = from[1] + carry;
+          g[0] = fmaf(g[1], e[1], from[0]);
+          carry = g[0] * e[0];
+          const f32x2 gg = pack2(g[0], g[1]);
+          const f32x2 m = mul2(gg, kept[t / 2 + i]);
+          unpack2(mul2(yy, fma2(uu, BB, kept[t / 2 + i])), vC[0], vC[1]);
+          unpack2(mul2(gg, uu), vB[0], vB[1]);
+          unpack2(mul2(gg, BB), p1[2 * i], p1[2 * i + 1]);
+          unpack2(mul2(m, both(A)), p2[2 * i], p2[2 * i + 1]);
+          sum_A2 = fma2(m, dd, sum_A2);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float* row = s_bc + (warp * kT + t + 2 * i + j) * ROW;
+            if constexpr (NP >= 32) {
+              row[lane] = vB[j];
+              row[32 + lane] = vC[j];
             } else {
-              row[lane] = v;
+              // lanes 0..15 keep dB, lanes 16..31 dC, of the channels 16 lanes apart
+              float v = (lane < 16 ? vB[j] : vC[j]) + __shfl_xor_sync(0xffffffffu, lane < 16 ? vC[j] : vB[j], 16);
+              if constexpr (NP == 8) {
+                v += __shfl_xor_sync(0xffffffffu, v, 8);
+                if ((lane & 8) == 0) row[(lane >> 4) * 8 + (lane & 7)] = v;
+              } else {
+                row[lane] = v;
+              }
             }
           }
         }
@@ -291,6 +317,9 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
         for (int off = 8; off < (NP < 32 ? NP : 32); off <<= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
         if ((n & 31) < 8) s_p[(((lane & 1) * CH + ch) * SL + n / 32) * kPitch + t + ((lane >> 1) & 3)] = r;
       }
+      float lo, hi;
+      unpack2(sum_A2, lo, hi);
+      add_to(sum_A, lost_A, lo + hi);
     };
     if (resets == 0u)
       walk(std::false_type());
@@ -310,7 +339,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
         gA += s_p[((CH + lc) * SL + s) * kPitch + lt + e * kStep];
       }
       const float dd = fmaf(x[e], gB, gA) * slope[e];
-      sum_bias += dd;
+      add_to(sum_bias, lost_bias, dd);
       const int64_t at = own + (int64_t)t * a.channels + c;
       static_cast<T*>(q.dx)[at] = narrow<T>(fmaf(d[e], gB, Dv * dy[e]));
       if (a.dt_f32)

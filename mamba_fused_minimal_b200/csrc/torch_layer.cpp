@@ -56,7 +56,7 @@ void param(const OptTensor& t, const Tensor& like, const char* name, Tensor& hol
 }
 
 // ---- residual addition + root-mean-square norm --------------------------------------------------------
-std::tuple<Tensor, OptTensor, Tensor, OptTensor> add_rms_norm_fwd(const Tensor& x, const Tensor& weight, const OptTensor& residual,
+std::tuple<Tensor, OptTensor, OptTensor, OptTensor> add_rms_norm_fwd(const Tensor& x, const Tensor& weight, const OptTensor& residual,
                                                                   double eps, std::optional<at::ScalarType> out_dtype,
                                                                   std::optional<at::ScalarType> residual_dtype) {
   check_input(x);
@@ -81,7 +81,7 @@ std::tuple<Tensor, OptTensor, Tensor, OptTensor> add_rms_norm_fwd(const Tensor& 
     p.residual = residual->data_ptr();
     row_strides(p.residual_stride, *residual);
   }
-  OptTensor total, scales;
+  OptTensor total, rstd, scales;
   p.residual_dtype = p.x_dtype;
   if (rdt.has_value()) {
     p.residual_dtype = dtype_code(*rdt);
@@ -93,13 +93,14 @@ std::tuple<Tensor, OptTensor, Tensor, OptTensor> add_rms_norm_fwd(const Tensor& 
   Tensor out = alloc_out(x.sizes(), x.options().dtype(odt));
   const auto f32 = x.options().dtype(at::kFloat);
   const auto rows = x.sizes().slice(0, x.dim() - 1);
-  Tensor rstd = alloc_out(rows, f32);
   if (p.out_dtype == SSD_I8 || p.out_dtype == SSD_E4M3) {
     scales = alloc_out(rows, f32);
     p.scales = scales->data_ptr<float>();
+  } else {
+    rstd = alloc_out(rows, f32);
+    p.rstd = rstd->data_ptr<float>();
   }
   p.out = out.data_ptr();
-  p.rstd = rstd.data_ptr<float>();
   p.eps = static_cast<float>(eps);
   check_rc(ssd_add_rms_norm_fwd(&p, current_stream(x)), "ssd_add_rms_norm_fwd");
   return {out, total, rstd, scales};

@@ -19,7 +19,8 @@ def _add_rms_norm_fwd(x, weight, residual=None, eps=1e-5, out_dtype=None, residu
 
     Returns (out, residual_out, rstd, scales).  residual_out is t in the residual's dtype (x's dtype or
     fp32), or in `residual_dtype` where there is no residual yet; None if neither is given.  rstd
-    (rows..., fp32), of residual_out as it was kept, is for the gradients.  scales is None unless out is in 8 bits."""
+    (rows..., fp32), of residual_out as it was kept, is for the gradients; scales (rows..., fp32) takes its
+    place where out is in 8 bits (the other of the two is None)."""
     assert x.dim() in (2, 3)
     assert weight.shape == x.shape[-1:]
     if residual is not None:
