@@ -3,19 +3,26 @@ same seven functions -- all five unfused kernels, and the two pipelines whose mi
 is a fused entry point -- and a comparison of their six outputs with
 isclose(rtol=1e-2, atol=1e-3).
 
+Then the same scan as a layer uses it: residual addition and norm, short convolution, chunk pipeline for a
+prompt, and the prompt's continuation token by token from the states that it left, against the longer
+prompt.
+
     python -m mamba_fused_minimal_b200.main
 """
 import torch
 from einops import rearrange
 
+from .kernels.add_rms_norm import _add_rms_norm_fwd
 from .kernels.fused_concurrent import _fused_chunk_state_state_passing_fwd_concurrent
 from .kernels.fused_globalbar import _fused_chunk_state_state_passing_fwd_globalbar
 from .kernels.rand_data import generate_dummy_data
+from .kernels.short_conv import _short_conv_fwd, _short_conv_step
 from .kernels.ssd_bmm import _bmm_chunk_fwd
 from .kernels.ssd_chunk_scan import _bmm_chunk_scan_fwd, _chunk_scan_fwd
 from .kernels.ssd_chunk_state import _chunk_cumsum_fwd, _chunk_state_fwd
 from .kernels.ssd_state_passing import _state_passing_fwd
 from .kernels.state_path import _state_path_fwd
+from .kernels.token_scan import _token_scan_step
 
 TENSOR_NAMES = ["out", "out_x", "dt", "dA_cumsum", "states", "final_states"]
 
@@ -101,6 +108,61 @@ def _mamba_chunk_scan_combined_fwd_concurrent(x, dt, A, B, C, chunk_size, D=None
                            dt_limit)
 
 
+def _layer_prompt_fwd(u, residual, dt, norm_weight, conv_weight, conv_bias, A, ngroups, dstate, chunk_size, D=None, dt_bias=None,
+                      dt_softplus=False):
+    """A layer's operators on a prompt: u and residual (batch, seqlen, d + 2 * ngroups * dstate), the channels of
+    x, B and C side by side, are added and normalised, pass the short convolution, and the scan runs through
+    the chunk kernels.  Returns (out (batch, seqlen, nheads, headdim), residual, conv_state, state)."""
+    batch, seqlen, width = u.shape
+    nheads = A.shape[0]
+    d = width - 2 * ngroups * dstate
+    y, residual, _, _ = _add_rms_norm_fwd(u, norm_weight, residual=residual)
+    xbc, conv_state = _short_conv_fwd(y, conv_weight, bias=conv_bias, return_final_states=True)
+    x, B, C = xbc.split([d, ngroups * dstate, ngroups * dstate], dim=-1)
+    out, _, _, _, _, state = _mamba_chunk_scan_combined_fwd_concurrent(
+        x.unflatten(-1, (nheads, d // nheads)), dt, A, B.unflatten(-1, (ngroups, dstate)), C.unflatten(-1, (ngroups, dstate)), chunk_size, D,
+        dt_bias=dt_bias, dt_softplus=dt_softplus)
+    return out, residual, conv_state, state
+
+
+def _layer_token_step(u, residual, dt, norm_weight, conv_weight, conv_bias, A, ngroups, dstate, conv_state, state, D=None, dt_bias=None,
+                      dt_softplus=False, state_indices=None):
+    """The same operators on one more position of each sequence: u and residual (batch, d + 2 * ngroups * dstate),
+    dt (batch, nheads); conv_state and state, as `_layer_prompt_fwd` returns them or pools of slots, are
+    updated in place.  Returns (out (batch, nheads, headdim), residual)."""
+    nheads = A.shape[0]
+    d = u.shape[-1] - 2 * ngroups * dstate
+    y, residual, _, _ = _add_rms_norm_fwd(u, norm_weight, residual=residual)
+    xbc = _short_conv_step(y, conv_state, conv_weight, bias=conv_bias, state_indices=state_indices)
+    x, B, C = xbc.split([d, ngroups * dstate, ngroups * dstate], dim=-1)
+    out = _token_scan_step(state, x.unflatten(-1, (nheads, d // nheads)), dt, A, B.unflatten(-1, (ngroups, dstate)),
+                           C.unflatten(-1, (ngroups, dstate)), D=D, dt_bias=dt_bias, dt_softplus=dt_softplus, state_indices=state_indices)
+    return out, residual
+
+
+def check_prompt_then_tokens(seqlen=512, tokens=8, nheads=80, headdim=64, ngroups=1, dstate=128, chunk_size=256, dtype=torch.bfloat16, verbose=True):
+    """A prompt and `tokens` single steps behind it against the prompt that holds them all: within 1e-2 of the
+    largest value (the chunk kernels round their scaled operands to `dtype`, the step does not)."""
+    torch.manual_seed(42)
+    width = nheads * headdim + 2 * ngroups * dstate
+    u, residual = (torch.randn(2, seqlen + tokens, width, dtype=dtype, device="cuda") for _ in range(2))
+    dt = torch.rand(2, seqlen + tokens, nheads, dtype=dtype, device="cuda") * 0.5 + 0.5
+    params = dict(norm_weight=torch.ones(width, device="cuda"), conv_weight=torch.randn(width, 4, device="cuda") * 0.5,
+                  conv_bias=torch.randn(width, device="cuda") * 0.1, A=-torch.rand(nheads, device="cuda"), ngroups=ngroups, dstate=dstate)
+    more = dict(D=torch.randn(nheads, device="cuda"), dt_bias=torch.rand(nheads, device="cuda") * 0.5 - 0.25, dt_softplus=True)
+    whole = _layer_prompt_fwd(u, residual, dt, chunk_size=chunk_size, **params, **more)
+    _, _, conv_state, state = _layer_prompt_fwd(u[:, :seqlen], residual[:, :seqlen], dt[:, :seqlen], chunk_size=chunk_size, **params, **more)
+    outs = [_layer_token_step(u[:, t], residual[:, t], dt[:, t], conv_state=conv_state, state=state, **params, **more)[0]
+            for t in range(seqlen, seqlen + tokens)]
+    ok = True
+    for name, a, b in (("out", torch.stack(outs, 1), whole[0][:, seqlen:]), ("conv_state", conv_state, whole[2]), ("state", state, whole[3])):
+        err = ((a.float() - b.float()).abs().max() / b.float().abs().max()).item()
+        ok = ok and err <= 1e-2
+        if verbose:
+            print(f"    {name}: largest difference {err:.2e} of the largest value")
+    return ok
+
+
 def check_same_tensors(t1, t2, tensor_name, verbose=True):
     """Elementwise isclose(rtol=0.01, atol=0.001, equal_nan=True) as in main.py:109-143."""
     if t1 is None and t2 is None:
@@ -144,8 +206,10 @@ def main():
     concurrent = _mamba_chunk_scan_combined_fwd_concurrent(x, dt, A, B, C, chunk_size, D, dt_bias=dt_bias)
     print("-------------------- concurrent entry point vs original")
     ok2 = check_same_results(concurrent, original)
-    print("results:", "all good" if ok0 and ok1 and ok2 else "bad")
-    return ok0 and ok1 and ok2
+    print("-------------------- a prompt and its next tokens vs the longer prompt")
+    ok3 = check_prompt_then_tokens()
+    print("results:", "all good" if ok0 and ok1 and ok2 and ok3 else "bad")
+    return ok0 and ok1 and ok2 and ok3
 
 
 if __name__ == "__main__":

@@ -602,6 +602,28 @@ def test_chunk_kernels_then_tokens_per_head(cuda_device):
     assert ((state - whole[5]).abs().max() / whole[5].abs().max()).item() <= 1e-2
 
 
+@pytest.mark.parametrize("seqlen,nheads,ngroups", [(512, 8, 1), (300, 4, 2), (1, 8, 1)])
+def test_layer_pipeline_of_main(cuda_device, seqlen, nheads, ngroups):
+    """The layer's operators as the package's command runs them, also with slots of a pool."""
+    from mamba_fused_minimal_b200.main import _layer_prompt_fwd, _layer_token_step, check_prompt_then_tokens
+    assert check_prompt_then_tokens(seqlen=seqlen, tokens=3, nheads=nheads, ngroups=ngroups, verbose=False)
+    r = maker(seqlen)
+    h, p, n, dtype = nheads, 64, 128, torch.bfloat16
+    width = h * p + 2 * ngroups * n
+    u, res = r(2, seqlen + 1, width, dtype=dtype).to("cuda"), r(2, seqlen + 1, width, dtype=dtype).to("cuda")
+    dt = r(2, seqlen + 1, h, dtype=dtype).to("cuda")
+    kw = dict(norm_weight=torch.ones(width, device="cuda"), conv_weight=r(width, 4).to("cuda"), conv_bias=r(width).to("cuda"),
+              A=-torch.rand(h, device="cuda"), ngroups=ngroups, dstate=n, dt_softplus=True)
+    _, _, cs, st = _layer_prompt_fwd(u[:, :-1], res[:, :-1], dt[:, :-1], chunk_size=128, **kw)
+    cpool, spool = torch.zeros(5, 3, width, dtype=dtype, device="cuda"), torch.zeros(5, h, p, n, device="cuda")
+    idx = torch.tensor([4, 1], dtype=torch.int32, device="cuda")
+    cpool[idx.long()], spool[idx.long()] = cs, st
+    a, ra = _layer_token_step(u[:, -1], res[:, -1], dt[:, -1], conv_state=cs, state=st, **kw)
+    b, rb = _layer_token_step(u[:, -1], res[:, -1], dt[:, -1], conv_state=cpool, state=spool, state_indices=idx, **kw)
+    assert torch.equal(a, b) and torch.equal(ra, rb)
+    assert torch.equal(cpool[idx.long()], cs) and torch.equal(spool[idx.long()], st) and not spool[[0, 2, 3]].any()
+
+
 def test_captured_and_replayed(cuda_device):
     """Forward, gradients and steps captured into graphs; two graphs replayed side by side on two streams with
     other inputs each give what the eager calls give."""
