@@ -131,7 +131,7 @@ def build_ext(force=False, verbose=False):
             raise RuntimeError("build step failed: " + " ".join(cmd))
     cmd = ["g++", "-shared", "-o", EXT] + objs
     cmd += ["-L" + p for p in libdirs] + ["-L" + PKG]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-l:libssd_b200.so"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-l:libssd_b200.so"]
     cmd += ["-Wl,-rpath,$ORIGIN"] + ["-Wl,-rpath," + p for p in libdirs]
     _run(cmd, verbose)
     _write_stamp(EXT, stamp)

@@ -1,8 +1,10 @@
 // PyTorch front end of the operators around the scan (sections 8 to 10 of include/ssd_b200.h): the residual
 // addition + root-mean-square norm, the short causal convolution and the token-by-token selective scan.
 // Shapes are asserted in the Python shims; devices, types and strides are checked here.  Scratch memory is
-// allocated for each call, so two captured graphs never share any.
+// allocated for each call, so two captured graphs never share any.  The calls of a single token assert their
+// shapes here, with the shims' AssertionError: in Python that took as long as the rest of the call.
 #include <ATen/MemoryOverlap.h>
+#include <ATen/cuda/EmptyTensor.h>
 
 #include <limits>
 #include <tuple>
@@ -17,6 +19,14 @@ int32_t i32(int64_t v) {
   TORCH_CHECK(v <= std::numeric_limits<int32_t>::max(), "a size of ", v, " is too large");
   return static_cast<int32_t>(v);
 }
+
+void assert_shapes(bool ok, const char* what) {
+  if (ok) return;
+  PyErr_SetString(PyExc_AssertionError, what);
+  throw pybind11::error_already_set();
+}
+bool is_1d(const OptTensor& t, int64_t n) { return !t.has_value() || (t->dim() == 1 && t->size(0) == n); }
+bool is_like(const OptTensor& t, const Tensor& x) { return !t.has_value() || t->sizes() == x.sizes(); }
 
 void check_input(const Tensor& t) { TORCH_CHECK(t.is_cuda(), "x must be a CUDA tensor (libssd_b200 has no CPU path)"); }
 
@@ -43,7 +53,7 @@ int out_code(at::ScalarType st) {
 }
 
 Tensor scratch(size_t bytes, const Tensor& like) {
-  return torch::empty({(int64_t)bytes}, torch::dtype(torch::kUInt8).device(like.device()));
+  return at::detail::empty_cuda({(int64_t)bytes}, at::kByte, like.device(), c10::nullopt);
 }
 
 // a parameter: any of the three types, made contiguous
@@ -59,6 +69,10 @@ void param(const OptTensor& t, const Tensor& like, const char* name, Tensor& hol
 std::tuple<Tensor, OptTensor, OptTensor, OptTensor> add_rms_norm_fwd(const Tensor& x, const Tensor& weight, const OptTensor& residual,
                                                                   double eps, std::optional<at::ScalarType> out_dtype,
                                                                   std::optional<at::ScalarType> residual_dtype) {
+  assert_shapes((x.dim() == 2 || x.dim() == 3) && weight.dim() == 1 && weight.size(0) == x.size(-1) && is_like(residual, x),
+                "x (batch, seqlen, dim) or (rows, dim), weight (dim,), residual as x");
+  assert_shapes(!out_dtype.has_value() || *out_dtype == x.scalar_type() || *out_dtype == at::kChar || *out_dtype == at::kFloat8_e4m3fn,
+                "out_dtype: x's dtype, int8 or float8_e4m3fn");
   check_input(x);
   c10::cuda::CUDAGuard guard(x.device());
   check_inner(x, "x");
@@ -253,6 +267,9 @@ const int32_t* slots_of(const OptTensor& indices, const Tensor& like, Tensor& ho
 
 Tensor short_conv_step(const Tensor& x, Tensor conv_state, const Tensor& weight, const OptTensor& bias, bool silu,
                        const OptTensor& state_indices) {
+  assert_shapes(x.dim() == 2 && conv_state.dim() == 3 && weight.dim() == 2 && conv_state.size(2) == x.size(1) && weight.size(0) == x.size(1) &&
+                    weight.size(1) == conv_state.size(1) + 1 && is_1d(bias, x.size(1)) && is_1d(state_indices, x.size(0)),
+                "x (batch, channels), conv_state (slots, width - 1, channels), weight (channels, width), bias (channels,), state_indices (batch,)");
   check_input(x);
   c10::cuda::CUDAGuard guard(x.device());
   check_inner(x, "x");
@@ -433,6 +450,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
 Tensor token_scan_step(Tensor state, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                        const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias, bool dt_softplus, double dt_min, double dt_max,
                        const OptTensor& state_indices) {
+  const int64_t rank = x.dim(), batch = x.size(0), heads = rank > 1 ? x.size(1) : 0;
+  assert_shapes((rank == 2 || rank == 3) && state.dim() == rank + 1 && B.dim() == 3 && C.sizes() == B.sizes() && B.size(0) == batch && B.size(1) > 0 &&
+                    heads % B.size(1) == 0 && state.sizes().slice(1, rank - 1) == x.sizes().slice(1) && state.size(-1) == B.size(2),
+                "state (slots, nheads, headdim, dstate) with x (batch, nheads, headdim), or (slots, channels, dstate) with (batch, channels); "
+                "B and C (batch, ngroups, dstate)");
+  assert_shapes(dt.dim() == 2 && dt.size(0) == batch && dt.size(1) == heads && A.size(0) == heads &&
+                    (rank == 3 ? A.dim() == 1 : A.dim() == 2 && A.size(1) == B.size(2)) && is_like(z, x) && is_1d(dt_bias, heads) &&
+                    is_1d(state_indices, batch) &&
+                    (!D.has_value() || (D->dim() == 1 && D->size(0) == heads) || (rank == 3 && D->sizes() == x.sizes().slice(1))),
+                "dt (batch, nheads), A (nheads,) or (channels, dstate), D (nheads,) or (nheads, headdim), z as x, dt_bias (nheads,), "
+                "state_indices (batch,)");
   check_input(x);
   c10::cuda::CUDAGuard guard(x.device());
   check_cuda(state, x, "state");

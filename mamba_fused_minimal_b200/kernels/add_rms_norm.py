@@ -1,11 +1,7 @@
 """Residual addition + root-mean-square norm, the step that opens every layer around the scan: forward with
 an output in x's type or in 8 bits with one scale a row, and the gradients.  The reference has no
 counterpart (its path begins behind a layer's input projection)."""
-import torch
-
 from .._ext import C as _C
-
-_EIGHT_BITS = (torch.int8, torch.float8_e4m3fn)
 
 
 def _add_rms_norm_fwd(x, weight, residual=None, eps=1e-5, out_dtype=None, residual_dtype=None):
@@ -21,12 +17,8 @@ def _add_rms_norm_fwd(x, weight, residual=None, eps=1e-5, out_dtype=None, residu
     fp32), or in `residual_dtype` where there is no residual yet; None if neither is given.  rstd
     (rows..., fp32), of residual_out as it was kept, is for the gradients; scales (rows..., fp32) takes its
     place where out is in 8 bits (the other of the two is None)."""
-    assert x.dim() in (2, 3)
-    assert weight.shape == x.shape[-1:]
-    if residual is not None:
-        assert residual.shape == x.shape
-    assert out_dtype is None or out_dtype == x.dtype or out_dtype in _EIGHT_BITS
-    return _C.add_rms_norm_fwd(x, weight, residual, float(eps), out_dtype, residual_dtype)
+    # the front end asserts the shapes: a token's call is short
+    return _C.add_rms_norm_fwd(x, weight, residual, eps, out_dtype, residual_dtype)
 
 
 def _add_rms_norm_bwd(dout, total, weight, rstd, dresidual=None, x_dtype=None):
