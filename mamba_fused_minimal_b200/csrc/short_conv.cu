@@ -168,7 +168,7 @@ struct ConvBwdArgs {
 // loads are issued one group ahead; dx of a position is complete once dpre of the width - 1 positions after it
 // is known.
 template <typename T, int W, int V, bool SEQ>
-__global__ void __launch_bounds__(kConvThreads) short_conv_bwd_kernel(ConvBwdArgs g) {
+__global__ void __launch_bounds__(kConvThreads, 5) short_conv_bwd_kernel(ConvBwdArgs g) {
   const ConvArgs& a = g.f;
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
