@@ -233,17 +233,14 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
     };
     fetch(t_begin);
     prepare(0);
+    Pack<T, EV> xk = xr, xn = xr, zk;
     if (tiles > 1) fetch(t_begin + kTile);
-    for (int i = 0; i < tiles; ++i) {
+    for (int i = 0; i < tiles; ++i, xk = xn) {
       const int t0 = t_begin + i * kTile;
-      // x and z of the tile whose y is awaited, read (again) before the next one is prepared
-      Pack<T, EV> xk, zk;
-      if (!STATE) {
-        const int t = min(t0 + lt, t_end - 1);
-        xk = load_some<EV, VEC>(xp + (int64_t)t * a.x_sl, lcount);
-        if (a.z) zk = load_some<EV, VEC>(zp + (int64_t)t * a.z_sl, lcount);
-      }
+      // z of the tile whose y is awaited, read before the next one is prepared
+      if (!STATE && a.z) zk = load_some<EV, VEC>(zp + (int64_t)min(t0 + lt, t_end - 1) * a.z_sl, lcount);
       if (i + 1 < tiles) prepare(i + 1);
+      xn = xr;
       if (i + 2 < tiles) fetch(t0 + 2 * kTile);
       bar_sync<3, NT>(i & 1);
       const int count = t0 + lt < t_end ? lcount : 0;
@@ -426,8 +423,13 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
       }
       const int end = min(stop, half + SSD_TOKEN_SCAN_CHECKPOINT);
       if (resets == 0u) {
+if (end - half == SSD_TOKEN_SCAN_CHECKPOINT) {
+#pragma unroll
+          for (int k = 0; k < SSD_TOKEN_SCAN_CHECKPOINT; k += 4) four(half + k, s_du, s_bc, s_y, std::false_type(), 0u);
+        } else {
 #pragma unroll 1
         for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::false_type(), 0u);
+        }
       } else {
 #pragma unroll 1
         for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::true_type(), resets >> t);
