@@ -299,9 +299,11 @@ struct NormBwdArgs {
 // A block walks rows blockIdx.x, + gridDim.x, ...; each thread keeps its columns' share of the weight
 // gradient in registers and writes it once, as the block's row of `partial`.  The second kernel adds the
 // rows of `partial` in a fixed order, so the result does not depend on which block ran first.
-// The next row's loads are issued before this row's sum is joined, so the barrier's wait is theirs too.
+// Where the registers allow it (one vector per thread, up to 512 threads) the next row's loads are issued
+// before this row's sum is joined, so the barrier's wait is theirs too.
 template <typename T, typename S, int V, int VPT, int THREADS>
 __global__ void __launch_bounds__(THREADS) add_rms_norm_bwd_kernel(NormBwdArgs a) {
+  constexpr bool kNext = VPT == 1 && THREADS <= 512;
   __shared__ float slots[2][32];
   float w[VPT][V], dw[VPT][V];
   int col[VPT];
@@ -337,9 +339,10 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_bwd_kernel(NormBwdArgs a
     }
     r_next = a.rstd[row];
   };
-  fetch(blockIdx.x);
+  if (kNext) fetch(blockIdx.x);
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    if (!kNext) fetch(row);
     const float r = r_next;
     float g[VPT][V], hat[VPT][V], u[VPT][V], sums[V], s[V];
 #pragma unroll
@@ -359,7 +362,7 @@ __global__ void __launch_bounds__(THREADS) add_rms_norm_bwd_kernel(NormBwdArgs a
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) sum += sums[i];
-    if (row + gridDim.x < a.rows) fetch(row + gridDim.x);
+    if (kNext && row + gridDim.x < a.rows) fetch(row + gridDim.x);
     const float mean = block_reduce<false>(sum, slots[turn]) / (float)a.dim;
     float m[V];
 #pragma unroll
@@ -443,19 +446,31 @@ int bwd_parts(int64_t rows) {
 template <typename T, typename S, int V>
 int launch_norm_bwd_v(const NormBwdArgs& a, cudaStream_t stream) {
   int threads, vpt;
-  row_shape((a.dim + V - 1) / V, 0, V == 8 ? 2 : 4, &threads, &vpt);
+  row_shape((a.dim + V - 1) / V, 0, V == 8 ? 2 : V == 1 ? 8 : 4, &threads, &vpt);
   const int parts = bwd_parts(a.rows);
   switch (vpt) {
     case 1:
-      // up to 512 threads have the registers for the next row's values
       if (threads <= 512)
         add_rms_norm_bwd_kernel<T, S, V, 1, 512><<<parts, threads, 0, stream>>>(a);
       else
         add_rms_norm_bwd_kernel<T, S, V, 1, kMaxThreads><<<parts, threads, 0, stream>>>(a);
       break;
-    case 2: add_rms_norm_bwd_kernel<T, S, V, 2, kMaxThreads><<<parts, threads, 0, stream>>>(a); break;
+    case 2:
+      if (threads <= 640)
+        add_rms_norm_bwd_kernel<T, S, V, 2, 640><<<parts, threads, 0, stream>>>(a);
+      else
+        add_rms_norm_bwd_kernel<T, S, V, 2, kMaxThreads><<<parts, threads, 0, stream>>>(a);
+      break;
     case 4:
       if constexpr (V < 8) add_rms_norm_bwd_kernel<T, S, V, 4, kMaxThreads><<<parts, threads, 0, stream>>>(a);
+      break;
+    case 8:
+      if constexpr (V == 1) {
+        if (threads <= 640)
+          add_rms_norm_bwd_kernel<T, S, V, 8, 640><<<parts, threads, 0, stream>>>(a);
+        else
+          add_rms_norm_bwd_kernel<T, S, V, 8, kMaxThreads><<<parts, threads, 0, stream>>>(a);
+      }
       break;
     default:
       add_rms_norm_bwd_long_kernel<T, S><<<(unsigned)a.rows, 1024, 0, stream>>>(a);

@@ -32,18 +32,21 @@ constexpr int kLdy = 4 * kTile + 4, kY = kCh * kLdy + 16;
 __device__ __forceinline__ int du_row(int ch) { return ch * kLdu + (ch >> 3) * 16; }
 __device__ __forceinline__ int y_row(int ch) { return ch * kLdy + (ch >> 3) * 16; }
 
-constexpr int kHelpers = 64;       // threads that load, prepare and store
-constexpr int kVec = kTile * kCh / kHelpers;   // elements of x such a thread loads per tile
-constexpr int kPerRow = kCh / kVec;            // such vectors per position
+// Threads that load, prepare and store: twice as many where a position's B and C are longer (2048 channels of
+// 128: 1764 us with 64).
+constexpr int helpers(int lpc) { return lpc == 16 ? 128 : 64; }
 
 constexpr int resident(int threads, int states) {
-  return threads <= 128 ? 5 : threads <= 192 ? (states <= 8 ? 3 : 2) : (states <= 4 ? 2 : 1);
+  return threads <= 128 ? 5 : threads <= 192 ? 3 : states <= 8 ? 2 : 1;
 }
 
 // LPC lanes share a channel, a thread holds NS components of K channels.
 template <typename T, int LPC, int NS, int K>
 struct ScanShape {
   static constexpr int kCompute = kCh * LPC / K;      // threads that hold states
+  static constexpr int kHelpers = helpers(LPC);
+  static constexpr int kVec = kTile * kCh / kHelpers; // elements of x a preparing thread loads per tile
+  static constexpr int kPerRow = kCh / kVec;          // such threads per position
   static constexpr int kThreads = kCompute + kHelpers;
   static constexpr int kState = LPC * NS;             // components, padded
   static constexpr int kChunk = NS < 4 ? NS : 4;      // components that are read together
@@ -104,7 +107,7 @@ __device__ __forceinline__ void bar_arrive(int stage) {
 template <typename T, int LPC, int NS, int K, bool STATE, bool VEC>
 __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<T, LPC, NS, K>::kResident) token_scan_kernel(ScanArgs a) {
   using Sh = ScanShape<T, LPC, NS, K>;
-  constexpr int NT = Sh::kThreads, EV = kVec, CB = Sh::kChunk, GR = Sh::kGroups, CK = kCh / K;
+  constexpr int NT = Sh::kThreads, EV = Sh::kVec, CB = Sh::kChunk, GR = Sh::kGroups, CK = kCh / K;
   extern __shared__ float4 smem4[];
   // a stage: dt' rows, dt' x rows, y rows, bc [kTile][GR][LPC][B: CB, C: CB]
   float* const s_stage = reinterpret_cast<float*>(smem4);
@@ -121,7 +124,7 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
   if (threadIdx.x >= Sh::kCompute) {
     const int tid = threadIdx.x - Sh::kCompute;
     // what this thread loads and stores: EV channels of one position
-    const int lt = tid / kPerRow, lc = (tid % kPerRow) * EV;
+    const int lt = tid / Sh::kPerRow, lc = (tid % Sh::kPerRow) * EV;
     const int lcount = max(0, min(EV, nch - lc));
     const int lfrom = c0 + (lcount > 0 ? lc : 0);
     const T* xp = static_cast<const T*>(a.x) + b * a.x_sb + lfrom;
@@ -147,7 +150,7 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
     Pack<T, CB> bcr[Sh::kAhead ? Sh::kPer : 1];
     // Chunk k of this thread of a tile's B (first half) and C: CB components from `bn` on, of position
     // bt + a multiple of kStep.  A chunk's lane and group: component gl * CB = lane * NS + grp * CB.
-    constexpr int kStep = kHelpers / (GR * LPC), kHalf = Sh::kPer / 2;
+    constexpr int kStep = Sh::kHelpers / (GR * LPC), kHalf = Sh::kPer / 2;
     const int gl = tid % (GR * LPC), bt = tid / (GR * LPC), bn = gl * CB;
     const bool bin = bn < a.dstate;
     const T* const Bt = Bp + (VEC && !bin ? 0 : bn);
@@ -471,7 +474,7 @@ ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
   s.ns = n / s.lpc;
   // segments: only where less than half of the blocks that fit the GPU at once would run, as many as fill
   // it, and none shorter than 256 positions
-  const int64_t fit = 148 * resident(kCh * s.lpc / s.k + kHelpers, s.ns * s.k);
+  const int64_t fit = 148 * resident(kCh * s.lpc / s.k + helpers(s.lpc), s.ns * s.k);
   const int64_t want = fit / blocks, room = p.seqlen / 256;
   s.segments = (int)(want < room ? want : room);
   if (s.segments < 3) s.segments = 1;            // the state pass doubles the work
@@ -503,7 +506,7 @@ int launch_vec(const ScanArgs& a, int batch, cudaStream_t stream) {
 template <typename T, int LPC, int NS, int K>
 int launch_plan(const ScanArgs& a, const ssd_token_scan_params_t& p, cudaStream_t stream) {
   using Sh = ScanShape<T, LPC, NS, K>;
-  constexpr int CB = Sh::kChunk, EV = kVec;
+  constexpr int CB = Sh::kChunk, EV = Sh::kVec;
   // a thread's vector of channels begins at a multiple of its length within a group
   constexpr size_t kMost = EV * sizeof(T) < 16 ? EV * sizeof(T) : 16;
   const int ds = dtype_size(p.dt_dtype);

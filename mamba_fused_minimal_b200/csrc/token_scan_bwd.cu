@@ -30,9 +30,9 @@ struct ScanBwdArgs {
   void* dz;
   float* dinit;
   float* part_bc;      // (b, l, g, tiles_per_group, 2, n): the blocks' shares of dB and dC
-  float* part_A;       // (b, d, n)
-  float* part_D;       // (b, d)
-  float* part_bias;    // (b, d)
+  float* part_A;       // (b, segments, d, n)
+  float* part_D;       // (b, segments, d)
+  float* part_bias;    // (b, segments, d)
   int64_t d_sb, d_sl;
   int unit, unit32, unit_bc, unit_ck;   // bytes copied at a time of x and the like, of an fp32 dt, of B and C, of the states
 };
@@ -85,7 +85,8 @@ __device__ __forceinline__ void add_to(float& sum, float& lost, float v) {
   sum = t;
 }
 
-template <typename T, int NP>
+// CARRY: only what a segment passes on to the one before it, from zero behind it, and the sum of its dt'.
+template <typename T, int NP, bool CARRY>
 __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdArgs q) {
   using Sh = BwdShape<T, NP>;
   constexpr int NT = kBwdThreads, CH = Sh::kChannels, SL = Sh::kSlabs, ROW = Sh::kRow, PER = Sh::kPer, NBC = Sh::kPerBc;
@@ -102,11 +103,13 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   float* s_bc = s_p + 2 * CH * SL * kPitch;          // [warps][kT][ROW]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int grp = blockIdx.x / a.tiles_per_group, tile_c = blockIdx.x % a.tiles_per_group;
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, seg = CARRY ? blockIdx.z + 1 : blockIdx.z;      // nothing needs what the first one passes on
+  const int t_lo = seg * a.seg_len, t_hi = min(a.seqlen, t_lo + a.seg_len);
+  const int64_t bs = (int64_t)b * a.segments + seg;
   const int c0 = grp * a.per_group + tile_c * CH;
   const int nch = min(CH, a.per_group - tile_c * CH);
   const int tiles = (a.seqlen + kT - 1) / kT;
-  const int last = (tiles - 1) * kT;                 // first position of the tile the walk begins with
+  const int last = t_lo + (t_hi - t_lo - 1) / kT * kT;   // first position of the tile the walk begins with
 
   // The tiles' values come through two buffers of shared memory: the copies of the next tile are in flight
   // while one is walked (held in registers they did not fit beside the walk: what was loaded was spilled,
@@ -129,7 +132,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
         if (a.z) rows(2 * kOne, a.z, b * a.z_sb, a.z_sl);
         break;
       case 3:
-        if (a.z) rows(3 * kOne, a.out_x, (row - t0) * a.channels, a.channels);
+        if (a.z && !CARRY) rows(3 * kOne, a.out_x, (row - t0) * a.channels, a.channels);
         break;
       case 4:
         if (a.dt_f32)
@@ -138,10 +141,12 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
         else
           rows(4 * kOne + 2 * kBC, a.dt, b * a.dt_sb, a.dt_sl);
         break;
-      case 5: states(4 * kOne, a.B, b * a.B_sb + grp * a.B_sg, a.B_sl); break;
+      case 5:
+        if (!CARRY) states(4 * kOne, a.B, b * a.B_sb + grp * a.B_sg, a.B_sl);
+        break;
       case 6: states(4 * kOne + kBC, a.C, b * a.C_sb + grp * a.C_sg, a.C_sl); break;
       default:
-        copy_rows<NP * 4>(raw + Sh::kRaw16 * ES + Sh::kItems * 4,
+        if (!CARRY) copy_rows<NP * 4>(raw + Sh::kRaw16 * ES + Sh::kItems * 4,
                           reinterpret_cast<const char*>(a.ckpt + (((int64_t)b * tiles + t0 / kT) * a.channels + c0) * a.dstate), (int64_t)a.dstate * 4, nch,
                           nch, a.dstate * 4, q.unit_ck, 4, lane);
     }
@@ -163,7 +168,18 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   const int at_n = has ? (c0 + ch) * a.dstate + n : 0;            // of a (channels, dstate) tensor
   const int64_t ck_step = (int64_t)a.channels * a.dstate;
   const float A = has ? load_f(a.A, a.A_dtype, at_n) : 0.0f;
-  float carry = has && q.dfinal ? q.dfinal[b * ck_step + at_n] : 0.0f;      // a_{t+1} g_{t+1}
+  float carry = has && q.dfinal && !CARRY ? q.dfinal[b * ck_step + at_n] : 0.0f;      // a_{t+1} g_{t+1}
+  if (!CARRY && has) {
+    // through the segments behind, from the last one on
+    for (int j = a.segments - 1; j > seg; --j) {
+      const int64_t at = (int64_t)b * a.segments + j;
+      const float2 dec = a.seg_decay[at * a.channels + c0 + ch];
+      const bool keeps = dec.y != 0.0f && (j < a.segments - 1 || q.dfinal != nullptr);      // else there is nothing to keep
+      carry = (keeps ? ex2_approx(A * kLog2e * dec.x) * carry : 0.0f) + a.seg_state[at * ck_step + at_n];
+    }
+  }
+  float sum_dt = 0.0f;
+  bool dropped = false;
   float sum_A = 0.0f, lost_A = 0.0f;
 
   // B and C: component bn of positions bt, bt + kBcStep, ...; the first half of the items is B (with eight
@@ -187,7 +203,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   int buf = 0;
-  for (int t0 = last; t0 >= 0; t0 -= kT, buf ^= 1) {
+  for (int t0 = last; t0 >= t_lo; t0 -= kT, buf ^= 1) {
     const T* const raw = reinterpret_cast<const T*>(s_raw + buf * Sh::kRaw);
     const float* const raw32 = reinterpret_cast<const float*>(s_raw + buf * Sh::kRaw + Sh::kRaw16 * ES);
     float d[PER], x[PER], dy[PER], slope[PER];         // slope: d dt' / d dt
@@ -211,7 +227,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
       dy[e] = in ? widen(raw[Sh::kItems + item]) : 0.0f;
       if (a.z) {
         const float zv = widen(raw[2 * Sh::kItems + item]), s = sigmoid_f(zv);
-        if (in) static_cast<T*>(q.dz)[own + (int64_t)t * a.channels + c] = 
+        if (in && !CARRY) static_cast<T*>(q.dz)[own + (int64_t)t * a.channels + c] = 
             narrow<T>(dy[e] * widen(raw[3 * Sh::kItems + item]) * (s * (1.0f + zv * (1.0f - s))));
         dy[e] = in ? dy[e] * (zv * s) : 0.0f;
       }
@@ -232,8 +248,25 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
     float h = has ? raw32[Sh::kItems + ch * NP + n] : 0.0f;
     const uint32_t resets = a.seq ? reset_mask(a, b, t0, lane) : 0u;
     __syncthreads();
-    if (t0 > 0) fetch(t0 - kT, buf ^ 1);
+    if (t0 > t_lo) fetch(t0 - kT, buf ^ 1);
 
+    const auto pass = [&](auto reset) {
+      constexpr bool RESET = decltype(reset)::value;
+#pragma unroll
+      for (int t = kT - 4; t >= 0; t -= 4) {
+        const float4 d4 = *reinterpret_cast<const float4*>(&s_d[ch * kPitch + t]);
+        const float4 g4 = *reinterpret_cast<const float4*>(&s_g[ch * kPitch + t]);
+        const float4 C4 = *reinterpret_cast<const float4*>(&s_C[n * kPitch + t]);
+        const float d[4] = {d4.x, d4.y, d4.z, d4.w}, y[4] = {g4.x, g4.y, g4.z, g4.w}, c[4] = {C4.x, C4.y, C4.z, C4.w};
+#pragma unroll
+        for (int i = 3; i >= 0; --i) {
+          carry = fmaf(c[i], y[i], carry) * ex2_approx(d[i] * (A * kLog2e));
+          if (RESET && (resets >> (t + i) & 1u)) carry = 0.0f;
+        }
+        sum_dt += (d[0] + d[1]) + (d[2] + d[3]);
+      }
+      dropped |= RESET;
+    };
     const auto walk = [&](auto reset) {
       constexpr bool RESET = decltype(reset)::value;
       // forwards through the tile: the decays, and what of the state before reaches each position; pairs are
@@ -321,12 +354,22 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
       unpack2(sum_A2, lo, hi);
       add_to(sum_A, lost_A, lo + hi);
     };
-    if (resets == 0u)
-      walk(std::false_type());
-    else
-      walk(std::true_type());
+    // the vote covers 32 positions, of which the tile has the first sixteen
+    const bool plain = (resets & 0xffffu) == 0u;
+    if constexpr (CARRY) {
+      if (plain)
+        pass(std::false_type());
+      else
+        pass(std::true_type());
+    } else {
+      if (plain)
+        walk(std::false_type());
+      else
+        walk(std::true_type());
+    }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
+    if constexpr (CARRY) continue;
 
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
@@ -367,9 +410,16 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
     }
   }
 
+  if constexpr (CARRY) {
+    if (has) {
+      a.seg_state[bs * ck_step + at_n] = carry;
+      if (n == 0) a.seg_decay[bs * a.channels + c0 + ch] = make_float2(sum_dt, dropped ? 0.0f : 1.0f);
+    }
+    return;
+  }
   if (has) {
-    q.part_A[b * ck_step + at_n] = sum_A;
-    if (q.dinit) q.dinit[b * ck_step + at_n] = carry;
+    q.part_A[bs * ck_step + at_n] = sum_A;
+    if (q.dinit && seg == 0) q.dinit[b * ck_step + at_n] = carry;
   }
   // dD and the bias's gradient: over the threads of a channel in order
   __syncthreads();
@@ -379,8 +429,8 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   if (tid < nch) {
     float u = 0.0f, v = 0.0f;
     for (int s = tid; s < min(NT, Sh::kItems); s += CH) u += s_bc[s], v += s_bc[NT + s];
-    q.part_D[(int64_t)b * a.channels + c0 + tid] = u;
-    q.part_bias[(int64_t)b * a.channels + c0 + tid] = v;
+    q.part_D[bs * a.channels + c0 + tid] = u;
+    q.part_bias[bs * a.channels + c0 + tid] = v;
   }
 }
 
@@ -414,8 +464,8 @@ __global__ void __launch_bounds__(256) sum_bc_kernel(const float* part, T* dB, T
   }
 }
 
-// dA, dD and the bias's gradient: over the batch in order.
-__global__ void __launch_bounds__(256) sum_batch_kernel(ScanBwdArgs q, int batch, float* dA, float* dD, float* dbias) {
+// dA, dD and the bias's gradient: over the batch and its segments in order.
+__global__ void __launch_bounds__(256) sum_batch_kernel(ScanBwdArgs q, int parts, float* dA, float* dD, float* dbias) {
   const int64_t dn = (int64_t)q.f.channels * q.f.dstate, d = q.f.channels;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const float* p;
@@ -433,7 +483,7 @@ __global__ void __launch_bounds__(256) sum_batch_kernel(ScanBwdArgs q, int batch
   if (out == nullptr) return;
   float v = 0.0f;
 #pragma unroll 4
-  for (int b = 0; b < batch; ++b) v += p[b * pitch + at];
+  for (int b = 0; b < parts; ++b) v += p[b * pitch + at];
   out[at] = v;
 }
 
@@ -444,15 +494,30 @@ int bwd_tiles(const ssd_token_scan_params_t& p) {
   return (p.channels / p.ngroups + ch - 1) / ch;
 }
 
+// Segments: where less than half of the blocks that fit the GPU would run, as many as fill it, none shorter
+// than 128 positions.  The pass that finds what a segment hands on costs a quarter of the walk.
+int bwd_segments(const ssd_token_scan_params_t& p, int* seg_len) {
+  const int64_t blocks = (int64_t)p.batch * p.ngroups * bwd_tiles(p);
+  const int64_t want = 2 * 148 / blocks, room = p.seqlen / 128;
+  int64_t n = want < room ? want : room;
+  if (n < 2) n = 1;
+  *seg_len = (int)(((p.seqlen + n - 1) / n + kT - 1) / kT * kT);
+  return (p.seqlen + *seg_len - 1) / *seg_len;
+}
+
 struct BwdWorkspace {
-  size_t bc, A, D, total;      // offsets in floats: shares of dB and dC, dA, dD; the bias's follow dD's
+  size_t bc, A, D, state, decay, total;      // offsets in floats; the bias's shares follow dD's
 };
 BwdWorkspace bwd_workspace(const ssd_token_scan_params_t& p) {
+  int seg_len;
+  const size_t segments = bwd_segments(p, &seg_len), dn = (size_t)p.channels * p.dstate;
   BwdWorkspace w;
-  w.bc = 0;
-  w.A = (size_t)p.batch * p.seqlen * p.ngroups * bwd_tiles(p) * 2 * p.dstate;
-  w.D = w.A + (size_t)p.batch * p.channels * p.dstate;
-  w.total = w.D + 2 * (size_t)p.batch * p.channels;
+  w.decay = 0;                               // pairs: the first, for their alignment
+  w.bc = w.decay + (segments > 1 ? 2 * (size_t)p.batch * segments * p.channels : 0);
+  w.A = w.bc + (size_t)p.batch * p.seqlen * p.ngroups * bwd_tiles(p) * 2 * p.dstate;
+  w.D = w.A + (size_t)p.batch * segments * dn;
+  w.state = w.D + 2 * (size_t)p.batch * segments * p.channels;
+  w.total = w.state + (segments > 1 ? (size_t)p.batch * segments * dn : 0);
   return w;
 }
 
@@ -479,8 +544,17 @@ int launch_bwd(ScanBwdArgs& q, int batch, cudaStream_t stream) {
   q.unit_bc = copy_unit(a.dstate * es, at(a.B), a.B_sb * es, a.B_sl * es, a.B_sg * es, at(a.C), a.C_sb * es, a.C_sl * es, a.C_sg * es);
   q.unit_ck = copy_unit(a.dstate * 4, at(a.ckpt));
   if (smem > 48 * 1024)
-    SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_bwd_kernel<T, NP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  token_scan_bwd_kernel<T, NP><<<dim3(q.f.ngroups * q.f.tiles_per_group, batch), kBwdThreads, smem, stream>>>(q);
+    SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_bwd_kernel<T, NP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  dim3 grid(a.ngroups * a.tiles_per_group, batch, a.segments);
+  if (a.segments > 1) {
+    if (smem > 48 * 1024)
+      SSD_CUDA_OK(cudaFuncSetAttribute(token_scan_bwd_kernel<T, NP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    grid.z = a.segments - 1;
+    token_scan_bwd_kernel<T, NP, true><<<grid, kBwdThreads, smem, stream>>>(q);
+    SSD_CUDA_OK(cudaGetLastError());
+    grid.z = a.segments;
+  }
+  token_scan_bwd_kernel<T, NP, false><<<grid, kBwdThreads, smem, stream>>>(q);
   SSD_CUDA_OK(cudaGetLastError());
   return SSD_OK;
 }
@@ -502,7 +576,10 @@ int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t str
   q.part_bc = ws + w.bc;
   q.part_A = ws + w.A;
   q.part_D = ws + w.D;
-  q.part_bias = q.part_D + (size_t)p.batch * p.channels;
+  q.f.segments = bwd_segments(p, &q.f.seg_len);
+  q.part_bias = q.part_D + (size_t)p.batch * q.f.segments * p.channels;
+  q.f.seg_state = ws + w.state;
+  q.f.seg_decay = reinterpret_cast<float2*>(ws + w.decay);
   q.d_sb = r.dout_stride[0], q.d_sl = r.dout_stride[1];
   SSD_REQUIRE(p.batch <= 65535 && (int64_t)p.batch * p.seqlen * p.ngroups <= 0x7fffffff, SSD_ERR_UNSUPPORTED,
               "token scan: batch %d, seqlen %d or ngroups %d too large", p.batch, p.seqlen, p.ngroups);
@@ -524,7 +601,7 @@ int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t str
                                                                q.f.tiles_per_group, p.dstate);
     SSD_CUDA_OK(cudaGetLastError());
     const int64_t par = (int64_t)p.channels * (p.dstate + 2);
-    sum_batch_kernel<<<(unsigned)((par + 255) / 256), 256, 0, stream>>>(q, p.batch, r.dA, r.dD, r.ddt_bias);
+    sum_batch_kernel<<<(unsigned)((par + 255) / 256), 256, 0, stream>>>(q, p.batch * q.f.segments, r.dA, r.dD, r.ddt_bias);
     SSD_CUDA_OK(cudaGetLastError());
     return SSD_OK;
   });
