@@ -223,10 +223,16 @@ __device__ __forceinline__ float softplus_f(float v) {
   r = fmaf(s * s2, r, s);
   return fmaf(2.0f, r, fmaxf(v, 0.0f));          // r is a NaN where v is
 }
+// v held between lo and hi; a NaN stays one
+__device__ __forceinline__ float clamp_f(float v, float lo, float hi) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(lo));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(hi));
+  return r;
+}
 // dt' of one position and channel
 __device__ __forceinline__ float scan_dt(float raw, bool softplus, float lo, float hi) {
-  const float v = softplus ? softplus_f(raw) : raw;
-  return fminf(fmaxf(v, lo), hi);
+  return clamp_f(softplus ? softplus_f(raw) : raw, lo, hi);
 }
 
 // ---- block-wide sum and maximum --------------------------------------------------------------------

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
           for (int e = 0; e < EV / 2; ++e) {
             float v[2];
             unpack2(d[e], v[0], v[1]);
-            d[e] = pack2(fminf(fmaxf(v[0], a.dt_min), a.dt_max), fminf(fmaxf(v[1], a.dt_min), a.dt_max));
+            d[e] = pack2(clamp_f(v[0], a.dt_min, a.dt_max), clamp_f(v[1], a.dt_min, a.dt_max));
           }
         }
 #pragma unroll

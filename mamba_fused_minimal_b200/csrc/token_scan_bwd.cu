@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
       }
       if (a.limits) {
         if (d[e] < a.dt_min || d[e] > a.dt_max) slope[e] = 0.0f;
-        d[e] = fminf(fmaxf(d[e], a.dt_min), a.dt_max);
+        d[e] = clamp_f(d[e], a.dt_min, a.dt_max);
       }
       if (!in) d[e] = 0.0f;
       dy[e] = in ? widen(raw[Sh::kItems + item]) : 0.0f;

@@ -244,6 +244,31 @@ def test_conv_in_pieces_is_the_whole(cuda_device):
     assert torch.equal(pool[idx.long()], x[:, 47:50])
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """Batch and position strides whose products pass 2^31 elements: rows of one huge buffer."""
+    norm, conv, scan = ops()
+    l, d, n = 5, 64, 16
+    pitch = 2 ** 31 // 4 + 64                          # elements between positions: the fifth lies past 2^31
+    buf = torch.zeros(4 * pitch + 4096, dtype=torch.bfloat16, device="cuda")
+    r = maker(60)
+    small = r(1, l, 3 * d + 2 * n, dtype=torch.bfloat16).to("cuda")
+    big = torch.as_strided(buf, (1, l, 3 * d + 2 * n), (4 * pitch, pitch, 1))
+    big.copy_(small)
+    w, cw, A = torch.ones(d, device="cuda"), r(d, 4).to("cuda"), -torch.rand(d, n, device="cuda")
+
+    def work(t):
+        x, dt, z, B, C = t.split([d, d, d, n, n], dim=-1)
+        B, C = B.unsqueeze(2), C.unsqueeze(2)
+        y, total, rstd, _ = norm._add_rms_norm_fwd(x, w, residual=z)
+        c, _ = conv._short_conv_fwd(x, cw)
+        out, fin, saved = scan._token_scan_fwd(x, dt, A, B, C, z=z, dt_softplus=True, for_backward=True)
+        g = scan._token_scan_bwd(dt, x, dt, A, B, C, saved, z=z, dt_softplus=True)
+        return [y, total, rstd, c, *conv._short_conv_bwd(dt, x, cw)[:2], *norm._add_rms_norm_bwd(dt, x, w, rstd, dresidual=z), out, fin, *g]
+
+    for a, b in zip(work(big), work(small)):
+        assert (a is None and b is None) or torch.equal(a, b)
+
+
 def test_conv_masked_positions_may_hold_anything(cuda_device):
     """What another sequence holds does not reach a position, infinities and NaN included; forward and dx."""
     _, conv, _ = ops()
@@ -412,6 +437,36 @@ def test_scan_dt_limits(cuda_device, dt_limit):
         g = scan._token_scan_bwd(dout.to("cuda"), *pos, saved, **kw)
         assert norm_err(g[1], leaves["dt"].grad) <= 256 * U * math.sqrt(60)
         assert torch.equal(g[1].cpu() == 0, leaves["dt"].grad == 0)
+
+
+@pytest.mark.parametrize("dt_limit", [(0.0, float("inf")), (0.01, 0.2)])
+def test_scan_infinities_and_nan_stay_in_their_channel(cuda_device, dt_limit):
+    """A NaN or an infinity in one channel's x or dt reaches that channel from there on and no other, forward,
+    gradients of the other channels and steps alike; a clamp does not swallow it."""
+    scan = ops()[2]
+    inp = {k: v.to("cuda") for k, v in scan_inputs(1, 50, 40, 16, 1, torch.float32, 33).items()}
+    keys = ("x", "dt", "A", "B", "C")
+    kw = dict(dt_softplus=True, dt_limit=dt_limit)
+    good, gfin, gsaved = scan._token_scan_fwd(*[inp[k] for k in keys], for_backward=True, **kw)
+    others = [c for c in range(40) if c not in (3, 17)]
+    for key in ("x", "dt"):
+        bad = dict(inp)
+        bad[key] = inp[key].clone()
+        bad[key][:, 20, 3] = float("nan")
+        bad[key][:, 25, 17] = float("inf")
+        got, fin, saved = scan._token_scan_fwd(*[bad[k] for k in keys], for_backward=True, **kw)
+        assert torch.equal(got[..., others], good[..., others]) and torch.equal(fin[:, others], gfin[:, others])
+        assert torch.equal(got[:, :20, 3], good[:, :20, 3]) and torch.equal(got[:, :25, 17], good[:, :25, 17])
+        assert got[:, 20:, 3].isnan().all() and fin[:, 3].isnan().all()
+        dout = torch.ones_like(good)
+        a = scan._token_scan_bwd(dout, *[inp[k] for k in keys], gsaved, **kw)
+        b = scan._token_scan_bwd(dout, *[bad[k] for k in keys], saved, **kw)
+        for i in (0, 1):                                # dx, ddt
+            assert torch.equal(a[i][..., others], b[i][..., others])
+        assert torch.equal(a[2][others], b[2][others])  # dA
+        st = torch.zeros(1, 40, 16, device="cuda")
+        out = scan._token_scan_step(st, bad["x"][:, 20], bad["dt"][:, 20], inp["A"], inp["B"][:, 20], inp["C"][:, 20], **kw)
+        assert out[:, 3].isnan().all() and torch.isfinite(out[:, others]).all() and torch.isfinite(st[:, others]).all()
 
 
 def test_scan_packed_sequences_are_the_sequences(cuda_device):
