@@ -434,57 +434,58 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   }
 }
 
-// dB and dC of one (position, group): over the blocks' shares in order, eight strides of blocks side by side
-// joined in order (one thread a sum was bound by the latency of its chain of loads: 160 us for 4096
-// positions of 320 blocks).
+// The blocks' shares, joined in a fixed order.  Block i < rows: dB and dC of one (position, group) over the
+// channel blocks, eight strides side by side (one thread a sum was bound by the latency of its chain of loads:
+// 160 us for 4096 positions of 320 blocks).  The blocks behind: dA, dD and the bias's gradient over the batch and
+// its segments, one thread an element.
 template <typename T>
-__global__ void __launch_bounds__(256) sum_bc_kernel(const float* part, T* dB, T* dC, int64_t rows, int tiles, int dstate) {
+__global__ void __launch_bounds__(256) sum_shares_kernel(ScanBwdArgs q, T* dB, T* dC, float* dA, float* dD, float* dbias, int rows, int parts) {
   __shared__ float s[8][33];
-  const int64_t row = blockIdx.x;
-  const float* p = part + row * tiles * (2 * dstate);
-  for (int j0 = 0; j0 < 2 * dstate; j0 += 32) {
-    const int j = j0 + threadIdx.x;
-    float v = 0.0f;
-    if (j < 2 * dstate) {
+  const int dstate = q.f.dstate, tiles = q.f.tiles_per_group;
+  if ((int)blockIdx.x < rows) {
+    const int64_t row = blockIdx.x;
+    const float* p = q.part_bc + row * tiles * (2 * dstate);
+    for (int j0 = 0; j0 < 2 * dstate; j0 += 32) {
+      const int j = j0 + threadIdx.x;
+      float v = 0.0f;
+      if (j < 2 * dstate) {
 #pragma unroll 8
-      for (int k = threadIdx.y; k < tiles; k += 8) v += p[(int64_t)k * 2 * dstate + j];
-    }
-    s[threadIdx.y][threadIdx.x] = v;
-    __syncthreads();
-    if (threadIdx.y == 0 && j < 2 * dstate) {
-      float u = 0.0f;
+        for (int k = threadIdx.y; k < tiles; k += 8) v += p[(int64_t)k * 2 * dstate + j];
+      }
+      s[threadIdx.y][threadIdx.x] = v;
+      __syncthreads();
+      if (threadIdx.y == 0 && j < 2 * dstate) {
+        float u = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) u += s[k][threadIdx.x];
-      if (j < dstate)
-        dB[row * dstate + j] = narrow<T>(u);
-      else
-        dC[row * dstate + j - dstate] = narrow<T>(u);
+        for (int k = 0; k < 8; ++k) u += s[k][threadIdx.x];
+        if (j < dstate)
+          dB[row * dstate + j] = narrow<T>(u);
+        else
+          dC[row * dstate + j - dstate] = narrow<T>(u);
+      }
+      __syncthreads();
     }
-    __syncthreads();
-  }
-}
-
-// dA, dD and the bias's gradient: over the batch and its segments in order.
-__global__ void __launch_bounds__(256) sum_batch_kernel(ScanBwdArgs q, int parts, float* dA, float* dD, float* dbias) {
-  const int64_t dn = (int64_t)q.f.channels * q.f.dstate, d = q.f.channels;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const float* p;
-  float* out;
-  int64_t at, pitch;
-  if (i < dn) {
-    p = q.part_A, out = dA, at = i, pitch = dn;
-  } else if (i < dn + d) {
-    p = q.part_D, out = dD, at = i - dn, pitch = d;
-  } else if (i < dn + 2 * d) {
-    p = q.part_bias, out = dbias, at = i - dn - d, pitch = d;
-  } else {
     return;
+  }
+  const int64_t dn = (int64_t)q.f.channels * dstate, d = q.f.channels;
+  int64_t i = (int64_t)(blockIdx.x - rows) * 256 + threadIdx.y * 32 + threadIdx.x;
+  const float* p = q.part_A;
+  float* out = dA;
+  int64_t pitch = dn;
+  if (i >= dn) {
+    i -= dn;
+    p = q.part_D, out = dD, pitch = d;
+    if (i >= d) {
+      i -= d;
+      p = q.part_bias, out = dbias;
+      if (i >= d) return;
+    }
   }
   if (out == nullptr) return;
   float v = 0.0f;
 #pragma unroll 4
-  for (int b = 0; b < parts; ++b) v += p[b * pitch + at];
-  out[at] = v;
+  for (int b = 0; b < parts; ++b) v += p[b * pitch + i];
+  out[i] = v;
 }
 
 int padded_state(int n) { return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : 256; }
@@ -581,7 +582,7 @@ int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t str
   q.f.seg_state = ws + w.state;
   q.f.seg_decay = reinterpret_cast<float2*>(ws + w.decay);
   q.d_sb = r.dout_stride[0], q.d_sl = r.dout_stride[1];
-  SSD_REQUIRE(p.batch <= 65535 && (int64_t)p.batch * p.seqlen * p.ngroups <= 0x7fffffff, SSD_ERR_UNSUPPORTED,
+  SSD_REQUIRE(p.batch <= 65535 && (int64_t)p.batch * p.seqlen * p.ngroups <= 0x3fffffff, SSD_ERR_UNSUPPORTED,
               "token scan: batch %d, seqlen %d or ngroups %d too large", p.batch, p.seqlen, p.ngroups);
   SSD_REQUIRE((int64_t)p.channels * p.dstate <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "token scan: %d channels of %d too many", p.channels, p.dstate);
   return with_type(p.x_dtype, [&](auto t) -> int {
@@ -596,12 +597,9 @@ int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t str
       default: rc = launch_bwd<T, 256>(q, p.batch, stream); break;
     }
     if (rc != SSD_OK) return rc;
-    const int64_t rows = (int64_t)p.batch * p.seqlen * p.ngroups;
-    sum_bc_kernel<T><<<(unsigned)rows, dim3(32, 8), 0, stream>>>(q.part_bc, static_cast<T*>(r.dB), static_cast<T*>(r.dC), rows,
-                                                               q.f.tiles_per_group, p.dstate);
-    SSD_CUDA_OK(cudaGetLastError());
-    const int64_t par = (int64_t)p.channels * (p.dstate + 2);
-    sum_batch_kernel<<<(unsigned)((par + 255) / 256), 256, 0, stream>>>(q, p.batch * q.f.segments, r.dA, r.dD, r.ddt_bias);
+    const int64_t rows = (int64_t)p.batch * p.seqlen * p.ngroups, params = ((int64_t)p.channels * (p.dstate + 2) + 255) / 256;
+    sum_shares_kernel<T><<<(unsigned)(rows + params), dim3(32, 8), 0, stream>>>(q, static_cast<T*>(r.dB), static_cast<T*>(r.dC), r.dA, r.dD, r.ddt_bias,
+                                                                               (int)rows, p.batch * q.f.segments);
     SSD_CUDA_OK(cudaGetLastError());
     return SSD_OK;
   });

@@ -1,8 +1,8 @@
 // PyTorch front end of the operators around the scan (sections 8 to 10 of include/ssd_b200.h): the residual
 // addition + root-mean-square norm, the short causal convolution and the token-by-token selective scan.
-// Shapes are asserted in the Python shims; devices, types and strides are checked here.  Scratch memory is
-// allocated for each call, so two captured graphs never share any.  The calls of a single token assert their
-// shapes here, with the shims' AssertionError: in Python that took as long as the rest of the call.
+// Scratch memory is
+// allocated for each call, so two captured graphs never share any.  Shapes are asserted here, with the
+// AssertionError that the other shims raise in Python: for small calls that took as long as the rest of it.
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 
@@ -26,6 +26,10 @@ void assert_shapes(bool ok, const char* what) {
   throw pybind11::error_already_set();
 }
 bool is_1d(const OptTensor& t, int64_t n) { return !t.has_value() || (t->dim() == 1 && t->size(0) == n); }
+bool is_3d(const OptTensor& t, int64_t a, int64_t b, int64_t c) {
+  return !t.has_value() || (t->dim() == 3 && t->size(0) == a && t->size(1) == b && t->size(2) == c);
+}
+bool is_2d(const OptTensor& t, int64_t a, int64_t b) { return !t.has_value() || (t->dim() == 2 && t->size(0) == a && t->size(1) == b); }
 bool is_like(const OptTensor& t, const Tensor& x) { return !t.has_value() || t->sizes() == x.sizes(); }
 
 void check_input(const Tensor& t) { TORCH_CHECK(t.is_cuda(), "x must be a CUDA tensor (libssd_b200 has no CPU path)"); }
@@ -174,6 +178,11 @@ struct ConvHold {
 
 void fill_conv(ssd_short_conv_params_t& p, ConvHold& h, const Tensor& x, const Tensor& weight, const OptTensor& bias, bool silu,
                const OptTensor& initial_states, const OptTensor& seq_idx) {
+  assert_shapes(x.dim() == 3 && weight.dim() == 2 && weight.size(0) == x.size(2) && is_1d(bias, x.size(2)) &&
+                    is_3d(initial_states, x.size(0), weight.size(1) - 1, x.size(2)) && is_2d(seq_idx, x.size(0), x.size(1)),
+                "x (batch, seqlen, channels), weight (channels, width), bias (channels,), initial_states (batch, width - 1, channels), "
+                "seq_idx (batch, seqlen)");
+  check_input(x);
   check_inner(x, "x");
   p.x = x.data_ptr();
   p.x_dtype = dtype_code(x, "x");
@@ -200,8 +209,7 @@ void fill_conv(ssd_short_conv_params_t& p, ConvHold& h, const Tensor& x, const T
 
 std::tuple<Tensor, OptTensor> short_conv_fwd(const Tensor& x, const Tensor& weight, const OptTensor& bias, bool silu,
                                              const OptTensor& initial_states, const OptTensor& seq_idx, bool return_final) {
-  check_input(x);
-  c10::cuda::CUDAGuard guard(x.device());
+  c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
   ssd_short_conv_params_t p{};
   ConvHold h;
   fill_conv(p, h, x, weight, bias, silu, initial_states, seq_idx);
@@ -219,14 +227,15 @@ std::tuple<Tensor, OptTensor> short_conv_fwd(const Tensor& x, const Tensor& weig
 std::tuple<Tensor, Tensor, OptTensor, OptTensor> short_conv_bwd(const Tensor& dout, const Tensor& x, const Tensor& weight,
                                                                 const OptTensor& bias, bool silu, const OptTensor& initial_states,
                                                                 const OptTensor& seq_idx, const OptTensor& dfinal) {
-  check_input(x);
-  c10::cuda::CUDAGuard guard(x.device());
-  check_cuda(dout, x, "dout");
-  check_inner(dout, "dout");
-  TORCH_CHECK(dout.scalar_type() == x.scalar_type(), "dout must have x's dtype");
+  c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  assert_shapes(x.dim() == 3 && weight.dim() == 2 && dout.sizes() == x.sizes(), "x (batch, seqlen, channels), weight (channels, width), dout as x");
+  assert_shapes(is_3d(dfinal, x.size(0), weight.size(1) - 1, x.size(2)), "dfinal_states (batch, width - 1, channels)");
   ssd_short_conv_bwd_params_t p{};
   ConvHold h;
   fill_conv(p.conv, h, x, weight, bias, silu, initial_states, seq_idx);
+  check_cuda(dout, x, "dout");
+  check_inner(dout, "dout");
+  TORCH_CHECK(dout.scalar_type() == x.scalar_type(), "dout must have x's dtype");
   p.dout = dout.data_ptr();
   copy_strides(p.dout_stride, dout, {0, 1});
   Tensor fh;
@@ -306,6 +315,14 @@ struct ScanHold {
 void fill_scan(ssd_token_scan_params_t& p, ScanHold& h, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias, bool dt_softplus, double dt_min, double dt_max,
                const OptTensor& initial_states, const OptTensor& seq_idx) {
+  assert_shapes(x.dim() == 3 && B.dim() == 4 && dt.sizes() == x.sizes() && B.size(0) == x.size(0) && B.size(1) == x.size(1) && B.size(2) > 0 &&
+                    x.size(2) % B.size(2) == 0 && C.sizes() == B.sizes(),
+                "x and dt (batch, seqlen, channels), B and C (batch, seqlen, ngroups, dstate), ngroups dividing channels");
+  const int64_t d = x.size(2), n = B.size(3);
+  assert_shapes(A.dim() == 2 && A.size(0) == d && A.size(1) == n && is_1d(D, d) && is_like(z, x) && is_1d(dt_bias, d) &&
+                    is_3d(initial_states, x.size(0), d, n) && is_2d(seq_idx, x.size(0), x.size(1)),
+                "A (channels, dstate), D and dt_bias (channels,), z as x, initial_states (batch, channels, dstate), seq_idx (batch, seqlen)");
+  check_input(x);
   check_inner(x, "x");
   check_cuda(dt, x, "dt");
   check_inner(dt, "dt");
@@ -355,8 +372,7 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_scan_fwd(const Tensor& x,
                                                                 const OptTensor& dt_bias, bool dt_softplus, double dt_min, double dt_max,
                                                                 const OptTensor& initial_states, const OptTensor& seq_idx,
                                                                 bool for_backward) {
-  check_input(x);
-  c10::cuda::CUDAGuard guard(x.device());
+  c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
   ssd_token_scan_params_t p{};
   ScanHold h;
   fill_scan(p, h, x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, initial_states, seq_idx);
@@ -389,14 +405,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
     const Tensor& dout, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Tensor& ckpt,
     const OptTensor& out_x, const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias, bool dt_softplus, double dt_min,
     double dt_max, const OptTensor& initial_states, const OptTensor& seq_idx, const OptTensor& dfinal) {
-  check_input(x);
-  c10::cuda::CUDAGuard guard(x.device());
-  check_cuda(dout, x, "dout");
-  check_inner(dout, "dout");
-  TORCH_CHECK(dout.scalar_type() == x.scalar_type(), "dout must have x's dtype");
+  c10::cuda::OptionalCUDAGuard guard(x.is_cuda() ? c10::optional<c10::Device>(x.device()) : c10::nullopt);
+  assert_shapes(dout.sizes() == x.sizes() && out_x.has_value() == z.has_value() && is_like(out_x, x), "dout as x, out_x with z and as x");
+  assert_shapes(x.dim() == 3 && B.dim() == 4, "x (batch, seqlen, channels), B (batch, seqlen, ngroups, dstate)");
+  const int64_t blocks = (x.size(1) + SSD_TOKEN_SCAN_CHECKPOINT - 1) / SSD_TOKEN_SCAN_CHECKPOINT;
+  assert_shapes(ckpt.dim() == 4 && ckpt.size(0) == x.size(0) && ckpt.size(1) == blocks && ckpt.size(2) == x.size(2) && ckpt.size(3) == B.size(3) &&
+                    is_3d(dfinal, x.size(0), x.size(2), B.size(3)),
+                "checkpoints of the same forward call, dfinal_states (batch, channels, dstate)");
   ssd_token_scan_bwd_params_t p{};
   ScanHold h;
   fill_scan(p.scan, h, x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, initial_states, seq_idx);
+  check_cuda(dout, x, "dout");
+  check_inner(dout, "dout");
+  TORCH_CHECK(dout.scalar_type() == x.scalar_type(), "dout must have x's dtype");
   check_cuda(ckpt, x, "checkpoints");
   TORCH_CHECK(ckpt.scalar_type() == at::kFloat && ckpt.is_contiguous(), "the forward call's checkpoints must be fp32 and contiguous");
   p.scan.checkpoints = ckpt.data_ptr<float>();

@@ -6,19 +6,6 @@ The state of a sequence is its last width - 1 inputs, (width - 1, channels), old
 from .._ext import C as _C
 
 
-def _check(x, weight, bias, initial_states, seq_idx):
-    batch, seqlen, channels = x.shape
-    _, width = weight.shape
-    assert weight.shape == (channels, width)
-    if bias is not None:
-        assert bias.shape == (channels,)
-    if initial_states is not None:
-        assert initial_states.shape == (batch, width - 1, channels)
-    if seq_idx is not None:
-        assert seq_idx.shape == (batch, seqlen)
-    return batch, width, channels
-
-
 def _short_conv_fwd(x, weight, bias=None, apply_silu=True, initial_states=None, seq_idx=None, return_final_states=False):
     """x (batch, seqlen, channels) with contiguous channels (a column range of a wider buffer will do),
     weight (channels, width):
@@ -28,19 +15,15 @@ def _short_conv_fwd(x, weight, bias=None, apply_silu=True, initial_states=None, 
     Before the first position stand initial_states (batch, width - 1, channels) or zeros.  With seq_idx
     (batch, seqlen) a position sees only its own sequence; initial_states belong to sequence 0.
     Returns (out, final_states); final_states is None unless asked for."""
-    _check(x, weight, bias, initial_states, seq_idx)
-    return _C.short_conv_fwd(x, weight, bias, bool(apply_silu), initial_states, seq_idx, bool(return_final_states))
+    # the front end asserts the shapes
+    return _C.short_conv_fwd(x, weight, bias, apply_silu, initial_states, seq_idx, return_final_states)
 
 
 def _short_conv_bwd(dout, x, weight, bias=None, apply_silu=True, initial_states=None, seq_idx=None, dfinal_states=None):
     """Gradients of `_short_conv_fwd` from its inputs (nothing has to be kept).  Returns (dx, dweight, dbias,
     dinitial_states): x's dtype, except dweight and dbias in fp32; dbias and dinitial_states are None where
     bias and initial_states are.  The same inputs give the same bits."""
-    batch, width, channels = _check(x, weight, bias, initial_states, seq_idx)
-    assert dout.shape == x.shape
-    if dfinal_states is not None:
-        assert dfinal_states.shape == (batch, width - 1, channels)
-    return _C.short_conv_bwd(dout, x, weight, bias, bool(apply_silu), initial_states, seq_idx, dfinal_states)
+    return _C.short_conv_bwd(dout, x, weight, bias, apply_silu, initial_states, seq_idx, dfinal_states)
 
 
 def _short_conv_step(x, conv_state, weight, bias=None, apply_silu=True, state_indices=None):

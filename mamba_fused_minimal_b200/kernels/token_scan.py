@@ -5,27 +5,6 @@ state).  The reference has no counterpart."""
 from .._ext import C as _C
 
 
-def _check(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx):
-    batch, seqlen, channels = x.shape
-    _, _, ngroups, dstate = B.shape
-    assert channels % ngroups == 0
-    assert dt.shape == x.shape
-    assert A.shape == (channels, dstate)
-    assert B.shape == (batch, seqlen, ngroups, dstate)
-    assert C.shape == B.shape
-    if D is not None:
-        assert D.shape == (channels,)
-    if z is not None:
-        assert z.shape == x.shape
-    if dt_bias is not None:
-        assert dt_bias.shape == (channels,)
-    if initial_states is not None:
-        assert initial_states.shape == (batch, channels, dstate)
-    if seq_idx is not None:
-        assert seq_idx.shape == (batch, seqlen)
-    return batch, seqlen, channels, dstate
-
-
 def _token_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, dt_limit=(0.0, float("inf")),
                     initial_states=None, seq_idx=None, for_backward=False):
     """x, dt, z (batch, seqlen, channels), A (channels, dstate), B, C (batch, seqlen, ngroups, dstate), D and
@@ -39,9 +18,9 @@ def _token_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fa
 
     Returns (out, final_states, saved): final_states (batch, channels, dstate) fp32, and with for_backward
     what `_token_scan_bwd` needs, else None."""
-    _check(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx)
-    out, final, checkpoints, out_x = _C.token_scan_fwd(x, dt, A, B, C, D, z, dt_bias, bool(dt_softplus), float(dt_limit[0]),
-                                                       float(dt_limit[1]), initial_states, seq_idx, bool(for_backward))
+    # the front end asserts the shapes
+    out, final, checkpoints, out_x = _C.token_scan_fwd(x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_limit[0], dt_limit[1],
+                                                       initial_states, seq_idx, for_backward)
     return out, final, (checkpoints, out_x) if for_backward else None
 
 
@@ -50,17 +29,9 @@ def _token_scan_bwd(dout, x, dt, A, B, C, saved, D=None, z=None, dt_bias=None, d
     """Gradients of `_token_scan_fwd`, called with the same inputs and with what it saved.  Returns (dx, ddt, dA,
     dB, dC, dD, dz, ddt_bias, dinitial_states): dA, dD, ddt_bias and dinitial_states in fp32, the others in
     their input's dtype; None for what was not given.  The same inputs give the same bits."""
-    batch, seqlen, channels, dstate = _check(x, dt, A, B, C, D, z, dt_bias, initial_states, seq_idx)
     checkpoints, out_x = saved
-    assert dout.shape == x.shape
-    assert checkpoints.shape == (batch, (seqlen + 15) // 16, channels, dstate)
-    assert (out_x is not None) == (z is not None)
-    if z is not None:
-        assert out_x.shape == x.shape
-    if dfinal_states is not None:
-        assert dfinal_states.shape == (batch, channels, dstate)
-    return _C.token_scan_bwd(dout, x, dt, A, B, C, checkpoints, out_x, D, z, dt_bias, bool(dt_softplus), float(dt_limit[0]),
-                             float(dt_limit[1]), initial_states, seq_idx, dfinal_states)
+    return _C.token_scan_bwd(dout, x, dt, A, B, C, checkpoints, out_x, D, z, dt_bias, dt_softplus, dt_limit[0], dt_limit[1],
+                             initial_states, seq_idx, dfinal_states)
 
 
 def _token_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, dt_limit=(0.0, float("inf")),
