@@ -84,12 +84,19 @@ __global__ void __launch_bounds__(kStepThreads, 5) token_step_kernel(StepArgs ar
   int64_t at[U];
   float acc[U];
   const int mine0 = lane * VS < n ? lane * VS : 0;   // this lane's first components, clamped
+  // rows of one head, or heads of one row: kGroups rows further lies the same distance further, and one 64-bit
+  // product serves all; a row past the end reads the first one's values
+  const bool even = PER_HEAD || P == 1;
+  const int64_t s_step = kGroups * (PER_HEAD ? p.state_stride[2] : p.state_stride[1]), x_step = kGroups * (PER_HEAD ? p.x_stride[2] : p.x_stride[1]);
+  const int first = row_of(0), h0 = head_of(first), p0 = p_of(first);
+  const int64_t at0 = h0 * p.state_stride[1] + p0 * p.state_stride[2], x0 = h0 * p.x_stride[1] + p0 * p.x_stride[2];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int r = row_of(u), h = head_of(r), pp = p_of(r);
-    at[u] = h * p.state_stride[1] + pp * p.state_stride[2];
+    const bool there = r0 + u * kGroups < rows;
+    at[u] = even ? at0 + (there ? u * s_step : 0) : h * p.state_stride[1] + pp * p.state_stride[2];
     st[u] = *reinterpret_cast<const Pack<S, VS>*>(state + at[u] + mine0);
-    x[u] = xb[h * p.x_stride[1] + pp * p.x_stride[2]];
+    x[u] = xb[even ? x0 + (there ? u * x_step : 0) : h * p.x_stride[1] + pp * p.x_stride[2]];
     if (u < H) {
       dtr[u].load(p.dt, p.dt_dtype, b * p.dt_stride[0] + h * p.dt_stride[1]);
       if (p.dt_bias) br[u].load(p.dt_bias, p.bias_dtype, h * p.bias_stride);
