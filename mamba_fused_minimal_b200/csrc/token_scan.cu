@@ -8,10 +8,14 @@
 //
 // A block takes 16 channels and walks the positions in tiles of 32.  dt' is formed once per position and
 // channel and put beside dt' x in shared memory, B and C are copied there as they are.  What a lane reads
-// back per component and position has to pass the shared memory's 128 bytes a clock, broadcast or not:
-// with B and C widened in shared memory that was the bound (17 of 19 cycles per 32 updates and
-// scheduler), so 16-bit ones are widened in registers.  The multiply-adds work on pairs of components
-// (packed fp32), which halves their issue slots.
+// back per component and position has to pass the shared memory's 128 bytes a clock, broadcast or not,
+// so 16-bit ones are widened in registers (1 x 65537 x 320 channels: 398 to 352 us).  The multiply-adds work on
+// pairs of components (packed fp32), which halves their issue slots.
+//
+// The threads that hold the states do nothing else; two more warps load, form dt' and apply D and the gate, a
+// tile ahead and a tile behind (594 to 443 us at 2 x 4096 x 5120 channels of 16).  Measured there: 367 us,
+// against 186 us for its exponentials and 51 us for its bytes; issue slots, shared memory and exponentials are
+// each a little over half used, and 640 blocks on 148 SMs leave 14 % of them idle at the end.
 //
 // Few channels and a long sequence: the sequence is cut into segments that run side by side.  A first pass
 // leaves each segment's state from a zero start and the sum of its dt'; since the decay over a segment is

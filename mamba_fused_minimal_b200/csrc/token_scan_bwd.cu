@@ -11,6 +11,12 @@
 // is summed over components (g . B and the A term) is exchanged between the lanes of a channel; what is
 // summed over channels (dB, dC) is added up over the block's channels in shared memory and leaves as the
 // block's share, which a second kernel adds over the blocks in a fixed order.
+//
+// Few channels and a long sequence: segments side by side as in the forward pass; a first walk finds what each
+// hands to the one before it (18000 positions of 256 channels: 2063 to 356 us).
+//
+// Measured at 2 x 2048 x 5120 channels of 16, bf16: 880 us, bound by issue slots (62 %): about 50 instructions
+// for each position, channel and component, half of them the exchanges of the two kinds of sums.
 #include "token_scan.cuh"
 
 namespace ssd {

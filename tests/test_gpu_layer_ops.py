@@ -309,6 +309,24 @@ def test_conv_step(cuda_device, dtype, width, channels):
     assert torch.equal(st.cpu(), expect)
 
 
+def test_conv_step_slots_named_twice(cuda_device):
+    """The first row of a slot is served, later ones are padding; more rows than slots too."""
+    _, conv, _ = ops()
+    r = maker(14)
+    x, state, w = r(300, 24).to("cuda"), r(4, 3, 24).to("cuda"), r(24, 4).to("cuda")
+    idx = torch.tensor([1, 1, 3] + [-1] * 280 + [3, 0] + [1] * 14 + [2], dtype=torch.int32, device="cuda")
+    first = [0, 2, 284, 299]
+    alone = state.clone()
+    ref = conv._short_conv_step(x[first], alone, w, state_indices=idx[first])
+    out = conv._short_conv_step(x, state, w, state_indices=idx)
+    assert torch.equal(out[first], ref) and torch.equal(state, alone)
+    rest = [i for i in range(300) if i not in first]
+    assert (out[rest] == 0).all()
+    # without indices: rows past the slots are padding
+    out = conv._short_conv_step(x, state, w)
+    assert (out[4:] == 0).all() and (out[:4] != 0).any()
+
+
 # ---------------------------------------------------------------------------------------------- scan
 def scan_inputs(b, l, d, n, g, dtype, seed, dt_dtype=None):
     r = maker(seed)
