@@ -238,11 +238,11 @@ int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 // Threads and vectors per thread of a row of `nvec` vectors: `most` vectors per thread at most (the
 // registers they take); 0 vectors per thread where the row does not fit a block's registers.
-void row_shape(int nvec, int64_t rows, int most, int* threads, int* vpt) {
+void row_shape(int nvec, int64_t rows, int want, int most, int* threads, int* vpt) {
   int v = 1;
-  // few rows: one vector per thread, the shortest way through a row.  Many rows: blocks of about 256
+  // few rows: one vector per thread, the shortest way through a row.  Many rows: blocks of about `want`
   // threads, so that several rows are in flight on an SM and one row's sums hide behind another's loads.
-  const int want = rows >= 2 * 148 ? 256 : kMaxThreads;
+  if (rows < 2 * 148) want = kMaxThreads;
   while (v < most && (nvec + v - 1) / v > want) v *= 2;
   *vpt = v;
   *threads = round_up((nvec + v - 1) / v, 32);
@@ -255,7 +255,7 @@ void row_shape(int nvec, int64_t rows, int most, int* threads, int* vpt) {
 template <typename T, typename R, typename O, int V>
 int launch_norm_v(const NormArgs& a, int64_t rows, cudaStream_t stream) {
   int threads, vpt;
-  row_shape((a.dim + V - 1) / V, rows, V == 8 ? 4 : 8, &threads, &vpt);
+  row_shape((a.dim + V - 1) / V, rows, 256, V == 8 ? 4 : 8, &threads, &vpt);
   const unsigned grid = (unsigned)rows;
   switch (vpt) {
     case 1: add_rms_norm_kernel<T, R, O, V, 1><<<grid, threads, 0, stream>>>(a); break;
@@ -439,17 +439,19 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial
   if (threadIdx.x == 0 && c < dim) out[c] = v;
 }
 
-// Rows of `partial`: as many blocks as are resident at once, two an SM, and no more than there are rows.
-int bwd_parts(int64_t rows) {
-  const int64_t most = 2 * 148;
+// Rows of `partial`: as many blocks as are resident at once -- two an SM, up to eight of short rows, whose
+// blocks are small -- and no more than there are rows.
+int bwd_parts(int64_t rows, int dim) {
+  const int per_sm = dim >= 4096 ? 2 : dim <= 1024 ? 8 : 8192 / dim;
+  const int64_t most = per_sm * 148;
   return (int)(rows < most ? rows : most);
 }
 
 template <typename T, typename S, int V>
 int launch_norm_bwd_v(const NormBwdArgs& a, cudaStream_t stream) {
   int threads, vpt;
-  row_shape((a.dim + V - 1) / V, 0, V == 8 ? 2 : V == 1 ? 8 : 4, &threads, &vpt);
-  const int parts = bwd_parts(a.rows);
+  row_shape((a.dim + V - 1) / V, a.rows, V == 1 ? 128 : 512, V == 8 ? 2 : V == 1 ? 8 : 4, &threads, &vpt);
+  const int parts = bwd_parts(a.rows, a.dim);
   switch (vpt) {
     case 1:
       if (threads <= 512)
@@ -524,7 +526,7 @@ int launch_add_rms_norm(const ssd_add_rms_norm_params_t& p, cudaStream_t stream)
 }
 
 size_t add_rms_norm_bwd_workspace(const ssd_add_rms_norm_bwd_params_t& p) {
-  return (size_t)bwd_parts((int64_t)p.batch * p.seqlen) * p.dim * sizeof(float);
+  return (size_t)bwd_parts((int64_t)p.batch * p.seqlen, p.dim) * p.dim * sizeof(float);
 }
 
 int launch_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t& p, cudaStream_t stream) {
@@ -549,7 +551,7 @@ int launch_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t& p, cudaStream_t
     return p.total_dtype == SSD_F32 ? launch_norm_bwd<T, float>(a, p, stream) : launch_norm_bwd<T, T>(a, p, stream);
   });
   if (rc != SSD_OK) return rc;
-  sum_partials_kernel<<<(p.dim + 31) / 32, dim3(32, 32), 0, stream>>>(a.partial, p.dweight, bwd_parts(a.rows), p.dim);
+  sum_partials_kernel<<<(p.dim + 31) / 32, dim3(32, 32), 0, stream>>>(a.partial, p.dweight, bwd_parts(a.rows, p.dim), p.dim);
   SSD_CUDA_OK(cudaGetLastError());
   return SSD_OK;
 }

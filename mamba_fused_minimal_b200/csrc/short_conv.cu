@@ -16,9 +16,17 @@ namespace {
 
 constexpr int kConvThreads = 128;
 constexpr int kGroup = 8;         // positions whose loads are issued together, one group ahead of their use
-constexpr int kFwdStrip = 64;     // positions of a forward strip
-// positions of a gradient strip: with the width - 1 behind it a whole number of groups
-__host__ __device__ constexpr int bwd_strip(int width) { return 64 - (width - 1); }
+constexpr int kStrip = 64;        // most positions of a strip
+
+// Positions of a strip: 64, or fewer where the strips would leave most of the GPU idle (993 x 984 channels, 32
+// blocks of 64 positions: 20 us).  With the `halo` positions behind it that a gradient strip walks, too, it is a
+// whole number of groups.
+int strip_of(int batch, int seqlen, int channels, int halo) {
+  int n = kStrip;
+  const int64_t rows = (int64_t)batch * ((channels + 511) / 512);
+  while (n > kGroup && rows * ((seqlen + n - halo - 1) / (n - halo)) < 2 * 148) n /= 2;
+  return n - halo;
+}
 
 struct ConvArgs {
   const void* x;
@@ -29,7 +37,7 @@ struct ConvArgs {
   void* out;
   void* final_states;
   int weight_dtype, bias_dtype;
-  int seqlen, channels;
+  int seqlen, channels, strip;
   int silu;
   int64_t x_sb, x_sl, s_sb, s_sl;
 };
@@ -88,12 +96,15 @@ __device__ __forceinline__ void tap(const float (&wr)[W][V], const float (&bs)[V
 // Channels are contiguous, so a thread takes V of them; 8 bytes a load leave the registers for eight loads in
 // flight and the next eight behind them.  Every load is unconditional (the position is clamped to the strip):
 // one under a condition would be waited for at once.
-template <typename T, int W, int V, bool SEQ>
+// FULL: the strip is the longest, a constant (with its length read at run time the packed gradients took 72 us
+// instead of 66).
+template <typename T, int W, int V, bool SEQ, bool FULL>
 __global__ void __launch_bounds__(kConvThreads) short_conv_fwd_kernel(ConvArgs a) {
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
   const int b = blockIdx.z;
-  const int t0 = blockIdx.y * kFwdStrip, t1 = min(t0 + kFwdStrip, a.seqlen);
+  const int strip = FULL ? kStrip : a.strip;
+  const int t0 = blockIdx.y * strip, t1 = min(t0 + strip, a.seqlen);
   const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
   T* out = static_cast<T*>(a.out) + ((int64_t)b * a.seqlen) * a.channels + c;
   const int64_t sbase = SEQ ? b * a.s_sb : 0;
@@ -169,13 +180,14 @@ struct ConvBwdArgs {
 // A strip walks its positions and the width - 1 behind it (whose dpre its last dx need), in groups whose
 // loads are issued one group ahead; dx of a position is complete once dpre of the width - 1 positions after it
 // is known.
-template <typename T, int W, int V, bool SEQ>
+template <typename T, int W, int V, bool SEQ, bool FULL>
 __global__ void __launch_bounds__(kConvThreads, 5) short_conv_bwd_kernel(ConvBwdArgs g) {
   const ConvArgs& a = g.f;
   const int c = (blockIdx.x * kConvThreads + threadIdx.x) * V;
   if (c >= a.channels) return;
   const int b = blockIdx.z;
-  const int t0 = blockIdx.y * bwd_strip(W), t1 = min(t0 + bwd_strip(W), a.seqlen);
+  const int strip = FULL ? kStrip - (W - 1) : a.strip;
+  const int t0 = blockIdx.y * strip, t1 = min(t0 + strip, a.seqlen);
   const T* x = static_cast<const T*>(a.x) + b * a.x_sb + c;
   const T* dout = static_cast<const T*>(g.dout) + b * g.d_sb + c;
   T* dx = static_cast<T*>(g.dx) + ((int64_t)b * a.seqlen) * a.channels + c;
@@ -397,8 +409,9 @@ int strips_of(int seqlen, int strip) { return (seqlen + strip - 1) / strip; }
 }  // namespace
 
 int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream) {
-  const ConvArgs a = conv_args(p);
-  const int strips = strips_of(p.seqlen, kFwdStrip);
+  ConvArgs a = conv_args(p);
+  a.strip = strip_of(p.batch, p.seqlen, p.channels, 0);
+  const int strips = strips_of(p.seqlen, a.strip);
   SSD_REQUIRE(strips <= 65535 && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv: seqlen %d or batch %d too large", p.seqlen, p.batch);
   return with_type(p.x_dtype, [&](auto t) {
     using T = decltype(t);
@@ -411,7 +424,10 @@ int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream)
       const auto go = [&](auto v, auto s) -> int {
         constexpr int N = decltype(v)::value;
         const dim3 grid((p.channels + kConvThreads * N - 1) / (kConvThreads * N), strips, p.batch);
-        short_conv_fwd_kernel<T, W, N, decltype(s)::value><<<grid, kConvThreads, 0, stream>>>(a);
+        if (a.strip == kStrip)
+          short_conv_fwd_kernel<T, W, N, decltype(s)::value, true><<<grid, kConvThreads, 0, stream>>>(a);
+        else
+          short_conv_fwd_kernel<T, W, N, decltype(s)::value, false><<<grid, kConvThreads, 0, stream>>>(a);
         SSD_CUDA_OK(cudaGetLastError());
         return SSD_OK;
       };
@@ -424,7 +440,9 @@ int launch_short_conv_fwd(const ssd_short_conv_params_t& p, cudaStream_t stream)
 }
 
 size_t short_conv_bwd_workspace(const ssd_short_conv_bwd_params_t& p) {
-  return (size_t)p.conv.batch * strips_of(p.conv.seqlen, bwd_strip(p.conv.width)) * (p.conv.width + 1) * p.conv.channels * sizeof(float);
+  const ssd_short_conv_params_t& c = p.conv;
+  const int strips = strips_of(c.seqlen, strip_of(c.batch, c.seqlen, c.channels, c.width - 1));
+  return (size_t)c.batch * strips * (c.width + 1) * c.channels * sizeof(float);
 }
 
 int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& q, cudaStream_t stream) {
@@ -437,7 +455,8 @@ int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& q, cudaStream_t str
   g.dinit = q.dinitial_states;
   g.partial = static_cast<float*>(q.workspace);
   g.d_sb = q.dout_stride[0], g.d_sl = q.dout_stride[1];
-  const int strips = strips_of(p.seqlen, bwd_strip(p.width));
+  g.f.strip = strip_of(p.batch, p.seqlen, p.channels, p.width - 1);
+  const int strips = strips_of(p.seqlen, g.f.strip);
   SSD_REQUIRE(strips <= 65535 && p.batch <= 65535, SSD_ERR_UNSUPPORTED, "short conv: seqlen %d or batch %d too large", p.seqlen, p.batch);
   return with_type(p.x_dtype, [&](auto t) {
     using T = decltype(t);
@@ -451,7 +470,10 @@ int launch_short_conv_bwd(const ssd_short_conv_bwd_params_t& q, cudaStream_t str
       const auto go = [&](auto v, auto s) -> int {
         constexpr int N = decltype(v)::value;
         const dim3 grid((p.channels + kConvThreads * N - 1) / (kConvThreads * N), strips, p.batch);
-        short_conv_bwd_kernel<T, W, N, decltype(s)::value><<<grid, kConvThreads, 0, stream>>>(g);
+        if (g.f.strip == kStrip - (W - 1))
+          short_conv_bwd_kernel<T, W, N, decltype(s)::value, true><<<grid, kConvThreads, 0, stream>>>(g);
+        else
+          short_conv_bwd_kernel<T, W, N, decltype(s)::value, false><<<grid, kConvThreads, 0, stream>>>(g);
         SSD_CUDA_OK(cudaGetLastError());
         short_conv_sum_kernel<W><<<dim3((p.channels + 31) / 32, W + 1), dim3(32, 32), 0, stream>>>(g.partial, q.dweight, q.dbias,
                                                                                                     strips * p.batch, p.channels);

@@ -140,6 +140,23 @@ def test_norm_strided_rows(cuda_device):
         assert all(torch.equal(p, q) for p, q in zip(a[:2], b[:2]))
 
 
+@pytest.mark.parametrize("rows,dim", [(400, 64), (1300, 743), (700, 744), (310, 4097), (900, 2560)])
+def test_norm_gradients_of_many_rows(cuda_device, rows, dim):
+    """More rows than blocks: rows one after another in a block, and its share of the weight's gradient."""
+    bwd = ops()[0]._add_rms_norm_bwd
+    r = maker(rows)
+    total, w, dout = 2 * r(rows, dim, dtype=torch.bfloat16), 1 + 0.1 * r(dim), r(rows, dim, dtype=torch.bfloat16)
+    td, wd = total.double().requires_grad_(), w.double().requires_grad_()
+    (L.add_rms_norm(td, wd)[0] * dout.double()).sum().backward()
+    rstd = (1 / torch.sqrt((total.double() ** 2).mean(-1) + 1e-5)).float()
+    dx, _, dw = bwd(*cuda(dout, total, w, rstd))
+    size = td.grad.abs() + (dout.double() * wd).abs().detach() * rstd.double()[:, None]
+    within(dx, td.grad, size, (dim / 64 + 32) * U, torch.bfloat16)
+    terms = (dout.double() * td.detach() * rstd.double()[:, None]).abs().sum(0)
+    # at most rows / blocks terms one after another, the blocks' shares in strides of 32
+    within(dw, wd.grad, terms, (rows / 148 + 64) * U, torch.float32)
+
+
 @pytest.mark.parametrize("dim", [1, 33, 256, 4097, 9000, 16384, 20001])
 @pytest.mark.parametrize("dtype,stype", [(torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32)])
 def test_norm_gradients(cuda_device, dim, dtype, stype):
@@ -219,6 +236,30 @@ def test_conv_forward_and_gradients(cuda_device, dtype, case):
             continue
         assert g.dtype == t and torch.equal(g, g2), name
         assert norm_err(g, leaf.grad) <= 256 * U + half_step(t), name
+
+
+@pytest.mark.parametrize("dtype,channels,has_seq", [(torch.bfloat16, 2056, True), (torch.float32, 2056, False), (torch.float16, 2049, True)])
+def test_conv_long_strips_are_the_short_ones(cuda_device, dtype, channels, has_seq):
+    """A batch large enough for the longest strips gives each row the bits that the row gives alone, where it is
+    cut into short ones; the filters' gradients are the rows' sum (64 terms more or less one after another)."""
+    _, conv, _ = ops()
+    r = maker(90)
+    b, l = 16, 260
+    x, dout = r(b, l, channels, dtype=dtype).to("cuda"), r(b, l, channels, dtype=dtype).to("cuda")
+    w, bias, init = (0.5 * r(channels, 4)).to("cuda"), r(channels).to("cuda"), r(b, 3, channels, dtype=dtype).to("cuda")
+    seq = packed(b, l, 7).to("cuda") if has_seq else None
+    kw = lambda i: dict(bias=bias, initial_states=init[i], seq_idx=None if seq is None else seq[i])  # noqa: E731
+    every = slice(0, b)
+    out, fin = conv._short_conv_fwd(x, w, return_final_states=True, **kw(every))
+    dx, dw, db, di = conv._short_conv_bwd(dout, x, w, dfinal_states=init, **kw(every))
+    dws, dbs = 0, 0
+    for i in range(b):
+        one = slice(i, i + 1)
+        o1, f1 = conv._short_conv_fwd(x[one], w, return_final_states=True, **kw(one))
+        g = conv._short_conv_bwd(dout[one], x[one], w, dfinal_states=init[one], **kw(one))
+        assert torch.equal(out[one], o1) and torch.equal(fin[one], f1) and torch.equal(dx[one], g[0]) and torch.equal(di[one], g[3])
+        dws, dbs = dws + g[1].double(), dbs + g[2].double()
+    assert norm_err(dw, dws.cpu()) <= 64 * U and norm_err(db, dbs.cpu()) <= 64 * U
 
 
 def test_conv_in_pieces_is_the_whole(cuda_device):
