@@ -545,7 +545,7 @@ SSD_API int ssd_short_conv_step(const ssd_short_conv_step_params_t* prm, ssd_str
  *    h starts from initial_states or zero and stays fp32.  With seq_idx the state is dropped where
  *    the sequence changes; initial_states belong to sequence 0.
  *    For a later ssd_token_scan_bwd give `checkpoints` (the states before positions 0, 16, 32, ...)
- *    and, with z, `out_x` (y before the gate).
+ *    and, with z, `out_x` (y before the gate, in fp32: dz is made of it and rounded once).
  *    x, dt, z with contiguous channels, B and C with contiguous state components; dt_dtype is x_dtype
  *    or SSD_F32; dstate at most 256; every output contiguous.
  *    workspace: 16-byte aligned, at least ssd_token_scan_workspace_bytes() bytes (may be 0), any
@@ -564,7 +564,7 @@ typedef struct {
   const void* initial_states; /* (b, d, n) of init_dtype, contiguous, or NULL */
   const int32_t* seq_idx;    /* (b, l) or NULL */
   void* out;                 /* (b, l, d) of x_dtype */
-  void* out_x;               /* (b, l, d) of x_dtype, or NULL */
+  float* out_x;              /* (b, l, d), or NULL: y before the gate */
   float* final_states;       /* (b, d, n) */
   float* checkpoints;        /* (b, ceil(l / SSD_TOKEN_SCAN_CHECKPOINT), d, n), or NULL */
   int32_t x_dtype, dt_dtype, A_dtype, D_dtype, bias_dtype, init_dtype;

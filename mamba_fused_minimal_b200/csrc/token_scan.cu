@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
 #pragma unroll
         for (int e = 0; e < EV; e += 2) unpack2(fma2(dv[e / 2], pair_of(xk, e / 2), pack2(o[e], o[e + 1])), o[e], o[e + 1]);
         if (a.z) {
-          if (a.out_x) store_some<EV, VEC>(static_cast<T*>(a.out_x) + at, o, count);
+          if (a.out_x) store_some<EV, VEC>(a.out_x + at, o, count);
 #pragma unroll
           for (int e = 0; e < EV; e += 2) unpack2(mul2(pack2(o[e], o[e + 1]), silu2(pair_of(zk, e / 2))), o[e], o[e + 1]);
         }
@@ -516,7 +516,7 @@ int launch_plan(const ScanArgs& a, const ssd_token_scan_params_t& p, cudaStream_
   const int ds = dtype_size(p.dt_dtype);
   const size_t dt_most = EV * ds < 16 ? EV * ds : 16;
   const bool vec = a.per_group % EV == 0 && rows_aligned(p.x, p.x_stride, 2, sizeof(T), kMost) && rows_aligned(p.dt, p.dt_stride, 2, ds, dt_most) &&
-                   (p.z == nullptr || rows_aligned(p.z, p.z_stride, 2, sizeof(T), kMost)) && aligned_to(p.out, kMost) && aligned_to(p.out_x, kMost) &&
+                   (p.z == nullptr || rows_aligned(p.z, p.z_stride, 2, sizeof(T), kMost)) && aligned_to(p.out, kMost) && aligned_to(p.out_x, 16) &&
                    p.dstate % CB == 0 && rows_aligned(p.B, p.B_stride, 3, sizeof(T), CB * sizeof(T)) &&
                    rows_aligned(p.C, p.C_stride, 3, sizeof(T), CB * sizeof(T));
   return vec ? launch_vec<T, LPC, NS, K, true>(a, p.batch, stream) : launch_vec<T, LPC, NS, K, false>(a, p.batch, stream);

@@ -17,7 +17,7 @@ struct ScanArgs {
   const void* init;
   const int32_t* seq;
   void* out;
-  void* out_x;
+  float* out_x;          // y before the gate, which dz is made of: in 32 bits, so that dz is rounded once
   float* final_states;
   float* ckpt;
   float* seg_state;      // (b, segments, d, n): the state a segment leaves from a zero start

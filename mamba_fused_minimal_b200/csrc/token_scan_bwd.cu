@@ -40,7 +40,7 @@ struct ScanBwdArgs {
   float* part_D;       // (b, segments, d)
   float* part_bias;    // (b, segments, d)
   int64_t d_sb, d_sl;
-  int unit, unit32, unit_bc, unit_ck;   // bytes copied at a time of x and the like, of an fp32 dt, of B and C, of the states
+  int unit, unit32, unit_y, unit_bc, unit_ck;   // bytes copied at a time of x and the like, of an fp32 dt, of out_x, of B and C, of the states
 };
 
 template <typename T, int NP>
@@ -52,9 +52,10 @@ struct BwdShape {
   static constexpr int kPer = kItems > kBwdThreads ? kItems / kBwdThreads : 1;
   static constexpr int kBc = 2 * kT * NP;
   static constexpr int kPerBc = kBc > kBwdThreads ? kBc / kBwdThreads : 1;
-  // a tile as it lies in memory: x, dout, z, out_x (kItems elements each), B and C (kT rows of dstate), dt and
-  // the states before the tile (in 4 bytes)
-  static constexpr int kRaw16 = 4 * kItems + 2 * kT * NP, kRaw32 = kItems + kBwdThreads;
+  // a tile as it lies in memory: x, dout, z (kItems elements each), B and C (kT rows of dstate), then dt, out_x
+  // and the states before the tile (in 4 bytes)
+  static constexpr int kBcAt = 3 * kItems, kRaw16 = kBcAt + 2 * kT * NP;
+  static constexpr int kYAt = kItems, kStateAt = 2 * kItems, kRaw32 = kStateAt + kBwdThreads;
   static constexpr size_t kRaw = (kRaw16 * sizeof(T) + kRaw32 * 4 + 15) / 16 * 16;
   static constexpr size_t kSmem = 2 * kRaw + sizeof(float) * ((3 * kChannels + 2 * NP) * kPitch + 2 * kChannels * kSlabs * kPitch + kBwdWarps * kT * kRow);
 };
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   // and so waited for at once).  A warp copies one tensor.
   const auto fetch = [&](int t0, int buf) {
     char* const raw = s_raw + buf * Sh::kRaw;
-    constexpr int kOne = Sh::kItems * ES, kBC = kT * NP * ES;
+    constexpr int kOne = Sh::kItems * ES, kBC = kT * NP * ES, k32 = Sh::kRaw16 * ES;
     const int tail = a.seqlen - 1 - t0;
     const int64_t row = (int64_t)b * a.seqlen + t0;
     const auto rows = [&](int at, const void* base, int64_t off, int64_t sl) {
@@ -138,21 +139,23 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
         if (a.z) rows(2 * kOne, a.z, b * a.z_sb, a.z_sl);
         break;
       case 3:
-        if (a.z && !CARRY) rows(3 * kOne, a.out_x, (row - t0) * a.channels, a.channels);
+        if (a.z && !CARRY)
+          copy_rows<CH * 4>(raw + k32 + Sh::kYAt * 4, reinterpret_cast<const char*>(a.out_x + row * a.channels + c0), (int64_t)a.channels * 4, kT, tail,
+                            nch * 4, q.unit_y, 4, lane);
         break;
       case 4:
         if (a.dt_f32)
-          copy_rows<CH * 4>(raw + 4 * kOne + 2 * kBC, static_cast<const char*>(a.dt) + (b * a.dt_sb + (int64_t)t0 * a.dt_sl + c0) * 4, a.dt_sl * 4, kT, tail,
+          copy_rows<CH * 4>(raw + k32, static_cast<const char*>(a.dt) + (b * a.dt_sb + (int64_t)t0 * a.dt_sl + c0) * 4, a.dt_sl * 4, kT, tail,
                             nch * 4, q.unit32, 4, lane);
         else
-          rows(4 * kOne + 2 * kBC, a.dt, b * a.dt_sb, a.dt_sl);
+          rows(k32, a.dt, b * a.dt_sb, a.dt_sl);
         break;
       case 5:
-        if (!CARRY) states(4 * kOne, a.B, b * a.B_sb + grp * a.B_sg, a.B_sl);
+        if (!CARRY) states(Sh::kBcAt * ES, a.B, b * a.B_sb + grp * a.B_sg, a.B_sl);
         break;
-      case 6: states(4 * kOne + kBC, a.C, b * a.C_sb + grp * a.C_sg, a.C_sl); break;
+      case 6: states(Sh::kBcAt * ES + kBC, a.C, b * a.C_sb + grp * a.C_sg, a.C_sl); break;
       default:
-        if (!CARRY) copy_rows<NP * 4>(raw + Sh::kRaw16 * ES + Sh::kItems * 4,
+        if (!CARRY) copy_rows<NP * 4>(raw + k32 + Sh::kStateAt * 4,
                           reinterpret_cast<const char*>(a.ckpt + (((int64_t)b * tiles + t0 / kT) * a.channels + c0) * a.dstate), (int64_t)a.dstate * 4, nch,
                           nch, a.dstate * 4, q.unit_ck, 4, lane);
     }
@@ -233,8 +236,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
       dy[e] = in ? widen(raw[Sh::kItems + item]) : 0.0f;
       if (a.z) {
         const float zv = widen(raw[2 * Sh::kItems + item]), s = sigmoid_f(zv);
-        if (in && !CARRY) static_cast<T*>(q.dz)[own + (int64_t)t * a.channels + c] = 
-            narrow<T>(dy[e] * widen(raw[3 * Sh::kItems + item]) * (s * (1.0f + zv * (1.0f - s))));
+        if (in && !CARRY) static_cast<T*>(q.dz)[own + (int64_t)t * a.channels + c] = narrow<T>(dy[e] * raw32[Sh::kYAt + item] * (s * (1.0f + zv * (1.0f - s))));
         dy[e] = in ? dy[e] * (zv * s) : 0.0f;
       }
       if (mine) {
@@ -249,9 +251,9 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
     for (int k = 0; k < NBC; ++k) {
       const bool is_b = k < kHalf && !second;
       const int t = bt + k % kHalf * kBcStep;
-      (is_b ? s_B : s_C)[bn * kPitch + t] = bin ? widen(raw[4 * Sh::kItems + (is_b ? t : kT + t) * NP + bn]) : 0.0f;
+      (is_b ? s_B : s_C)[bn * kPitch + t] = bin ? widen(raw[Sh::kBcAt + (is_b ? t : kT + t) * NP + bn]) : 0.0f;
     }
-    float h = has ? raw32[Sh::kItems + ch * NP + n] : 0.0f;
+    float h = has ? raw32[Sh::kStateAt + ch * NP + n] : 0.0f;
     const uint32_t resets = a.seq ? reset_mask(a, b, t0, lane) : 0u;
     __syncthreads();
     if (t0 > t_lo) fetch(t0 - kT, buf ^ 1);
@@ -546,8 +548,9 @@ int launch_bwd(ScanBwdArgs& q, int batch, cudaStream_t stream) {
   // a block's channels begin at a multiple of its own within the group, and its last block ends with it
   const int64_t ch = Sh::kChannels * es, pg = (int64_t)a.per_group * es;
   q.unit = copy_unit(ch, pg, at(a.x), a.x_sb * es, a.x_sl * es, at(q.dout), q.d_sb * es, q.d_sl * es, at(a.z), a.z ? a.z_sb * es : 0, a.z ? a.z_sl * es : 0,
-                     at(a.out_x), a.channels * es, a.dt_f32 ? 0 : at(a.dt), a.dt_f32 ? 0 : a.dt_sb * es, a.dt_f32 ? 0 : a.dt_sl * es);
+                     a.dt_f32 ? 0 : at(a.dt), a.dt_f32 ? 0 : a.dt_sb * es, a.dt_f32 ? 0 : a.dt_sl * es);
   q.unit32 = copy_unit(Sh::kChannels * 4, (int64_t)a.per_group * 4, at(a.dt), a.dt_sb * 4, a.dt_sl * 4);
+  q.unit_y = copy_unit(Sh::kChannels * 4, (int64_t)a.per_group * 4, at(a.out_x), (int64_t)a.channels * 4);
   q.unit_bc = copy_unit(a.dstate * es, at(a.B), a.B_sb * es, a.B_sl * es, a.B_sg * es, at(a.C), a.C_sb * es, a.C_sl * es, a.C_sg * es);
   q.unit_ck = copy_unit(a.dstate * 4, at(a.ckpt));
   if (smem > 48 * 1024)

@@ -387,8 +387,8 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_scan_fwd(const Tensor& x,
     ckpt = alloc_out({b, (l + SSD_TOKEN_SCAN_CHECKPOINT - 1) / SSD_TOKEN_SCAN_CHECKPOINT, d, n}, f32);
     p.checkpoints = ckpt->data_ptr<float>();
     if (z.has_value()) {
-      out_x = alloc_out(x.sizes(), x.options());
-      p.out_x = out_x->data_ptr();
+      out_x = alloc_out(x.sizes(), f32);
+      p.out_x = out_x->data_ptr<float>();
     }
   }
   p.workspace_bytes = ssd_token_scan_workspace_bytes(&p);
@@ -422,10 +422,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
   TORCH_CHECK(ckpt.scalar_type() == at::kFloat && ckpt.is_contiguous(), "the forward call's checkpoints must be fp32 and contiguous");
   p.scan.checkpoints = ckpt.data_ptr<float>();
   if (z.has_value()) {
-    TORCH_CHECK(out_x.has_value() && out_x->scalar_type() == x.scalar_type() && out_x->is_contiguous(),
-                "with z the forward call's output before the gate is needed");
+    TORCH_CHECK(out_x.has_value() && out_x->scalar_type() == at::kFloat && out_x->is_contiguous(),
+                "with z the forward call's output before the gate is needed, fp32 and contiguous");
     check_cuda(*out_x, x, "out_x");
-    p.scan.out_x = out_x->data_ptr();
+    p.scan.out_x = out_x->data_ptr<float>();
   }
   p.dout = dout.data_ptr();
   copy_strides(p.dout_stride, dout, {0, 1});

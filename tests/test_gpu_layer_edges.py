@@ -1,0 +1,36 @@
+"""The operators around the scan where their arithmetic has an edge: what a rounding is made of, infinities behind
+a border, values near the smallest number, parameters in 16 bits, scratch that is used again and again.
+
+Tolerances as in test_gpu_layer_ops.py, fixed before the first run; what differs is derived at the test."""
+import math
+
+import pytest
+import torch
+
+from oracle import layer_oracle as L
+from test_gpu_layer_ops import TYPES, U, cuda, half_step, maker, norm_err, ops, packed, scan_inputs, within
+
+pytestmark = pytest.mark.gpu
+
+KEYS = ("x", "dt", "A", "B", "C")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,l,d,n,g", [(2, 20, 48, 16, 1), (1, 17, 7, 5, 1), (1, 20, 24, 64, 2), (1, 20, 33, 8, 1), (1, 12, 9, 256, 1)])
+def test_gate_gradient_is_rounded_once(cuda_device, dtype, b, l, d, n, g):
+    """dz = dout y silu'(z) element by element: y may be off by what 66 u a position allows, the gate's derivative
+    by 80 u of its terms' absolute values, and one rounding of the result stands on top."""
+    scan = ops()[2]
+    inp = scan_inputs(b, l, d, n, g, dtype, 70 + l)
+    pos = [inp[k] for k in KEYS]
+    _, _, y, size = L.token_scan(*pos, D=inp["D"], z=inp["z"], dt_bias=inp["dt_bias"], dt_softplus=True)
+    dout = maker(71)(b, l, d, dtype=dtype)
+    z = inp["z"].double()
+    s = torch.sigmoid(z)
+    ref = dout.double() * y * s * (1 + z * (1 - s))
+    terms = (dout.double() * s * (1 + z.abs() * (1 - s))).abs()
+    dpos = cuda(*pos)
+    kw = {k: inp[k].to("cuda") for k in ("D", "z", "dt_bias")}
+    _, _, saved = scan._token_scan_fwd(*dpos, dt_softplus=True, for_backward=True, **kw)
+    dz = scan._token_scan_bwd(dout.to("cuda"), *dpos, saved, dt_softplus=True, **kw)[6]
+    within(dz, ref, size * terms, (66 * l + 80) * U, dtype)
