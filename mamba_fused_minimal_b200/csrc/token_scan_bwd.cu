@@ -317,9 +317,11 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
           float from[2], e[2], g[2], vB[2], vC[2];
           unpack2(mul2(CC, yy), from[0], from[1]);
           unpack2(dec[t / 2 + i], e[0], e[1]);
+          // a position that begins a sequence hands nothing on: selected, since what it holds may not be finite
+          const int first = RESET ? (int)(resets >> (t + 2 * i)) : 0;
           g[1] = from[1] + carry;
-          g[0] = fmaf(g[1], e[1], from[0]);
-          carry = g[0] * e[0];
+          g[0] = first & 2 ? from[0] : fmaf(g[1], e[1], from[0]);
+          carry = first & 1 ? 0.0f : g[0] * e[0];
           const f32x2 gg = pack2(g[0], g[1]);
           const f32x2 m = mul2(gg, kept[t / 2 + i]);
           unpack2(mul2(yy, fma2(uu, BB, kept[t / 2 + i])), vC[0], vC[1]);

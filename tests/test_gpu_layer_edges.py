@@ -34,3 +34,37 @@ def test_gate_gradient_is_rounded_once(cuda_device, dtype, b, l, d, n, g):
     _, _, saved = scan._token_scan_fwd(*dpos, dt_softplus=True, for_backward=True, **kw)
     dz = scan._token_scan_bwd(dout.to("cuda"), *dpos, saved, dt_softplus=True, **kw)[6]
     within(dz, ref, size * terms, (66 * l + 80) * U, dtype)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("where", ["dout", "C", "z", "dt", "dfinal"])
+@pytest.mark.parametrize("b,l,d,n,cuts", [(2, 61, 20, 16, (22, 45)), (1, 61, 9, 64, (33, 34)), (1, 1700, 24, 16, (301, 1600)), (1, 1700, 24, 8, (512, 1111))])
+def test_gradients_of_a_sequence_see_no_later_one(cuda_device, bad, where, b, l, d, n, cuts):
+    """Packed sequences: an infinity or a NaN of the last one leaves the bits of the others' gradients, for rows
+    that one block walks and rows that are cut into segments, with borders at even and odd positions."""
+    scan = ops()[2]
+    inp = {k: v.to("cuda") for k, v in scan_inputs(b, l, d, n, 1, torch.float32, 72).items()}
+    seq = torch.zeros(b, l, dtype=torch.int32, device="cuda")
+    for c in cuts:
+        seq[:, c:] += 1
+    r = maker(73)
+    inp |= dict(dout=r(b, l, d).to("cuda"), dfinal=r(b, d, n).to("cuda"), init=r(b, d, n).to("cuda"))
+
+    def grads(v):
+        kw = dict(D=v["D"], z=v["z"], dt_bias=v["dt_bias"], dt_softplus=True, initial_states=v["init"], seq_idx=seq)
+        pos = [v[k] for k in KEYS]
+        _, _, saved = scan._token_scan_fwd(*pos, for_backward=True, **kw)
+        return scan._token_scan_bwd(v["dout"], *pos, saved, dfinal_states=v["dfinal"], **kw)
+
+    poisoned = dict(inp)
+    poisoned[where] = inp[where].clone()
+    if where == "dfinal":
+        poisoned[where][:, :, n // 2] = bad
+    else:
+        poisoned[where][:, cuts[-1]:cuts[-1] + 3] = bad
+        poisoned[where][:, -1] = bad
+    good, got = grads(inp), grads(poisoned)
+    names = ("dx", "ddt", "dA", "dB", "dC", "dD", "dz", "ddt_bias", "dinitial")
+    for i in (0, 1, 3, 4, 6):
+        assert torch.isfinite(good[i]).all() and torch.equal(got[i][:, :cuts[-1]], good[i][:, :cuts[-1]]), names[i]
+    assert torch.equal(got[8], good[8]) and torch.isfinite(good[8]).all()
