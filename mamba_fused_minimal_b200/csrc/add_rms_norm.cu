@@ -27,6 +27,11 @@ struct NormArgs {
   float eps;
 };
 
+// Rows whose largest |y| lies below kTiny are multiplied by kLift, and their scale too, before codes are made of
+// them: both are powers of two, so nothing is rounded by it.  Lifted values lie between 2^-49 and 2^40.
+constexpr float kTiny = 0x1p-60f;
+constexpr float kLift = 0x1p100f;
+
 // What an output element is made of: y for the input's types, y / scale for the 8-bit types.
 struct I8 {};
 struct E4M3 {};
@@ -34,7 +39,9 @@ template <typename O> struct OutKind { static constexpr float kMost = 0.0f; };
 template <> struct OutKind<I8> { static constexpr float kMost = 127.0f; };
 template <> struct OutKind<E4M3> { static constexpr float kMost = 448.0f; };
 
-// y / scale, rounded as a division rounds: the product with the reciprocal, and what it left over
+// y / scale, rounded as a division rounds: the product with the reciprocal, corrected by what it left over, which a
+// fused multiply-add finds exactly (Markstein, IBM Journal of Research and Development 34, 1990).  That holds while
+// neither the reciprocal nor what is left over leaves fp32's range: smaller rows are lifted first, see kTiny.
 template <int V>
 __device__ __forceinline__ void quotients(const float (&y)[V], float scale, float inv, float (&q)[V]) {
   float left[V], iv[V], sc[V];
@@ -216,19 +223,31 @@ __global__ void __launch_bounds__(kMaxThreads) add_rms_norm_kernel(NormArgs a) {
     // an infinite y has no scale either: infinity becomes the NaN that marks such a row
     const float scale = most <= 3.4028235e38f ? most / OutKind<O>::kMost : __int_as_float(0x7fc00000);
     if (threadIdx.x == 0) a.scales[row] = scale;
-    // zero for a row of zeros; finite for the smallest rows
-    const float inv = most > 0.0f ? fminf(OutKind<O>::kMost / most, 1e38f) : 0.0f;
+    // the same for every thread of the block
+    const bool tiny = most < kTiny;
+    const float scale_up = tiny ? scale * kLift : scale;
+    // zero for a row of zeros (and one so small that its scale is zero)
+    const float inv = tiny ? (scale > 0.0f ? 1.0f / scale_up : 0.0f) : OutKind<O>::kMost / most;
+    const auto lift = [&](float (&v)[V]) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] *= kLift;
+    };
     if (kHold) {
+      if (tiny) {
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) lift(t[k]);
+      }
 #pragma unroll
       for (int k = 0; k < VPT; ++k) {
         const int col = (k * blockDim.x + threadIdx.x) * V;
-        if (col < a.dim) store_out<O, V>(a.out, obase + col, t[k], scale, inv);
+        if (col < a.dim) store_out<O, V>(a.out, obase + col, t[k], scale_up, inv);
       }
     } else {
       for (int col = threadIdx.x * V; col < a.dim; col += blockDim.x * V) {
         fetch(col, t[0]);
         finish(col, t[0], false);
-        store_out<O, V>(a.out, obase + col, t[0], scale, inv);
+        if (tiny) lift(t[0]);
+        store_out<O, V>(a.out, obase + col, t[0], scale_up, inv);
       }
     }
   }

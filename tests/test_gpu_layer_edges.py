@@ -68,3 +68,37 @@ def test_gradients_of_a_sequence_see_no_later_one(cuda_device, bad, where, b, l,
     for i in (0, 1, 3, 4, 6):
         assert torch.isfinite(good[i]).all() and torch.equal(got[i][:, :cuts[-1]], good[i][:, :cuts[-1]]), names[i]
     assert torch.equal(got[8], good[8]) and torch.isfinite(good[8]).all()
+
+
+@pytest.mark.parametrize("dim", [96, 97, 2560, 33024])
+@pytest.mark.parametrize("kind,most", [(torch.int8, 127.0), (torch.float8_e4m3fn, 448.0)])
+@pytest.mark.parametrize("dtype", TYPES[:2])
+def test_norm_in_8_bits_of_tiny_rows(cuda_device, dim, kind, most, dtype):
+    """Rows whose largest |y| lies between 1 and the smallest numbers, through small weights and through small rows
+    under eps: what the codes stand for.  On top of test_norm_forward's bound half a unit of the smallest numbers,
+    2^-150, for y itself and, |code| times, for the scale that is kept."""
+    fwd = ops()[0]._add_rms_norm_fwd
+    x = maker(74)(12, dim)
+    x[1], x[2], x[11] = 0, x[2] * 1e15, x[11] * 1e-15
+    for i, p in enumerate((8, 20, 30, 33, 35, 36, 37)):
+        x[3 + i] *= 10.0 ** -p
+    x = x.to(dtype)
+    tol = (dim / 64 + 16) * U
+    for power in (0, 12, 20, 30, 34, 35, 36, 37):
+        w = (1 + 0.1 * maker(75)(dim)) * 10.0 ** -power
+        y, _ = L.add_rms_norm(x, w)
+        q, _, _, sc = fwd(*cuda(x, w), out_dtype=kind)
+        q, sc = q.cpu().float().double(), sc.cpu().double()
+        assert torch.isfinite(q).all() and torch.isfinite(sc).all()
+        assert (q[1] == 0).all() and sc[1] == 0
+        ref_sc = y.abs().amax(-1) / most
+        assert ((sc - ref_sc).abs() <= (tol + 2 * U) * ref_sc + 2.0 ** -149).all()
+        rows = ref_sc >= 2.0 ** -135                   # below it the scale itself has lost its digits
+        step = ref_sc[:, None] * 0.5 if kind is torch.int8 else torch.maximum(y.abs() * 2.0 ** -4, ref_sc[:, None] * 2.0 ** -10)
+        bound = step * (1 + 1e-5) + (tol + 4 * U) * y.abs() * 17 + (q.abs() + 1) * 2.0 ** -149
+        # a scale of so few digits may round down: the largest codes end at `most`
+        bound = bound + (2.0 ** -149 / ref_sc.clamp_min(2.0 ** -149))[:, None] * y.abs()
+        bad = ((q * sc[:, None] - y).abs() > bound)[rows]
+        assert not bad.any(), (power, bad.any(-1).nonzero().flatten().tolist())
+        top = q.abs().amax(-1)
+        assert (top[rows & (ref_sc > 0)] == most).all(), (power, top.tolist())
