@@ -70,11 +70,22 @@ int check_workspace(const void* workspace, size_t bytes, size_t need) {
   return SSD_OK;
 }
 
+// what a workspace query needs to be true of its struct, too
+int check_conv_sizes(const ssd_short_conv_params_t& p) {
+  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.channels > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE(p.width >= 2 && p.width <= 4, SSD_ERR_UNSUPPORTED, "short conv: width %d is not 2, 3 or 4", p.width);
+  return SSD_OK;
+}
+
 int check_conv(const ssd_short_conv_params_t& p) {
   SSD_REQUIRE(p.x && p.weight, SSD_ERR_BAD_ARGUMENT, "x and weight must not be NULL");
   SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype) && absent_or_valid(p.bias, p.bias_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
-  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.channels > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
-  SSD_REQUIRE(p.width >= 2 && p.width <= 4, SSD_ERR_UNSUPPORTED, "short conv: width %d is not 2, 3 or 4", p.width);
+  return check_conv_sizes(p);
+}
+
+int check_norm_sizes(int32_t batch, int32_t seqlen, int32_t dim) {
+  SSD_REQUIRE(batch > 0 && seqlen > 0 && dim > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
+  SSD_REQUIRE((int64_t)batch * seqlen <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   return SSD_OK;
 }
 
@@ -422,13 +433,13 @@ int ssd_add_rms_norm_fwd(const ssd_add_rms_norm_params_t* prm, ssd_stream_t stre
               "out must have x's dtype, int8 or e4m3");
   SSD_REQUIRE(p.out_dtype == p.x_dtype ? p.rstd != nullptr : p.scales != nullptr, SSD_ERR_BAD_ARGUMENT,
               "rstd must not be NULL, nor scales with an 8-bit out");
-  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.dim > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
-  SSD_REQUIRE((int64_t)p.batch * p.seqlen <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
+  const int rc = check_norm_sizes(p.batch, p.seqlen, p.dim);
+  if (rc != SSD_OK) return rc;
   return launch_add_rms_norm(p, reinterpret_cast<cudaStream_t>(stream));
 }
 
 size_t ssd_add_rms_norm_bwd_workspace_bytes(const ssd_add_rms_norm_bwd_params_t* prm) {
-  return prm == nullptr ? 0 : add_rms_norm_bwd_workspace(*prm);
+  return prm == nullptr || check_norm_sizes(prm->batch, prm->seqlen, prm->dim) != SSD_OK ? 0 : add_rms_norm_bwd_workspace(*prm);
 }
 
 int ssd_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t* prm, ssd_stream_t stream) {
@@ -439,9 +450,9 @@ int ssd_add_rms_norm_bwd(const ssd_add_rms_norm_bwd_params_t* prm, ssd_stream_t 
               "dout, total, weight, rstd, dx and dweight must not be NULL");
   SSD_REQUIRE(valid_dtype(p.x_dtype) && valid_dtype(p.weight_dtype), SSD_ERR_BAD_ARGUMENT, "bad dtype");
   SSD_REQUIRE(p.total_dtype == p.x_dtype || p.total_dtype == SSD_F32, SSD_ERR_UNSUPPORTED, "total must have x's dtype or be fp32");
-  SSD_REQUIRE(p.batch > 0 && p.seqlen > 0 && p.dim > 0, SSD_ERR_BAD_ARGUMENT, "sizes must be positive");
-  SSD_REQUIRE((int64_t)p.batch * p.seqlen <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
-  const int rc = check_workspace(p.workspace, p.workspace_bytes, add_rms_norm_bwd_workspace(p));
+  int rc = check_norm_sizes(p.batch, p.seqlen, p.dim);
+  if (rc != SSD_OK) return rc;
+  rc = check_workspace(p.workspace, p.workspace_bytes, add_rms_norm_bwd_workspace(p));
   if (rc != SSD_OK) return rc;
   return launch_add_rms_norm_bwd(p, reinterpret_cast<cudaStream_t>(stream));
 }
@@ -456,7 +467,7 @@ int ssd_short_conv_fwd(const ssd_short_conv_params_t* prm, ssd_stream_t stream) 
 }
 
 size_t ssd_short_conv_bwd_workspace_bytes(const ssd_short_conv_bwd_params_t* prm) {
-  return prm == nullptr ? 0 : short_conv_bwd_workspace(*prm);
+  return prm == nullptr || check_conv_sizes(prm->conv) != SSD_OK ? 0 : short_conv_bwd_workspace(*prm);
 }
 
 int ssd_short_conv_bwd(const ssd_short_conv_bwd_params_t* prm, ssd_stream_t stream) {

@@ -102,3 +102,11 @@ def test_norm_in_8_bits_of_tiny_rows(cuda_device, dim, kind, most, dtype):
         assert not bad.any(), (power, bad.any(-1).nonzero().flatten().tolist())
         top = q.abs().amax(-1)
         assert (top[rows & (ref_sc > 0)] == most).all(), (power, top.tolist())
+
+
+def test_conv_gradients_refuse_wide_filters(cuda_device):
+    _, conv, _ = ops()
+    for width in (1, 5, 9, 17):
+        x, w = torch.zeros(2, 40, 64, device="cuda"), torch.zeros(64, width, device="cuda")
+        with pytest.raises(RuntimeError, match="not 2, 3 or 4"):
+            conv._short_conv_bwd(x, x, w)
