@@ -583,7 +583,10 @@ SSD_API int ssd_token_scan_fwd(const ssd_token_scan_params_t* prm, ssd_stream_t 
 
 /*    Gradients of the scan.  `scan` holds the forward call's inputs with its checkpoints and out_x
  *    (now inputs); scan.out, scan.final_states and scan.workspace are ignored.  The parameters'
- *    gradients are fp32; every gradient carries the same bits on every run. */
+ *    gradients are fp32; every gradient carries the same bits on every run.  The workspace holds the
+ *    channel blocks' shares of dB and dC, b * l * channels * n^2 / 32 bytes (n: dstate rounded up to a
+ *    power of two, at least 8) up to 512 MB, from where on the problem is walked in ranges of positions
+ *    (at least 16 positions of one batch element), and a few times the states. */
 typedef struct {
   ssd_token_scan_params_t scan;
   const void* dout;          /* (b, l, d) of x_dtype */

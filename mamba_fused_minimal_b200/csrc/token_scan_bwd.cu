@@ -15,6 +15,11 @@
 // Few channels and a long sequence: segments side by side as in the forward pass; a first walk finds what each
 // hands to the one before it (18000 positions of 256 channels: 2063 to 356 us).
 //
+// A block's share of dB and dC takes 2 dstate floats a position, and a block holds 256 / dstate channels, so the
+// shares grow with the square of dstate.  Where they pass 512 MB the problem is walked in ranges of positions,
+// the last one first, and in parts of the batch; one range's shares are summed before the next one overwrites
+// them, and what it hands on waits in memory.
+//
 // Measured at 2 x 2048 x 5120 channels of 16, bf16: 880 us, bound by issue slots (62 %): about 50 instructions
 // for each position, channel and component, half of them the exchanges of the two kinds of sums.
 #include "token_scan.cuh"
@@ -30,15 +35,17 @@ constexpr int kPitch = kT + 4;                    // row pitch in shared memory
 struct ScanBwdArgs {
   ScanArgs f;
   const void* dout;
-  const float* dfinal;
+  const float* carry_in;   // (batch, d, n): what comes from behind the range, or null
+  float* carry_out;        // (batch, d, n): what it hands on, or null
   void* dx;
   void* ddt;
   void* dz;
-  float* dinit;
-  float* part_bc;      // (b, l, g, tiles_per_group, 2, n): the blocks' shares of dB and dC
-  float* part_A;       // (b, segments, d, n)
-  float* part_D;       // (b, segments, d)
-  float* part_bias;    // (b, segments, d)
+  int b0, r_lo, r_hi;      // the launch's first batch element, its positions r_lo .. r_hi - 1
+  // of the launch's batch elements and positions:
+  float* part_bc;      // (batch, positions, g, tiles_per_group, 2, n): the blocks' shares of dB and dC
+  float* part_A;       // (batch, segments, d, n)
+  float* part_D;       // (batch, segments, d)
+  float* part_bias;    // (batch, segments, d)
   int64_t d_sb, d_sl;
   int unit, unit32, unit_y, unit_bc, unit_ck;   // bytes copied at a time of x and the like, of an fp32 dt, of out_x, of B and C, of the states
 };
@@ -110,9 +117,9 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   float* s_bc = s_p + 2 * CH * SL * kPitch;          // [warps][kT][ROW]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int grp = blockIdx.x / a.tiles_per_group, tile_c = blockIdx.x % a.tiles_per_group;
-  const int b = blockIdx.y, seg = CARRY ? blockIdx.z + 1 : blockIdx.z;      // nothing needs what the first one passes on
-  const int t_lo = seg * a.seg_len, t_hi = min(a.seqlen, t_lo + a.seg_len);
-  const int64_t bs = (int64_t)b * a.segments + seg;
+  const int bl = blockIdx.y, b = q.b0 + bl, seg = CARRY ? blockIdx.z + 1 : blockIdx.z;      // nothing needs what the first one passes on
+  const int t_lo = q.r_lo + seg * a.seg_len, t_hi = min(q.r_hi, t_lo + a.seg_len);
+  const int64_t bs = (int64_t)bl * a.segments + seg;
   const int c0 = grp * a.per_group + tile_c * CH;
   const int nch = min(CH, a.per_group - tile_c * CH);
   const int tiles = (a.seqlen + kT - 1) / kT;
@@ -177,13 +184,13 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   const int at_n = has ? (c0 + ch) * a.dstate + n : 0;            // of a (channels, dstate) tensor
   const int64_t ck_step = (int64_t)a.channels * a.dstate;
   const float A = has ? load_f(a.A, a.A_dtype, at_n) : 0.0f;
-  float carry = has && q.dfinal && !CARRY ? q.dfinal[b * ck_step + at_n] : 0.0f;      // a_{t+1} g_{t+1}
+  float carry = has && q.carry_in && !CARRY ? q.carry_in[bl * ck_step + at_n] : 0.0f;      // a_{t+1} g_{t+1}
   if (!CARRY && has) {
     // through the segments behind, from the last one on
     for (int j = a.segments - 1; j > seg; --j) {
-      const int64_t at = (int64_t)b * a.segments + j;
+      const int64_t at = (int64_t)bl * a.segments + j;
       const float2 dec = a.seg_decay[at * a.channels + c0 + ch];
-      const bool keeps = dec.y != 0.0f && (j < a.segments - 1 || q.dfinal != nullptr);      // else there is nothing to keep
+      const bool keeps = dec.y != 0.0f && (j < a.segments - 1 || q.carry_in != nullptr);      // else there is nothing to keep
       carry = (keeps ? ex2_approx(A * kLog2e * dec.x) * carry : 0.0f) + a.seg_state[at * ck_step + at_n];
     }
   }
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   constexpr int kOuts = kT * SL * ROW / NT, kQ = NT / ROW, kSum = kBwdWarps / SL;
   const int oq = tid / ROW, oj = tid % ROW;
   const int64_t out_row = (int64_t)a.ngroups * a.tiles_per_group * 2 * a.dstate;
-  float* const part = q.part_bc + ((int64_t)b * a.seqlen * a.ngroups + grp) * a.tiles_per_group * (2 * a.dstate) + (int64_t)tile_c * 2 * a.dstate;
+  float* const part = q.part_bc + ((int64_t)bl * (q.r_hi - q.r_lo) - q.r_lo) * out_row + ((int64_t)grp * a.tiles_per_group + tile_c) * 2 * a.dstate;
   const int part_at = (oj / (ROW / 2)) * a.dstate + oj % (ROW / 2);
 
   fetch(last, 0);
@@ -429,7 +436,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   }
   if (has) {
     q.part_A[bs * ck_step + at_n] = sum_A;
-    if (q.dinit && seg == 0) q.dinit[b * ck_step + at_n] = carry;
+    if (q.carry_out && seg == 0) q.carry_out[bl * ck_step + at_n] = carry;
   }
   // dD and the bias's gradient: over the threads of a channel in order
   __syncthreads();
@@ -444,41 +451,42 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
   }
 }
 
-// The blocks' shares, joined in a fixed order.  Block i < rows: dB and dC of one (position, group) over the
-// channel blocks, eight strides side by side (one thread a sum was bound by the latency of its chain of loads:
-// 160 us for 4096 positions of 320 blocks).  The blocks behind: dA, dD and the bias's gradient over the batch and
-// its segments, one thread an element.
+// The blocks' shares, joined in a fixed order.  Block i < sums: 32 components of dB and dC of one (position, group)
+// over the channel blocks, eight strides side by side (one thread a sum was bound by the latency of its chain of
+// loads: 160 us for 4096 positions of 320 blocks).  The blocks behind: dA, dD and the bias's gradient over the batch
+// and its segments, one thread an element; `more` adds them to what earlier launches left.
+__host__ __device__ constexpr int sum_columns(int dstate) { return (2 * dstate + 31) / 32; }
 template <typename T>
-__global__ void __launch_bounds__(256) sum_shares_kernel(ScanBwdArgs q, T* dB, T* dC, float* dA, float* dD, float* dbias, int rows, int parts) {
+__global__ void __launch_bounds__(256) sum_shares_kernel(ScanBwdArgs q, T* dB, T* dC, float* dA, float* dD, float* dbias, int sums, int parts, bool more) {
   __shared__ float s[8][33];
   const int dstate = q.f.dstate, tiles = q.f.tiles_per_group;
-  if ((int)blockIdx.x < rows) {
-    const int64_t row = blockIdx.x;
+  if ((int)blockIdx.x < sums) {
+    const int columns = sum_columns(dstate);
+    const int64_t row = blockIdx.x / columns;
+    const int j = (int)(blockIdx.x % columns) * 32 + threadIdx.x;
     const float* p = q.part_bc + row * tiles * (2 * dstate);
-    for (int j0 = 0; j0 < 2 * dstate; j0 += 32) {
-      const int j = j0 + threadIdx.x;
-      float v = 0.0f;
-      if (j < 2 * dstate) {
+    float v = 0.0f;
+    if (j < 2 * dstate) {
 #pragma unroll 8
-        for (int k = threadIdx.y; k < tiles; k += 8) v += p[(int64_t)k * 2 * dstate + j];
-      }
-      s[threadIdx.y][threadIdx.x] = v;
-      __syncthreads();
-      if (threadIdx.y == 0 && j < 2 * dstate) {
-        float u = 0.0f;
+      for (int k = threadIdx.y; k < tiles; k += 8) v += p[(int64_t)k * 2 * dstate + j];
+    }
+    s[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0 && j < 2 * dstate) {
+      float u = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) u += s[k][threadIdx.x];
-        if (j < dstate)
-          dB[row * dstate + j] = narrow<T>(u);
-        else
-          dC[row * dstate + j - dstate] = narrow<T>(u);
-      }
-      __syncthreads();
+      for (int k = 0; k < 8; ++k) u += s[k][threadIdx.x];
+      const int64_t each = (int64_t)(q.r_hi - q.r_lo) * q.f.ngroups, bl = row / each;
+      const int64_t to = (((q.b0 + bl) * q.f.seqlen + q.r_lo) * q.f.ngroups + (row - bl * each)) * dstate;
+      if (j < dstate)
+        dB[to + j] = narrow<T>(u);
+      else
+        dC[to + j - dstate] = narrow<T>(u);
     }
     return;
   }
   const int64_t dn = (int64_t)q.f.channels * dstate, d = q.f.channels;
-  int64_t i = (int64_t)(blockIdx.x - rows) * 256 + threadIdx.y * 32 + threadIdx.x;
+  int64_t i = (int64_t)(blockIdx.x - sums) * 256 + threadIdx.y * 32 + threadIdx.x;
   const float* p = q.part_A;
   float* out = dA;
   int64_t pitch = dn;
@@ -492,7 +500,7 @@ __global__ void __launch_bounds__(256) sum_shares_kernel(ScanBwdArgs q, T* dB, T
     }
   }
   if (out == nullptr) return;
-  float v = 0.0f;
+  float v = more ? out[i] : 0.0f;
 #pragma unroll 4
   for (int b = 0; b < parts; ++b) v += p[b * pitch + i];
   out[i] = v;
@@ -505,30 +513,52 @@ int bwd_tiles(const ssd_token_scan_params_t& p) {
   return (p.channels / p.ngroups + ch - 1) / ch;
 }
 
-// Segments: where less than half of the blocks that fit the GPU would run, as many as fill it, none shorter
-// than 128 positions.  The pass that finds what a segment hands on costs a quarter of the walk.
-int bwd_segments(const ssd_token_scan_params_t& p, int* seg_len) {
-  const int64_t blocks = (int64_t)p.batch * p.ngroups * bwd_tiles(p);
-  const int64_t want = 2 * 148 / blocks, room = p.seqlen / 128;
-  int64_t n = want < room ? want : room;
+constexpr int64_t kShares = 512 << 20;      // bytes of the shares of dB and dC that a launch may leave
+
+// How a problem is walked: `batch` batch elements and `len` positions a launch, in segments of `seg_len`.
+struct BwdPlan {
+  int batch, len, segments, seg_len;
+};
+BwdPlan plan_bwd(const ssd_token_scan_params_t& p) {
+  BwdPlan s{p.batch, p.seqlen, 1, p.seqlen};
+  const int64_t fit = 2 * 148, blocks = (int64_t)p.ngroups * bwd_tiles(p);      // of one batch element
+  const int64_t bytes = blocks * 2 * p.dstate * sizeof(float);                  // and one position
+  if (bytes > kShares / ((int64_t)p.batch * p.seqlen)) {
+    // batch elements side by side as long as they are needed for four waves of blocks, then as many positions as
+    // there is room for, evenly
+    const int64_t want = (4 * fit + blocks - 1) / blocks;
+    const int64_t parts = (p.batch + (want < p.batch ? want : p.batch) - 1) / (want < p.batch ? want : p.batch);
+    s.batch = (int)((p.batch + parts - 1) / parts);
+    int64_t len = kShares / (bytes * s.batch) / kT * kT;
+    if (len < kT) len = kT;
+    if (len < p.seqlen) {
+      const int64_t ranges = (p.seqlen + len - 1) / len;
+      s.len = (int)(((p.seqlen + ranges - 1) / ranges + kT - 1) / kT * kT);
+    }
+  }
+  // Segments: where less than half of the blocks that fit the GPU would run, as many as fill it, none shorter
+  // than 128 positions.  The pass that finds what a segment hands on costs a quarter of the walk.
+  const int64_t side = fit / (blocks * s.batch), room = s.len / 128;
+  int64_t n = side < room ? side : room;
   if (n < 2) n = 1;
-  *seg_len = (int)(((p.seqlen + n - 1) / n + kT - 1) / kT * kT);
-  return (p.seqlen + *seg_len - 1) / *seg_len;
+  s.seg_len = (int)(((s.len + n - 1) / n + kT - 1) / kT * kT);
+  s.segments = (s.len + s.seg_len - 1) / s.seg_len;
+  return s;
 }
 
 struct BwdWorkspace {
-  size_t bc, A, D, state, decay, total;      // offsets in floats; the bias's shares follow dD's
+  size_t bc, A, D, state, carry, decay, total;      // offsets in floats; the bias's shares follow dD's
 };
-BwdWorkspace bwd_workspace(const ssd_token_scan_params_t& p) {
-  int seg_len;
-  const size_t segments = bwd_segments(p, &seg_len), dn = (size_t)p.channels * p.dstate;
+BwdWorkspace bwd_workspace(const ssd_token_scan_params_t& p, const BwdPlan& s) {
+  const size_t dn = (size_t)p.channels * p.dstate, each = (size_t)s.batch * s.segments;
   BwdWorkspace w;
   w.decay = 0;                               // pairs: the first, for their alignment
-  w.bc = w.decay + (segments > 1 ? 2 * (size_t)p.batch * segments * p.channels : 0);
-  w.A = w.bc + (size_t)p.batch * p.seqlen * p.ngroups * bwd_tiles(p) * 2 * p.dstate;
-  w.D = w.A + (size_t)p.batch * segments * dn;
-  w.state = w.D + 2 * (size_t)p.batch * segments * p.channels;
-  w.total = w.state + (segments > 1 ? (size_t)p.batch * segments * dn : 0);
+  w.bc = w.decay + (s.segments > 1 ? 2 * each * p.channels : 0);
+  w.A = w.bc + (size_t)s.batch * s.len * p.ngroups * bwd_tiles(p) * 2 * p.dstate;
+  w.D = w.A + each * dn;
+  w.state = w.D + 2 * each * p.channels;
+  w.carry = w.state + (s.segments > 1 ? each * dn : 0);
+  w.total = w.carry + (s.len < p.seqlen ? 2 * (size_t)s.batch * dn : 0);      // one is read while the other is written
   return w;
 }
 
@@ -573,45 +603,58 @@ int launch_bwd(ScanBwdArgs& q, int batch, cudaStream_t stream) {
 
 }  // namespace
 
-size_t token_scan_bwd_workspace(const ssd_token_scan_bwd_params_t& p) { return bwd_workspace(p.scan).total * sizeof(float); }
+size_t token_scan_bwd_workspace(const ssd_token_scan_bwd_params_t& p) { return bwd_workspace(p.scan, plan_bwd(p.scan)).total * sizeof(float); }
 
 int launch_token_scan_bwd(const ssd_token_scan_bwd_params_t& r, cudaStream_t stream) {
   const ssd_token_scan_params_t& p = r.scan;
-  const BwdWorkspace w = bwd_workspace(p);
+  SSD_REQUIRE(p.batch <= 65535 && (int64_t)p.batch * p.seqlen * p.ngroups <= 0x3fffffff, SSD_ERR_UNSUPPORTED,
+              "token scan: batch %d, seqlen %d or ngroups %d too large", p.batch, p.seqlen, p.ngroups);
+  SSD_REQUIRE((int64_t)p.channels * p.dstate <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "token scan: %d channels of %d too many", p.channels, p.dstate);
+  const BwdPlan s = plan_bwd(p);
+  const BwdWorkspace w = bwd_workspace(p, s);
+  const int64_t dn = (int64_t)p.channels * p.dstate;
   ScanBwdArgs q;
   q.f = scan_args(p);
   q.f.tiles_per_group = bwd_tiles(p);
+  q.f.seg_len = s.seg_len;
   q.dout = r.dout;
-  q.dfinal = r.dfinal_states;
-  q.dx = r.dx, q.ddt = r.ddt, q.dz = r.dz, q.dinit = r.dinitial_states;
+  q.dx = r.dx, q.ddt = r.ddt, q.dz = r.dz;
   float* ws = static_cast<float*>(r.workspace);
   q.part_bc = ws + w.bc;
   q.part_A = ws + w.A;
   q.part_D = ws + w.D;
-  q.f.segments = bwd_segments(p, &q.f.seg_len);
-  q.part_bias = q.part_D + (size_t)p.batch * q.f.segments * p.channels;
+  q.part_bias = q.part_D + (size_t)s.batch * s.segments * p.channels;
   q.f.seg_state = ws + w.state;
   q.f.seg_decay = reinterpret_cast<float2*>(ws + w.decay);
   q.d_sb = r.dout_stride[0], q.d_sl = r.dout_stride[1];
-  SSD_REQUIRE(p.batch <= 65535 && (int64_t)p.batch * p.seqlen * p.ngroups <= 0x3fffffff, SSD_ERR_UNSUPPORTED,
-              "token scan: batch %d, seqlen %d or ngroups %d too large", p.batch, p.seqlen, p.ngroups);
-  SSD_REQUIRE((int64_t)p.channels * p.dstate <= 0x7fffffff, SSD_ERR_UNSUPPORTED, "token scan: %d channels of %d too many", p.channels, p.dstate);
   return with_type(p.x_dtype, [&](auto t) -> int {
     using T = decltype(t);
-    int rc;
-    switch (padded_state(p.dstate)) {
-      case 8: rc = launch_bwd<T, 8>(q, p.batch, stream); break;
-      case 16: rc = launch_bwd<T, 16>(q, p.batch, stream); break;
-      case 32: rc = launch_bwd<T, 32>(q, p.batch, stream); break;
-      case 64: rc = launch_bwd<T, 64>(q, p.batch, stream); break;
-      case 128: rc = launch_bwd<T, 128>(q, p.batch, stream); break;
-      default: rc = launch_bwd<T, 256>(q, p.batch, stream); break;
+    bool more = false;
+    for (q.b0 = 0; q.b0 < p.batch; q.b0 += s.batch) {
+      const int batch = p.batch - q.b0 < s.batch ? p.batch - q.b0 : s.batch;
+      float* carry[2] = {ws + w.carry, ws + w.carry + s.batch * dn};
+      for (int range = (p.seqlen - 1) / s.len; range >= 0; --range, more = true) {
+        q.r_lo = range * s.len;
+        q.r_hi = p.seqlen - q.r_lo < s.len ? p.seqlen : q.r_lo + s.len;
+        q.f.segments = (q.r_hi - q.r_lo + s.seg_len - 1) / s.seg_len;
+        q.carry_in = q.r_hi < p.seqlen ? carry[range & 1] : r.dfinal_states ? r.dfinal_states + q.b0 * dn : nullptr;
+        q.carry_out = range > 0 ? carry[(range - 1) & 1] : r.dinitial_states ? r.dinitial_states + q.b0 * dn : nullptr;
+        int rc;
+        switch (padded_state(p.dstate)) {
+          case 8: rc = launch_bwd<T, 8>(q, batch, stream); break;
+          case 16: rc = launch_bwd<T, 16>(q, batch, stream); break;
+          case 32: rc = launch_bwd<T, 32>(q, batch, stream); break;
+          case 64: rc = launch_bwd<T, 64>(q, batch, stream); break;
+          case 128: rc = launch_bwd<T, 128>(q, batch, stream); break;
+          default: rc = launch_bwd<T, 256>(q, batch, stream); break;
+        }
+        if (rc != SSD_OK) return rc;
+        const int64_t sums = (int64_t)batch * (q.r_hi - q.r_lo) * p.ngroups * sum_columns(p.dstate), params = ((int64_t)p.channels * (p.dstate + 2) + 255) / 256;
+        sum_shares_kernel<T><<<(unsigned)(sums + params), dim3(32, 8), 0, stream>>>(q, static_cast<T*>(r.dB), static_cast<T*>(r.dC), r.dA, r.dD,
+                                                                                   r.ddt_bias, (int)sums, batch * q.f.segments, more);
+        SSD_CUDA_OK(cudaGetLastError());
+      }
     }
-    if (rc != SSD_OK) return rc;
-    const int64_t rows = (int64_t)p.batch * p.seqlen * p.ngroups, params = ((int64_t)p.channels * (p.dstate + 2) + 255) / 256;
-    sum_shares_kernel<T><<<(unsigned)(rows + params), dim3(32, 8), 0, stream>>>(q, static_cast<T*>(r.dB), static_cast<T*>(r.dC), r.dA, r.dD, r.ddt_bias,
-                                                                               (int)rows, p.batch * q.f.segments);
-    SSD_CUDA_OK(cudaGetLastError());
     return SSD_OK;
   });
 }

@@ -110,3 +110,72 @@ def test_conv_gradients_refuse_wide_filters(cuda_device):
         x, w = torch.zeros(2, 40, 64, device="cuda"), torch.zeros(64, width, device="cuda")
         with pytest.raises(RuntimeError, match="not 2, 3 or 4"):
             conv._short_conv_bwd(x, x, w)
+
+
+def in_pieces(scan, dout, dfinal, pos, kw, size):
+    """Forward and gradients of a sequence piece by piece, each from the state the one before it left."""
+    pieces, state = [], kw["initial_states"]
+    l = dout.shape[1]
+    cut = lambda t, lo, hi: t if t is None or t.dim() < 3 else t[:, lo:hi]  # noqa: E731
+    for lo in range(0, l, size):
+        hi = min(l, lo + size)
+        p = [cut(t, lo, hi) for t in pos]
+        k = dict(kw, z=cut(kw["z"], lo, hi), initial_states=state)
+        out, state, saved = scan._token_scan_fwd(*p, for_backward=True, **k)
+        pieces.append((lo, hi, p, k, saved, out))
+    grads, g = [], dfinal
+    for lo, hi, p, k, saved, _ in reversed(pieces):
+        grads.insert(0, scan._token_scan_bwd(dout[:, lo:hi], *p, saved, dfinal_states=g, **k))
+        g = grads[0][8]
+    join = lambda i: None if grads[0][i] is None else torch.cat([t[i] for t in grads], 1)  # noqa: E731
+    total = lambda i: sum(t[i].double() for t in grads)  # noqa: E731
+    return [join(0), join(1), total(2), join(3), join(4), total(5), join(6), total(7), g]
+
+
+@pytest.mark.parametrize("dtype,b,l,d,n,g,piece", [
+    (torch.float32, 1, 300, 1024, 256, 1, 96),           # many channel blocks: a few positions at a time
+    (torch.bfloat16, 3, 437, 600, 200, 2, 112),          # the batch, too, in parts
+    (torch.bfloat16, 1, 17001, 32, 256, 1, 4096),        # few channels, long: segments within each range
+])
+def test_scan_gradients_of_long_states_in_ranges(cuda_device, dtype, b, l, d, n, g, piece):
+    """Problems whose channel blocks' shares of dB and dC do not fit the scratch at once, against the same sequence
+    in pieces that do: the same sums, cut elsewhere.  Per tensor 64 u sqrt(l), and half a step where it is kept
+    in 16 bits (once for each side)."""
+    scan = ops()[2]
+    inp = {k: v.to("cuda") for k, v in scan_inputs(b, l, d, n, g, dtype, 76).items()}
+    r = maker(77)
+    dout, dfinal, init = r(b, l, d, dtype=dtype).to("cuda"), r(b, d, n).to("cuda"), r(b, d, n).to("cuda")
+    pos = [inp[k] for k in KEYS]
+    kw = dict(D=inp["D"], z=inp["z"], dt_bias=inp["dt_bias"], dt_softplus=True, initial_states=init)
+    _, _, saved = scan._token_scan_fwd(*pos, for_backward=True, **kw)
+    got = scan._token_scan_bwd(dout, *pos, saved, dfinal_states=dfinal, **kw)
+    again = scan._token_scan_bwd(dout, *pos, saved, dfinal_states=dfinal, **kw)
+    ref = in_pieces(scan, dout, dfinal, pos, kw, piece)
+    names = ("dx", "ddt", "dA", "dB", "dC", "dD", "dz", "ddt_bias", "dinitial")
+    for name, a, a2, e in zip(names, got, again, ref):
+        step = 2 * half_step(dtype) if name in ("dx", "ddt", "dB", "dC", "dz") else 0
+        assert torch.equal(a, a2) and norm_err(a, e.double().cpu()) <= 4 * 64 * U * math.sqrt(l) + step, name
+
+
+def test_scan_gradients_in_ranges_against_the_oracle(cuda_device):
+    """The same against autograd through the 64-bit definition, with packed sequences, a gradient of the last
+    state and none."""
+    scan = ops()[2]
+    b, l, d, n = 1, 300, 1024, 256
+    inp = {k: v.to("cuda") for k, v in scan_inputs(b, l, d, n, 1, torch.float32, 78).items()}
+    r = maker(79)
+    dout, dfinal, init = r(b, l, d).to("cuda"), r(b, d, n).to("cuda"), r(b, d, n).to("cuda")
+    seq = packed(b, l, 5).to("cuda")
+    kw = dict(D=inp["D"], dt_bias=inp["dt_bias"], initial_states=init)
+    leaves = [inp[k].double().requires_grad_() for k in KEYS]
+    lkw = {k: v.double().requires_grad_() for k, v in kw.items()}
+    for s, df in ((None, dfinal), (seq, None)):
+        for t in (*leaves, *lkw.values()):
+            t.grad = None
+        out, last, _, _ = L.token_scan(*leaves, dt_softplus=True, seq_idx=s, **lkw)
+        ((out * dout.double()).sum() + (0 if df is None else (last * df.double()).sum())).backward()
+        pos = [inp[k] for k in KEYS]
+        _, _, saved = scan._token_scan_fwd(*pos, dt_softplus=True, seq_idx=s, for_backward=True, **kw)
+        g = scan._token_scan_bwd(dout, *pos, saved, dt_softplus=True, seq_idx=s, dfinal_states=df, **kw)
+        for a, t in zip((*g[:6], g[7], g[8]), (*leaves, lkw["D"], lkw["dt_bias"], lkw["initial_states"])):
+            assert norm_err(a, t.grad.cpu()) <= 4 * 64 * U * math.sqrt(l)

@@ -53,3 +53,31 @@ def test_norm_workspace_of_no_size(field, value):
     assert query("ssd_add_rms_norm_bwd", p) == 80 * 64 * 4
     setattr(p, field, value)
     assert query("ssd_add_rms_norm_bwd", p) == 0
+
+
+Scan = struct("Scan", [(k, PTR) for k in "x dt A B C D z bias init seq out out_x fin ckpt".split()] +
+              [(k, I32) for k in "xd dtd Ad Dd bd id batch seqlen channels ngroups dstate softplus".split()] +
+              [("dt_min", ctypes.c_float), ("dt_max", ctypes.c_float), ("s", I64 * 14), ("workspace", PTR), ("bytes", ctypes.c_size_t)])
+ScanBwd = struct("ScanBwd", [("scan", Scan)] + [(k, PTR) for k in "dout dfinal dx ddt dA dB dC dD dz dbias dinit".split()] +
+                 [("ds", I64 * 2), ("workspace", PTR), ("bytes", ctypes.c_size_t)])
+
+
+@pytest.mark.parametrize("batch,seqlen,channels,ngroups,dstate", [
+    (1, 4096, 2048, 1, 128), (8, 4096, 5120, 1, 128), (2, 2048, 5120, 1, 256), (1, 65537, 296, 1, 256), (1, 1 << 20, 5120, 8, 64),
+    (64, 4096, 5120, 1, 16), (3, 1000, 64, 64, 256), (1, 40000, 8192, 1, 200), (2, 2048, 5120, 1, 16), (1, 1, 1, 1, 1)])
+def test_scan_gradients_scratch_is_bounded(batch, seqlen, channels, ngroups, dstate):
+    """Whatever the problem's size: 512 MB for the channel blocks' shares of dB and dC, or 16 positions' of one batch
+    element where those are more, and a few times the states (as many as there are batch elements, or blocks
+    on the GPU, whichever is more)."""
+    p = ScanBwd()
+    s = p.scan
+    for k in "x dt A B C".split():
+        setattr(s, k, 16)                  # never followed: a query looks at sizes only
+    s.batch, s.seqlen, s.channels, s.ngroups, s.dstate = batch, seqlen, channels, ngroups, dstate
+    s.xd = s.dtd = 1
+    padded = max(8, 1 << (dstate - 1).bit_length())
+    tiles = -(-(channels // ngroups) // (256 // padded))
+    shares = 16 * ngroups * tiles * 2 * dstate * 4
+    states = channels * dstate * 4
+    got = query("ssd_token_scan_bwd", p)
+    assert 0 < got <= max(2 ** 29, shares) + 6 * batch * states + 8 * 2 ** 20
