@@ -57,6 +57,10 @@ inline Tensor as_int32(const Tensor& seq_idx) {
 
 // An output tensor; between guard bands when debug_set_guard_bytes asked for them (torch_ext.cpp).
 Tensor alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts);
+// The same straight from the CUDA allocator, for the operators around the scan: what torch::empty's dispatch adds
+// is a third of a small call's time.  Dispatch modes, the profiler's list of operators and the deterministic mode's
+// fill do not see such an output.
+Tensor alloc_direct(at::IntArrayRef sizes, const at::TensorOptions& opts);
 
 // Adds the operators around the scan (torch_layer.cpp).
 void bind_layer(pybind11::module& m);

@@ -88,12 +88,7 @@ struct Guarded {
 };
 std::vector<Guarded> g_guarded;
 
-}  // namespace
-
-Tensor ssd_torch::alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts) {
-  const int64_t guard = g_guard_bytes.load(std::memory_order_relaxed);
-  // straight to the CUDA allocator: what torch::empty's dispatch adds is a third of a small call's time
-  if (guard == 0) return at::detail::empty_cuda(sizes, c10::typeMetaToScalarType(opts.dtype()), opts.device_opt(), c10::nullopt);
+Tensor alloc_guarded(at::IntArrayRef sizes, const at::TensorOptions& opts, int64_t guard) {
   int64_t numel = 1;
   for (int64_t d : sizes) numel *= d;
   const int64_t payload = numel * (int64_t)c10::elementSize(c10::typeMetaToScalarType(opts.dtype()));
@@ -103,6 +98,19 @@ Tensor ssd_torch::alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts
   std::lock_guard<std::mutex> lock(g_guard_mutex);
   g_guarded.push_back({buf, payload});
   return out;
+}
+
+}  // namespace
+
+Tensor ssd_torch::alloc_out(at::IntArrayRef sizes, const at::TensorOptions& opts) {
+  const int64_t guard = g_guard_bytes.load(std::memory_order_relaxed);
+  return guard == 0 ? torch::empty(sizes, opts) : alloc_guarded(sizes, opts, guard);
+}
+
+Tensor ssd_torch::alloc_direct(at::IntArrayRef sizes, const at::TensorOptions& opts) {
+  const int64_t guard = g_guard_bytes.load(std::memory_order_relaxed);
+  if (guard != 0) return alloc_guarded(sizes, opts, guard);
+  return at::detail::empty_cuda(sizes, c10::typeMetaToScalarType(opts.dtype()), opts.device_opt(), c10::nullopt);
 }
 
 namespace {

@@ -103,19 +103,19 @@ std::tuple<Tensor, OptTensor, OptTensor, OptTensor> add_rms_norm_fwd(const Tenso
   p.residual_dtype = p.x_dtype;
   if (rdt.has_value()) {
     p.residual_dtype = dtype_code(*rdt);
-    total = alloc_out(x.sizes(), x.options().dtype(*rdt));
+    total = alloc_direct(x.sizes(), x.options().dtype(*rdt));
     p.residual_out = total->data_ptr();
   }
   const at::ScalarType odt = out_dtype.value_or(x.scalar_type());
   p.out_dtype = out_code(odt);
-  Tensor out = alloc_out(x.sizes(), x.options().dtype(odt));
+  Tensor out = alloc_direct(x.sizes(), x.options().dtype(odt));
   const auto f32 = x.options().dtype(at::kFloat);
   const auto rows = x.sizes().slice(0, x.dim() - 1);
   if (p.out_dtype == SSD_I8 || p.out_dtype == SSD_E4M3) {
-    scales = alloc_out(rows, f32);
+    scales = alloc_direct(rows, f32);
     p.scales = scales->data_ptr<float>();
   } else {
-    rstd = alloc_out(rows, f32);
+    rstd = alloc_direct(rows, f32);
     p.rstd = rstd->data_ptr<float>();
   }
   p.out = out.data_ptr();
@@ -155,13 +155,13 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_bwd(const Tensor& dout, const Te
     p.dresidual = dresidual->data_ptr();
     row_strides(p.dresidual_stride, *dresidual);
   }
-  Tensor dx = alloc_out(total.sizes(), total.options().dtype(xdt));
+  Tensor dx = alloc_direct(total.sizes(), total.options().dtype(xdt));
   Tensor dres = dx;
   if (xdt != total.scalar_type()) {
-    dres = alloc_out(total.sizes(), total.options());
+    dres = alloc_direct(total.sizes(), total.options());
     p.dresidual_in = dres.data_ptr();
   }
-  Tensor dweight = alloc_out({total.size(-1)}, total.options().dtype(at::kFloat));
+  Tensor dweight = alloc_direct({total.size(-1)}, total.options().dtype(at::kFloat));
   p.dx = dx.data_ptr();
   p.dweight = dweight.data_ptr<float>();
   p.workspace_bytes = ssd_add_rms_norm_bwd_workspace_bytes(&p);
@@ -213,11 +213,11 @@ std::tuple<Tensor, OptTensor> short_conv_fwd(const Tensor& x, const Tensor& weig
   ssd_short_conv_params_t p{};
   ConvHold h;
   fill_conv(p, h, x, weight, bias, silu, initial_states, seq_idx);
-  Tensor out = alloc_out(x.sizes(), x.options());
+  Tensor out = alloc_direct(x.sizes(), x.options());
   OptTensor fin;
   p.out = out.data_ptr();
   if (return_final) {
-    fin = alloc_out({x.size(0), weight.size(1) - 1, x.size(2)}, x.options());
+    fin = alloc_direct({x.size(0), weight.size(1) - 1, x.size(2)}, x.options());
     p.final_states = fin->data_ptr();
   }
   check_rc(ssd_short_conv_fwd(&p, current_stream(x)), "ssd_short_conv_fwd");
@@ -246,17 +246,17 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> short_conv_bwd(const Tensor& do
     p.dfinal_states = fh.data_ptr();
   }
   const auto f32 = x.options().dtype(at::kFloat);
-  Tensor dx = alloc_out(x.sizes(), x.options());
-  Tensor dweight = alloc_out(weight.sizes(), f32);
+  Tensor dx = alloc_direct(x.sizes(), x.options());
+  Tensor dweight = alloc_direct(weight.sizes(), f32);
   OptTensor dbias, dinit;
   p.dx = dx.data_ptr();
   p.dweight = dweight.data_ptr<float>();
   if (bias.has_value()) {
-    dbias = alloc_out(bias->sizes(), f32);
+    dbias = alloc_direct(bias->sizes(), f32);
     p.dbias = dbias->data_ptr<float>();
   }
   if (initial_states.has_value()) {
-    dinit = alloc_out(initial_states->sizes(), x.options());
+    dinit = alloc_direct(initial_states->sizes(), x.options());
     p.dinitial_states = dinit->data_ptr();
   }
   p.workspace_bytes = ssd_short_conv_bwd_workspace_bytes(&p);
@@ -293,7 +293,7 @@ Tensor short_conv_step(const Tensor& x, Tensor conv_state, const Tensor& weight,
   param(weight, x, "weight", wh, p.weight, p.weight_dtype);
   param(bias, x, "bias", bh, p.bias, p.bias_dtype);
   p.state_indices = slots_of(state_indices, x, ih);
-  Tensor out = alloc_out(x.sizes(), x.options());
+  Tensor out = alloc_direct(x.sizes(), x.options());
   p.out = out.data_ptr();
   p.x_dtype = dtype_code(x, "x");
   p.batch = i32(x.size(0));
@@ -378,16 +378,16 @@ std::tuple<Tensor, Tensor, OptTensor, OptTensor> token_scan_fwd(const Tensor& x,
   fill_scan(p, h, x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_min, dt_max, initial_states, seq_idx);
   const int64_t b = x.size(0), l = x.size(1), d = x.size(2), n = B.size(3);
   const auto f32 = x.options().dtype(at::kFloat);
-  Tensor out = alloc_out(x.sizes(), x.options());
-  Tensor fin = alloc_out({b, d, n}, f32);
+  Tensor out = alloc_direct(x.sizes(), x.options());
+  Tensor fin = alloc_direct({b, d, n}, f32);
   OptTensor out_x, ckpt;
   p.out = out.data_ptr();
   p.final_states = fin.data_ptr<float>();
   if (for_backward) {
-    ckpt = alloc_out({b, (l + SSD_TOKEN_SCAN_CHECKPOINT - 1) / SSD_TOKEN_SCAN_CHECKPOINT, d, n}, f32);
+    ckpt = alloc_direct({b, (l + SSD_TOKEN_SCAN_CHECKPOINT - 1) / SSD_TOKEN_SCAN_CHECKPOINT, d, n}, f32);
     p.checkpoints = ckpt->data_ptr<float>();
     if (z.has_value()) {
-      out_x = alloc_out(x.sizes(), f32);
+      out_x = alloc_direct(x.sizes(), f32);
       p.out_x = out_x->data_ptr<float>();
     }
   }
@@ -436,8 +436,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
     p.dfinal_states = fh.data_ptr<float>();
   }
   const auto f32 = x.options().dtype(at::kFloat);
-  Tensor dx = alloc_out(x.sizes(), x.options()), ddt = alloc_out(dt.sizes(), dt.options()), dA = alloc_out(A.sizes(), f32);
-  Tensor dB = alloc_out(B.sizes(), B.options()), dC = alloc_out(C.sizes(), C.options());
+  Tensor dx = alloc_direct(x.sizes(), x.options()), ddt = alloc_direct(dt.sizes(), dt.options()), dA = alloc_direct(A.sizes(), f32);
+  Tensor dB = alloc_direct(B.sizes(), B.options()), dC = alloc_direct(C.sizes(), C.options());
   OptTensor dD, dz, dbias, dinit;
   p.dx = dx.data_ptr();
   p.ddt = ddt.data_ptr();
@@ -445,19 +445,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
   p.dB = dB.data_ptr();
   p.dC = dC.data_ptr();
   if (D.has_value()) {
-    dD = alloc_out(D->sizes(), f32);
+    dD = alloc_direct(D->sizes(), f32);
     p.dD = dD->data_ptr<float>();
   }
   if (z.has_value()) {
-    dz = alloc_out(x.sizes(), x.options());
+    dz = alloc_direct(x.sizes(), x.options());
     p.dz = dz->data_ptr();
   }
   if (dt_bias.has_value()) {
-    dbias = alloc_out(dt_bias->sizes(), f32);
+    dbias = alloc_direct(dt_bias->sizes(), f32);
     p.ddt_bias = dbias->data_ptr<float>();
   }
   if (initial_states.has_value()) {
-    dinit = alloc_out(initial_states->sizes(), f32);
+    dinit = alloc_direct(initial_states->sizes(), f32);
     p.dinitial_states = dinit->data_ptr<float>();
   }
   p.workspace_bytes = ssd_token_scan_bwd_workspace_bytes(&p);
@@ -546,7 +546,7 @@ Tensor token_scan_step(Tensor state, const Tensor& x, const Tensor& dt, const Te
   }
   Tensor ih;
   p.state_indices = slots_of(state_indices, x, ih);
-  Tensor out = alloc_out(x.sizes(), x.options());
+  Tensor out = alloc_direct(x.sizes(), x.options());
   p.out = out.data_ptr();
   check_rc(ssd_token_scan_step(&p, current_stream(x)), "ssd_token_scan_step");
   return out;

@@ -179,3 +179,26 @@ def test_scan_gradients_in_ranges_against_the_oracle(cuda_device):
         g = scan._token_scan_bwd(dout, *pos, saved, dt_softplus=True, seq_idx=s, dfinal_states=df, **kw)
         for a, t in zip((*g[:6], g[7], g[8]), (*leaves, lkw["D"], lkw["dt_bias"], lkw["initial_states"])):
             assert norm_err(a, t.grad.cpu()) <= 4 * 64 * U * math.sqrt(l)
+
+
+def test_chunk_kernels_outputs_pass_the_dispatcher(cuda_device):
+    """Dispatch modes see the outputs that the chunk kernels' calls allocate."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from mamba_fused_minimal_b200.kernels.ssd_chunk_state import _chunk_cumsum_fwd
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.shapes = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            out = func(*args, **(kwargs or {}))
+            if func.overloadpacket in (torch.ops.aten.empty, torch.ops.aten.empty_strided):
+                self.shapes.append(tuple(out.shape))
+            return out
+
+    dt, A = torch.rand(2, 64, 4, device="cuda"), -torch.rand(4, device="cuda")
+    with Seen() as seen:
+        outs = _chunk_cumsum_fwd(dt, A, 32)
+    for t in outs:
+        assert tuple(t.shape) in seen.shapes
