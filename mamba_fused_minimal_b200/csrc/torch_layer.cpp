@@ -471,13 +471,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, OptTensor, OptTensor, OptTens
 Tensor token_scan_step(Tensor state, const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
                        const OptTensor& D, const OptTensor& z, const OptTensor& dt_bias, bool dt_softplus, double dt_min, double dt_max,
                        const OptTensor& state_indices) {
-  const int64_t rank = x.dim(), batch = x.size(0), heads = rank > 1 ? x.size(1) : 0;
+  const int64_t rank = x.dim(), batch = rank > 1 ? x.size(0) : 0, heads = rank > 1 ? x.size(1) : 0;
   assert_shapes((rank == 2 || rank == 3) && state.dim() == rank + 1 && B.dim() == 3 && C.sizes() == B.sizes() && B.size(0) == batch && B.size(1) > 0 &&
                     heads % B.size(1) == 0 && state.sizes().slice(1, rank - 1) == x.sizes().slice(1) && state.size(-1) == B.size(2),
                 "state (slots, nheads, headdim, dstate) with x (batch, nheads, headdim), or (slots, channels, dstate) with (batch, channels); "
                 "B and C (batch, ngroups, dstate)");
-  assert_shapes(dt.dim() == 2 && dt.size(0) == batch && dt.size(1) == heads && A.size(0) == heads &&
-                    (rank == 3 ? A.dim() == 1 : A.dim() == 2 && A.size(1) == B.size(2)) && is_like(z, x) && is_1d(dt_bias, heads) &&
+  assert_shapes(dt.dim() == 2 && dt.size(0) == batch && dt.size(1) == heads &&
+                    (rank == 3 ? A.dim() == 1 : A.dim() == 2 && A.size(1) == B.size(2)) && A.size(0) == heads && is_like(z, x) && is_1d(dt_bias, heads) &&
                     is_1d(state_indices, batch) &&
                     (!D.has_value() || (D->dim() == 1 && D->size(0) == heads) || (rank == 3 && D->sizes() == x.sizes().slice(1))),
                 "dt (batch, nheads), A (nheads,) or (channels, dstate), D (nheads,) or (nheads, headdim), z as x, dt_bias (nheads,), "

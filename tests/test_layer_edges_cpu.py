@@ -81,3 +81,24 @@ def test_scan_gradients_scratch_is_bounded(batch, seqlen, channels, ngroups, dst
     states = channels * dstate * 4
     got = query("ssd_token_scan_bwd", p)
     assert 0 < got <= max(2 ** 29, shares) + 6 * batch * states + 8 * 2 ** 20
+
+
+def test_tensors_of_no_dimension_are_refused():
+    from mamba_fused_minimal_b200.kernels.add_rms_norm import _add_rms_norm_bwd, _add_rms_norm_fwd
+    from mamba_fused_minimal_b200.kernels.short_conv import _short_conv_bwd, _short_conv_fwd, _short_conv_step
+    from mamba_fused_minimal_b200.kernels.token_scan import _token_scan_bwd, _token_scan_fwd, _token_scan_step
+    z = torch.zeros
+    calls = [(_add_rms_norm_fwd, [z(2, 8), z(8)]),
+             (_add_rms_norm_bwd, [z(2, 8), z(2, 8), z(8), z(2)]),
+             (_short_conv_fwd, [z(1, 4, 8), z(8, 4)]),
+             (_short_conv_bwd, [z(1, 4, 8), z(1, 4, 8), z(8, 4)]),
+             (_short_conv_step, [z(1, 8), z(1, 3, 8), z(8, 4)]),
+             (_token_scan_fwd, [z(1, 4, 8), z(1, 4, 8), z(8, 4), z(1, 4, 1, 4), z(1, 4, 1, 4)]),
+             (lambda *a: _token_scan_bwd(*a, (z(1, 1, 8, 4), None)),
+              [z(1, 4, 8), z(1, 4, 8), z(1, 4, 8), z(8, 4), z(1, 4, 1, 4), z(1, 4, 1, 4)]),
+             (_token_scan_step, [z(1, 8, 4), z(1, 8), z(1, 8), z(8, 4), z(1, 1, 4), z(1, 1, 4)]),
+             (_token_scan_step, [z(1, 2, 4, 4), z(1, 2, 4), z(1, 2), z(2), z(1, 1, 4), z(1, 1, 4)])]
+    for call, args in calls:
+        for i in range(len(args)):
+            with pytest.raises(AssertionError):
+                call(*[z(()) if k == i else a for k, a in enumerate(args)])
