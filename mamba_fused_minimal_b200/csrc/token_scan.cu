@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
           unpack2(h[k][s / 2], v[0], v[1]);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            if (n0 + s + i < a.dstate) v[i] = (keeps ? ex2_approx(A[i] * dec.x) * v[i] : 0.0f) + a.seg_state[at * a.dstate + n0 + s + i];
+            if (n0 + s + i < a.dstate) v[i] = (keeps ? through_segment(A[i], dec.x, v[i]) : 0.0f) + a.seg_state[at * a.dstate + n0 + s + i];
           }
           h[k][s / 2] = pack2(v[0], v[1]);
         }

@@ -97,6 +97,10 @@ __device__ __forceinline__ uint32_t reset_mask(const ScanArgs& a, int b, int t0,
   return __ballot_sync(0xffffffffu, reset);
 }
 
+// What of a state is left behind a segment whose dt' add up to `sum`; A2 is A log2(e).  Zero stays zero where A > 0
+// and the decay passes the largest number.
+__device__ __forceinline__ float through_segment(float A2, float sum, float state) { return state == 0.0f ? 0.0f : ex2_approx(A2 * sum) * state; }
+
 ScanArgs scan_args(const ssd_token_scan_params_t& p);
 
 }  // namespace ssd

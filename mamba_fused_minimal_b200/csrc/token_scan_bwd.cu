@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kBwdThreads, 2) token_scan_bwd_kernel(ScanBwdA
       const int64_t at = (int64_t)bl * a.segments + j;
       const float2 dec = a.seg_decay[at * a.channels + c0 + ch];
       const bool keeps = dec.y != 0.0f && (j < a.segments - 1 || q.carry_in != nullptr);      // else there is nothing to keep
-      carry = (keeps ? ex2_approx(A * kLog2e * dec.x) * carry : 0.0f) + a.seg_state[at * ck_step + at_n];
+      carry = (keeps ? through_segment(A * kLog2e, dec.x, carry) : 0.0f) + a.seg_state[at * ck_step + at_n];
     }
   }
   float sum_dt = 0.0f;

@@ -202,3 +202,29 @@ def test_chunk_kernels_outputs_pass_the_dispatcher(cuda_device):
         outs = _chunk_cumsum_fwd(dt, A, 32)
     for t in outs:
         assert tuple(t.shape) in seen.shapes
+
+
+def test_growing_states_across_segments(cuda_device):
+    """Positive A: over a segment the decay passes the largest number, where the state it multiplies is zero.  Few
+    channels and a long row are cut into segments; the result is the one of the definition."""
+    scan = ops()[2]
+    b, l, d, n = 1, 1700, 8, 16
+    r = maker(80)
+    x, dout = r(b, l, d), r(b, l, d)
+    x[:, :l - 20] = 0
+    dout[:, 20:] = 0
+    dt, A = torch.ones(b, l, d), torch.full((d, n), 0.5)
+    B, C = r(b, l, 1, n), r(b, l, 1, n)
+    leaves = [t.double().requires_grad_() for t in (x, dt, A, B, C)]
+    out, last, _, size = L.token_scan(*leaves)
+    pos = cuda(x, dt, A, B, C)
+    got, fin, saved = scan._token_scan_fwd(*pos, for_backward=True)
+    # 20 positions count, each with the sum of 16 terms
+    within(got, out.detach(), size, 66 * 20 * U, torch.float32)
+    assert norm_err(fin, last) <= 66 * 20 * U
+    g = scan._token_scan_bwd(dout.to("cuda"), *pos, saved)
+    # x is zero wherever the gradient reaches: only dx is not zero
+    (out * dout.double()).sum().backward()
+    assert all(torch.isfinite(t).all() for t in g if t is not None)
+    assert norm_err(g[0], leaves[0].grad) <= 66 * 20 * U
+    assert all((t == 0).all() for t in (g[1], g[2], g[3], g[4]))
