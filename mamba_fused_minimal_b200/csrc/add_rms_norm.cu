@@ -261,7 +261,7 @@ void row_shape(int nvec, int64_t rows, int want, int most, int* threads, int* vp
   int v = 1;
   // few rows: one vector per thread, the shortest way through a row.  Many rows: blocks of about `want`
   // threads, so that several rows are in flight on an SM and one row's sums hide behind another's loads.
-  if (rows < 2 * 148) want = kMaxThreads;
+  if (rows < 2 * kSMs) want = kMaxThreads;
   while (v < most && (nvec + v - 1) / v > want) v *= 2;
   *vpt = v;
   *threads = round_up((nvec + v - 1) / v, 32);
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(1024) sum_partials_kernel(const float* partial
 // blocks are small -- and no more than there are rows.
 int bwd_parts(int64_t rows, int dim) {
   const int per_sm = dim >= 4096 ? 2 : dim <= 1024 ? 8 : 8192 / dim;
-  const int64_t most = per_sm * 148;
+  const int64_t most = per_sm * kSMs;
   return (int)(rows < most ? rows : most);
 }
 

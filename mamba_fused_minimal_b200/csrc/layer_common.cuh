@@ -1,6 +1,6 @@
 // Helpers shared by the layer operators around the scan (add_rms_norm.cu, short_conv.cu, token_scan.cu,
 // token_scan_bwd.cu, token_step.cu): vectors of elements widened to fp32, block sums, the activation
-// functions, and the deterministic second pass over partial sums.
+// functions, and the slot of a row of a single-token call.
 #pragma once
 
 #include <cuda_fp8.h>
@@ -12,6 +12,9 @@
 #include "ssd_launch.h"
 
 namespace ssd {
+
+// SMs of a B200, what the plans below count blocks against (a workspace query and its launch have to agree).
+constexpr int kSMs = 148;
 
 // ---- V consecutive elements of type T, widened to fp32 ---------------------------------------------
 template <typename T, int V>
@@ -313,15 +316,6 @@ int with_type(int dtype, F f) {
     case SSD_F16: return f(__half());
     default: return f(float());
   }
-}
-
-inline int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return 148;
-  }
-  return n;
 }
 
 }  // namespace ssd

@@ -24,7 +24,7 @@ constexpr int kStrip = 64;        // most positions of a strip
 int strip_of(int batch, int seqlen, int channels, int halo) {
   int n = kStrip;
   const int64_t rows = (int64_t)batch * ((channels + 511) / 512);
-  while (n > kGroup && rows * ((seqlen + n - halo - 1) / (n - halo)) < 2 * 148) n /= 2;
+  while (n > kGroup && rows * ((seqlen + n - halo - 1) / (n - halo)) < 2 * kSMs) n /= 2;
   return n - halo;
 }
 

@@ -478,7 +478,7 @@ ScanPlan plan_scan(const ssd_token_scan_params_t& p) {
   s.ns = n / s.lpc;
   // segments: only where less than half of the blocks that fit the GPU at once would run, as many as fill
   // it, and none shorter than 256 positions
-  const int64_t fit = 148 * resident(kCh * s.lpc / s.k + helpers(s.lpc), s.ns * s.k);
+  const int64_t fit = kSMs * resident(kCh * s.lpc / s.k + helpers(s.lpc), s.ns * s.k);
   const int64_t want = fit / blocks, room = p.seqlen / 256;
   s.segments = (int)(want < room ? want : room);
   if (s.segments < 3) s.segments = 1;            // the state pass doubles the work

@@ -521,7 +521,7 @@ struct BwdPlan {
 };
 BwdPlan plan_bwd(const ssd_token_scan_params_t& p) {
   BwdPlan s{p.batch, p.seqlen, 1, p.seqlen};
-  const int64_t fit = 2 * 148, blocks = (int64_t)p.ngroups * bwd_tiles(p);      // of one batch element
+  const int64_t fit = 2 * kSMs, blocks = (int64_t)p.ngroups * bwd_tiles(p);      // of one batch element
   const int64_t bytes = blocks * 2 * p.dstate * sizeof(float);                  // and one position
   if (bytes > kShares / ((int64_t)p.batch * p.seqlen)) {
     // batch elements side by side as long as they are needed for four waves of blocks, then as many positions as
