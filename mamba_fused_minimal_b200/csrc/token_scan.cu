@@ -430,12 +430,12 @@ __global__ void __launch_bounds__(ScanShape<T, LPC, NS, K>::kThreads, ScanShape<
       }
       const int end = min(stop, half + SSD_TOKEN_SCAN_CHECKPOINT);
       if (resets == 0u) {
-if (end - half == SSD_TOKEN_SCAN_CHECKPOINT) {
+        if (end - half == SSD_TOKEN_SCAN_CHECKPOINT) {
 #pragma unroll
           for (int k = 0; k < SSD_TOKEN_SCAN_CHECKPOINT; k += 4) four(half + k, s_du, s_bc, s_y, std::false_type(), 0u);
         } else {
 #pragma unroll 1
-        for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::false_type(), 0u);
+          for (int t = half; t < end; t += 4) four(t, s_du, s_bc, s_y, std::false_type(), 0u);
         }
       } else {
 #pragma unroll 1

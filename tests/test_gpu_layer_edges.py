@@ -228,3 +228,171 @@ def test_growing_states_across_segments(cuda_device):
     assert all(torch.isfinite(t).all() for t in g if t is not None)
     assert norm_err(g[0], leaves[0].grad) <= 66 * 20 * U
     assert all((t == 0).all() for t in (g[1], g[2], g[3], g[4]))
+
+
+P16 = [torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("ptype", P16)
+@pytest.mark.parametrize("dim", [96, 97, 33024])
+def test_norm_weight_in_16_bits(cuda_device, ptype, dim):
+    norm = ops()[0]
+    r = maker(81)
+    x, w, dout = r(5, dim, dtype=torch.bfloat16), (1 + 0.1 * r(dim)).to(ptype), r(5, dim, dtype=torch.bfloat16)
+    y, _ = L.add_rms_norm(x, w)
+    tol = (dim / 64 + 32) * U
+    out, _, rstd, _ = norm._add_rms_norm_fwd(*cuda(x, w))
+    within(out, y, y.abs(), tol, torch.bfloat16)
+    xd, wd = x.double().requires_grad_(), w.double().requires_grad_()
+    (L.add_rms_norm(xd, wd)[0] * dout.double()).sum().backward()
+    dx, _, dw = norm._add_rms_norm_bwd(*cuda(dout, x, w), rstd)
+    size = xd.grad.abs() + (dout.double() * wd).abs().detach() * rstd.double().cpu()[:, None]
+    within(dx, xd.grad, size, tol, torch.bfloat16)
+    assert dw.dtype == torch.float32
+    within(dw, wd.grad, (dout.double() * x.double() * rstd.double().cpu()[:, None]).abs().sum(0), tol, torch.float32)
+    # the weight is widened exactly: the bits of the same weight in fp32
+    for kind in (None, torch.int8, torch.float8_e4m3fn):
+        a, b = (norm._add_rms_norm_fwd(x.to("cuda"), v.to("cuda"), out_dtype=kind)[0] for v in (w, w.float()))
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("ptype", P16)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("channels,width", [(72, 4), (13, 3), (70, 2)])
+def test_conv_parameters_in_16_bits(cuda_device, ptype, dtype, channels, width):
+    """16-bit filters and biases are widened exactly: the bits of the same ones in fp32, which the other tests
+    hold against the oracle."""
+    conv = ops()[1]
+    r = maker(82)
+    x, w, bias = r(2, 37, channels, dtype=dtype).to("cuda"), r(channels, width).to(ptype).to("cuda"), r(channels).to(ptype).to("cuda")
+    state = r(2, width - 1, channels, dtype=dtype).to("cuda")
+
+    def work(w, bias):
+        out, fin = conv._short_conv_fwd(x, w, bias=bias, initial_states=state, return_final_states=True)
+        st = state.clone()
+        step = conv._short_conv_step(x[:, 0], st, w, bias=bias)
+        return [out, fin, step, st, *conv._short_conv_bwd(x, x, w, bias=bias, initial_states=state)]
+
+    for a, b in zip(work(w, bias), work(w.float(), bias.float())):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("ptype", P16)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,l,d,n,g", [(2, 40, 48, 16, 1), (1, 1500, 10, 5, 2), (1, 33, 24, 64, 1)])
+def test_scan_parameters_in_16_bits(cuda_device, ptype, dtype, b, l, d, n, g):
+    """A, D, dt_bias and the initial states in 16 bits: the bits of the same ones in fp32."""
+    scan = ops()[2]
+    inp = {k: v.to("cuda") for k, v in scan_inputs(b, l, d, n, g, dtype, 83).items()}
+    for k in ("A", "D", "dt_bias"):
+        inp[k] = inp[k].to(ptype)
+    init = maker(84)(b, d, n).to(ptype).to("cuda")
+    dout = maker(85)(b, l, d, dtype=dtype).to("cuda")
+
+    def work(wide):
+        f = (lambda t: t.float()) if wide else (lambda t: t)
+        pos = [inp["x"], inp["dt"], f(inp["A"]), inp["B"], inp["C"]]
+        kw = dict(D=f(inp["D"]), z=inp["z"], dt_bias=f(inp["dt_bias"]), dt_softplus=True)
+        out, fin, saved = scan._token_scan_fwd(*pos, for_backward=True, initial_states=f(init), **kw)
+        gr = scan._token_scan_bwd(dout, *pos, saved, initial_states=f(init), **kw)
+        st = init.float()
+        tok = scan._token_scan_step(st, inp["x"][:, 0], inp["dt"][:, 0], pos[2], inp["B"][:, 0], inp["C"][:, 0], D=kw["D"], z=inp["z"][:, 0],
+                                    dt_bias=kw["dt_bias"], dt_softplus=True)
+        return [out, fin, *gr, tok, st]
+
+    for a, c in zip(work(False), work(True)):
+        assert a.dtype == c.dtype and torch.equal(a, c)
+
+
+@pytest.mark.parametrize("ptype", P16)
+@pytest.mark.parametrize("headdim,n", [(64, 128), (8, 16), (33, 20)])
+def test_step_parameters_in_16_bits_per_head(cuda_device, ptype, headdim, n):
+    scan = ops()[2]
+    r = maker(86)
+    b, h = 3, 4
+    x, dt, B, C = (r(b, *s, dtype=torch.bfloat16).to("cuda") for s in ((h, headdim), (h,), (1, n), (1, n)))
+    A, D, bias = (-torch.rand(h, generator=torch.Generator().manual_seed(1))).to(ptype).to("cuda"), r(h).to(ptype).to("cuda"), r(h).to(ptype).to("cuda")
+    state = r(b, h, headdim, n).to("cuda")
+    outs = []
+    for f in (lambda t: t, lambda t: t.float()):
+        st = state.clone()
+        outs.append((scan._token_scan_step(st, x, dt, f(A), B, C, D=f(D), dt_bias=f(bias), dt_softplus=True), st))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_gradients_of_a_sequence_see_no_earlier_one(cuda_device):
+    """Packed sequences, the other way: an infinity or a NaN of an earlier sequence, and initial states that no position
+    sees, leave the bits of the later ones' gradients; scan and convolution, short rows and segments."""
+    _, conv, scan = ops()
+    r = maker(90)
+    for b, l, d, n, cut in ((2, 61, 20, 16, 33), (1, 1700, 24, 8, 801)):
+        inp = {k: v.to("cuda") for k, v in scan_inputs(b, l, d, n, 1, torch.float32, 91).items()}
+        seq = torch.zeros(b, l, dtype=torch.int32, device="cuda")
+        seq[:, cut:] = 1
+        inp |= dict(dout=r(b, l, d).to("cuda"), init=r(b, d, n).to("cuda"), cinit=r(b, 3, d).to("cuda"), w=r(d, 4).to("cuda"))
+
+        def work(v, seq):
+            kw = dict(D=v["D"], z=v["z"], dt_bias=v["dt_bias"], dt_softplus=True, initial_states=v["init"], seq_idx=seq)
+            pos = [v[k] for k in KEYS]
+            out, fin, saved = scan._token_scan_fwd(*pos, for_backward=True, **kw)
+            g = scan._token_scan_bwd(v["dout"], *pos, saved, **kw)
+            ckw = dict(bias=v["D"], initial_states=v["cinit"], seq_idx=seq)
+            c, cf = conv._short_conv_fwd(v["x"], v["w"], return_final_states=True, **ckw)
+            cg = conv._short_conv_bwd(v["dout"], v["x"], v["w"], dfinal_states=inp["cinit"], **ckw)
+            return [t[:, cut:] for t in (out, g[0], g[1], g[3], g[4], g[6], c, cg[0])] + [fin, cf], [g[2], g[5], g[7], g[8], cg[1], cg[2], cg[3]]
+
+        good, _ = work(inp, seq)
+        for bad in (float("nan"), float("inf")):
+            for key in ("x", "dt", "B", "C", "z", "dout", "init", "cinit"):
+                v = dict(inp)
+                v[key] = inp[key].clone()
+                v[key][:, :3] = bad
+                if key not in ("init", "cinit"):
+                    v[key][:, cut - 2:cut] = bad
+                for a, c in zip(work(v, seq)[0], good):
+                    assert torch.equal(a, c), (key, bad)
+        # rows that do not begin with sequence 0 see nothing of the initial states, and hand nothing back to them
+        v = dict(inp, init=torch.full_like(inp["init"], float("nan")), cinit=torch.full_like(inp["cinit"], float("nan")))
+        a, b_ = work(inp, seq + 1), work(v, seq + 1)
+        for p, q in zip((*a[0], *a[1]), (*b_[0], *b_[1])):
+            assert torch.equal(p, q)
+        assert (a[1][3] == 0).all() and (a[1][6] == 0).all()
+
+
+def test_scan_gradients_in_ranges_captured_and_on_another_stream(cuda_device):
+    """The launches of a problem that is walked in ranges as one graph, replayed with other inputs, beside an eager call
+    on another stream."""
+    scan = ops()[2]
+    b, l, d, n = 1, 300, 1024, 256
+
+    def inputs(seed):
+        v = {k: t.to("cuda") for k, t in scan_inputs(b, l, d, n, 1, torch.bfloat16, seed).items()}
+        v["dout"] = maker(seed + 1)(b, l, d, dtype=torch.bfloat16).to("cuda")
+        return v
+
+    def work(v):
+        pos = [v[k] for k in KEYS]
+        kw = dict(D=v["D"], z=v["z"], dt_bias=v["dt_bias"], dt_softplus=True)
+        _, _, saved = scan._token_scan_fwd(*pos, for_backward=True, **kw)
+        return [t for t in scan._token_scan_bwd(v["dout"], *pos, saved, **kw) if t is not None]
+
+    first, second = inputs(92), inputs(94)
+    want = [[t.clone() for t in work(v)] for v in (first, second)]
+    static, stream = {k: t.clone() for k, t in first.items()}, torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        work(static)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work(static)
+    for k, t in second.items():
+        static[k].copy_(t)
+    stream.wait_stream(torch.cuda.current_stream())
+    for _ in range(2):
+        graph.replay()
+        with torch.cuda.stream(stream):
+            eager = work(first)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(outs, want[1]))
+    assert all(torch.equal(a, c) for a, c in zip(eager, want[0]))
