@@ -13,7 +13,7 @@
 // pairs of components (packed fp32), which halves their issue slots.
 //
 // The threads that hold the states do nothing else; two more warps load, form dt' and apply D and the gate, a
-// tile ahead and a tile behind (594 to 443 us at 2 x 4096 x 5120 channels of 16).  Measured there: 367 us,
+// tile ahead and a tile behind (594 to 443 us at 2 x 4096 x 5120 channels of 16).  Measured there: 363 to 367 us,
 // against 186 us for its exponentials and 51 us for its bytes; issue slots, shared memory and exponentials are
 // each a little over half used, and 640 blocks on 148 SMs leave 14 % of them idle at the end.
 //

@@ -20,8 +20,9 @@
 // the last one first, and in parts of the batch; one range's shares are summed before the next one overwrites
 // them, and what it hands on waits in memory.
 //
-// Measured at 2 x 2048 x 5120 channels of 16, bf16: 880 us, bound by issue slots (62 %): about 50 instructions
-// for each position, channel and component, half of them the exchanges of the two kinds of sums.
+// Measured at 2 x 2048 x 5120 channels of 16, bf16: 915 us with the sum of the shares, bound by issue slots (63 %):
+// about 50 instructions for each position, channel and component, half of them the exchanges of the two kinds of
+// sums.  1 x 4096 x 2048 x 128, in eight ranges: 5.3 ms with the forward pass.
 #include "token_scan.cuh"
 
 namespace ssd {

@@ -1,6 +1,6 @@
 """Residual addition + root-mean-square norm, the step that opens every layer around the scan: forward with
-an output in x's type or in 8 bits with one scale a row, and the gradients.  The reference has no
-counterpart (its path begins behind a layer's input projection)."""
+an output in x's type or in 8 bits with one scale a row, and the gradients.  Plain calls: their results carry no
+autograd history.  The reference has no counterpart (its path begins behind a layer's input projection)."""
 from .._ext import C as _C
 
 
@@ -16,7 +16,9 @@ def _add_rms_norm_fwd(x, weight, residual=None, eps=1e-5, out_dtype=None, residu
     Returns (out, residual_out, rstd, scales).  residual_out is t in the residual's dtype (x's dtype or
     fp32), or in `residual_dtype` where there is no residual yet; None if neither is given.  rstd
     (rows..., fp32), of residual_out as it was kept, is for the gradients; scales (rows..., fp32) takes its
-    place where out is in 8 bits (the other of the two is None)."""
+    place where out is in 8 bits (the other of the two is None).
+
+    The squares are summed in fp32: |t| has to stay below about 1e19 / sqrt(dim)."""
     # the front end asserts the shapes: a token's call is short
     return _C.add_rms_norm_fwd(x, weight, residual, eps, out_dtype, residual_dtype)
 

@@ -1,6 +1,7 @@
 """Short causal convolution over the sequence, one filter of 2 to 4 taps for each channel: what stands
 between a layer's input projection and the scan (its channels are x, B and C side by side).  Prompts,
-gradients and single tokens.  The reference has no counterpart.
+gradients and single tokens, as plain calls (their results carry no autograd history).  The reference has no
+counterpart.
 
 The state of a sequence is its last width - 1 inputs, (width - 1, channels), oldest first."""
 from .._ext import C as _C

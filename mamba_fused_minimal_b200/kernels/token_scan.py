@@ -1,7 +1,7 @@
 """Selective scan, position by position, with a decay for each channel and state component; the chunk kernels
 of this package have one decay for each head.  Prompts, gradients, and single tokens; the single-token
 step takes both forms, so it also continues what the chunk kernels began (their final_states are its
-state).  The reference has no counterpart."""
+state).  Plain calls: their results carry no autograd history.  The reference has no counterpart."""
 from .._ext import C as _C
 
 
@@ -17,7 +17,8 @@ def _token_scan_fwd(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fa
     dropped where the sequence changes, and initial_states belong to sequence 0.  dt has x's dtype or fp32.
 
     Returns (out, final_states, saved): final_states (batch, channels, dstate) fp32, and with for_backward
-    what `_token_scan_bwd` needs, else None."""
+    what `_token_scan_bwd` needs, else None: the states before every 16th position and, with z, y before the
+    gate, in fp32 (dstate / 4 and 4 bytes for each position and channel)."""
     # the front end asserts the shapes
     out, final, checkpoints, out_x = _C.token_scan_fwd(x, dt, A, B, C, D, z, dt_bias, dt_softplus, dt_limit[0], dt_limit[1],
                                                        initial_states, seq_idx, for_backward)
@@ -28,7 +29,8 @@ def _token_scan_bwd(dout, x, dt, A, B, C, saved, D=None, z=None, dt_bias=None, d
                     initial_states=None, seq_idx=None, dfinal_states=None):
     """Gradients of `_token_scan_fwd`, called with the same inputs and with what it saved.  Returns (dx, ddt, dA,
     dB, dC, dD, dz, ddt_bias, dinitial_states): dA, dD, ddt_bias and dinitial_states in fp32, the others in
-    their input's dtype; None for what was not given.  The same inputs give the same bits."""
+    their input's dtype; None for what was not given.  The same inputs give the same bits.  Scratch: up to 512 MB
+    and a few times the states (or 16 positions' shares of dB and dC, where those are more)."""
     checkpoints, out_x = saved
     return _C.token_scan_bwd(dout, x, dt, A, B, C, checkpoints, out_x, D, z, dt_bias, dt_softplus, dt_limit[0], dt_limit[1],
                              initial_states, seq_idx, dfinal_states)
