@@ -525,10 +525,10 @@ BwdPlan plan_bwd(const ssd_token_scan_params_t& p) {
   const int64_t fit = 2 * kSMs, blocks = (int64_t)p.ngroups * bwd_tiles(p);      // of one batch element
   const int64_t bytes = blocks * 2 * p.dstate * sizeof(float);                  // and one position
   if (bytes > kShares / ((int64_t)p.batch * p.seqlen)) {
-    // batch elements side by side as long as they are needed for four waves of blocks, then as many positions as
-    // there is room for, evenly
-    const int64_t want = (4 * fit + blocks - 1) / blocks;
-    const int64_t parts = (p.batch + (want < p.batch ? want : p.batch) - 1) / (want < p.batch ? want : p.batch);
+    // as many batch elements side by side as leave room for 256 positions, so that a launch has many waves of blocks
+    // and a block many tiles, then as many positions as there is room for; both evenly
+    const int64_t room = kShares / (bytes * 256), most = room < 1 ? 1 : room < p.batch ? room : p.batch;
+    const int64_t parts = (p.batch + most - 1) / most;
     s.batch = (int)((p.batch + parts - 1) / parts);
     int64_t len = kShares / (bytes * s.batch) / kT * kT;
     if (len < kT) len = kT;
