@@ -5,7 +5,7 @@
 //
 // Both directions move every element once and compute little: the bound is memory bandwidth.  A block
 // holds a row in registers between the sum over it and the writing, so nothing is read twice.  Measured:
-// 32768 x 2560 bf16 with residual to e4m3 105 to 109 us (5.4 to 5.6 TB/s of 6.5 for a copy; 115 with a weight in bf16,
+// 32768 x 2560 bf16 with residual to e4m3 104 to 109 us (5.4 to 5.6 TB/s of 6.5 for a copy; 115 with a weight in bf16,
 // which is read element by element), 8188 x 4096 with an fp32 residual forward and gradients 164 to 166 us (5.7 TB/s).
 // Gradients of longer rows do not fit the registers of a block that size and spill: 4092 x 8192 205 us, floor 143.
 #include "layer_common.cuh"

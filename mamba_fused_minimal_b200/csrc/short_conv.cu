@@ -7,8 +7,8 @@
 // Every element is read and written once: the bound is memory bandwidth.  Channels are contiguous, so a
 // thread owns a vector of channels and walks a strip of positions with the last width - 1 inputs in
 // registers; only a strip's first width - 1 positions are read twice.  Measured: 8 x 4096 x 5376 bf16 out of a
-// wider buffer 150 us (4.7 TB/s of 6.5 for a copy): the loads in flight are held in registers, 96 a thread, which
-// leaves 20 warps an SM; packed 3 x 2049 x 1792 gradients 41 us, bound by issue (66 %).
+// wider buffer 144 to 152 us (4.6 to 4.9 TB/s of 6.5 for a copy): the loads in flight are held in registers, 96 a
+// thread, which leaves 20 warps an SM; packed 3 x 2049 x 1792 gradients 41 us, bound by issue (66 %).
 #include "layer_common.cuh"
 
 namespace ssd {

@@ -7,7 +7,7 @@
 // as 16-byte vectors, and all loads of a thread's U rows are issued before the first is used, none of them
 // under a condition that would be waited for.  With one decay a head (the Mamba2 form) a block stays
 // inside a head and forms dt' and the decay once; with a decay for each component every row has its own.
-// Measured: 128 sequences of 80 heads of 64 x 128 in fp32 126 to 129 us (5.3 TB/s of 6.5 for a copy), one sequence of
+// Measured: 128 sequences of 80 heads of 64 x 128 in fp32 125 to 129 us (5.2 to 5.4 TB/s of 6.5 for a copy), one sequence of
 // 1536 channels of 16 6.3 us replayed.
 #include "layer_common.cuh"
 
